@@ -1,0 +1,84 @@
+// Moments of an optimizer in 8 bits (device helpers of adamw.hip).
+//
+// Blocks of 256 consecutive elements share one exponent byte E, the biased float32 exponent of the block's largest
+// magnitude.  A value's code counts the steps of its "key" (float32 bit pattern >> 20: exponent and three mantissa
+// bits) above the block's base:
+//   second moment: code 1..255 <-> key base + code, base = max(0, 8 (E + 1) - 255)         31.75 powers of two
+//   first moment:  sign and code 1..127,            base = max(0, 8 (E + 1) - 127)         15.75 powers of two
+// Code 0 is zero.  Because the grid is a cut of the float32 pattern, its points do not move when a block's exponent
+// does: a value that is stored, read and stored again stays what it is.  The largest code stands for 2^(E + 1 - 127),
+// so a largest value that rounds up has a place.
+//
+// The cut is stochastic (a 16-bit random number is added just below the last kept bit).  With beta2 = 0.999 a step
+// moves v by a thousandth of g^2 - v while the grid's points are an eighth to a sixteenth of v apart: a cut to the
+// nearest would leave v where it is for good, and on average the cut that is drawn keeps the change.  16 random bits and
+// not 8, because that change is about a hundredth of the grid's spacing.  The spread that the draws leave in v is about
+// 0.2 v (each step adds 0.09 v * 0.001 |g^2 - v| to the variance, and 1 / (1 - beta2^2) = 500 steps are remembered),
+// 0.1 of its root.  v has 3 mantissa bits and 5 of exponent, because its root's range beside eps (2^16 in a block)
+// matters more than the third of that spread that a fourth mantissa bit would take away.
+// A second moment that is not zero never gets code 0: its root divides.  What a first moment loses below its smallest
+// code is 2^-16 of the block's largest.  A block with a value that is not finite gets E = 255 and stands for NaN.
+#pragma once
+#include "fdgs_common.h"
+
+#define M8_BLOCK 256
+
+// 32 bits from an element's index and a tensor's key of the step.  Three odd multipliers from the fractions of the
+// golden ratio and of the roots of 2 and 3, with shifts in between that bring the high bits back down.
+__device__ __forceinline__ uint32_t m8_hash(uint32_t index_lo, uint32_t key_and_hi) {
+    uint32_t x = index_lo + key_and_hi;
+    x *= 0x9E3779B9u;
+    x ^= x >> 16;
+    x *= 0x6A09E667u;
+    x ^= x >> 15;
+    x *= 0xBB67AE85u;
+    return x ^ (x >> 16);
+}
+// the part of the hash that is the same for 2^32 elements
+__device__ __forceinline__ uint32_t m8_key(uint32_t key, long long index) {
+    return key + (uint32_t)((unsigned long long)index >> 32) * 0x6A09E667u;
+}
+
+// What the two fields of the hash add below the kept bits.
+__device__ __forceinline__ uint32_t m8_noise_m(uint32_t h) { return (h >> 12) & 0xFFFF0u; }
+__device__ __forceinline__ uint32_t m8_noise_v(uint32_t h) { return (h << 4) & 0xFFFF0u; }
+
+template <bool SIGNED>
+__device__ __forceinline__ int m8_base(int e) {
+    const int b = 8 * (e + 1) - (SIGNED ? 127 : 255);
+    return b > 0 ? b : 0;
+}
+
+template <bool SIGNED>
+__device__ __forceinline__ float m8_decode(uint32_t code, int e, int base) {
+    const uint32_t size = SIGNED ? (code & 127u) : code;
+    uint32_t bits = size ? (size + (uint32_t)base) << 20 : 0u;
+    if (SIGNED) bits |= (code & 128u) << 24;
+    return __uint_as_float(e == 255 ? 0x7FC00000u : bits);
+}
+
+template <bool SIGNED>
+__device__ __forceinline__ uint32_t m8_encode(float x, uint32_t noise, int e, int base) {
+    const uint32_t all = __float_as_uint(x), bits = all & 0x7FFFFFFFu;
+    int code = (int)((bits + noise) >> 20) - base;
+    if (SIGNED) {
+        code = code > 0 ? code : 0;
+        code |= (int)(all >> 24) & 128;
+    } else {
+        const int least = bits ? 1 : 0;
+        code = code > least ? code : least;
+    }
+    return e == 255 ? 0u : (uint32_t)code;
+}
+
+typedef unsigned short m8_u16x2 __attribute__((ext_vector_type(2)));
+// Largest of two 16-bit fields over a wave, in every lane: the exponents of both moments in one reduction.
+__device__ __forceinline__ uint32_t m8_wave_max2(uint32_t v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        const uint32_t w = (uint32_t)__shfl_xor((int)v, o);
+        const m8_u16x2 a = __builtin_bit_cast(m8_u16x2, v), b = __builtin_bit_cast(m8_u16x2, w);
+        v = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(a, b));
+    }
+    return v;
+}

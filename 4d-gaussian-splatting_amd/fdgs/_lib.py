@@ -9,6 +9,8 @@ import os
 
 import torch
 
+from . import _records
+
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("FDGS_LIBRARY") or os.path.join(_HERE, "libfdgs.so")   # override: a build of the same ABI
 
@@ -228,6 +230,12 @@ SYMBOLS = {
     "fdgs_ssim_fwd": (C.c_int, [C.POINTER(SsimFwdArgs), c_p]),
     "fdgs_ssim_bwd": (C.c_int, [C.POINTER(SsimBwdArgs), c_p]),
     "fdgs_deform_bwd": (C.c_int, [C.POINTER(DeformBwdArgs), c_p]),
+    "fdgs_adamw_step": (C.c_int, [C.POINTER(_records.AdamWArgs), c_p]),
+    "fdgs_moment8_unpack": (C.c_int, [C.POINTER(_records.Moment8Args), c_p]),
+    "fdgs_embedding_fwd": (C.c_int, [C.POINTER(_records.EmbeddingFwdArgs), c_p]),
+    "fdgs_embedding_bwd_workspace_bytes": (c_sz, [c_i64, c_i32, c_i32, c_i32]),
+    "fdgs_embedding_bwd": (C.c_int, [C.POINTER(_records.EmbeddingBwdArgs), c_p]),
+    "fdgs_moment8_pack": (C.c_int, [C.POINTER(_records.Moment8Args), c_p]),
 }
 
 BINSORT_ALL, BINSORT_COUNT, BINSORT_FINISH = 0, 1, 2      # fdgs_binsort_args.phase
@@ -279,6 +287,15 @@ def call(name, args):
         e.record()
         PROFILE.setdefault(name, []).append((s, e))
     check(rc, name)
+
+
+def call_on(device, name, args):
+    """call() with `device` as the current one: the stream is then a stream of the device the tensors are on."""
+    if device.index == torch.cuda.current_device():
+        call(name, args)
+    else:
+        with torch.cuda.device(device):
+            call(name, args)
 
 
 def ptr(t):

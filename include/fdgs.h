@@ -472,6 +472,112 @@ typedef struct {
 
 int fdgs_adam_step(const fdgs_adam_args* a, void* stream);
 
+/* ---- AdamW over many tensors, moments in float32 or in 8 bits ------------------------------------
+ * One step of torch.optim.AdamW (decoupled weight decay, no amsgrad) over any number of tensors:
+ *   m = beta1 m + (1-beta1) g;  v = beta2 v + (1-beta2) g^2;
+ *   p = (1 - lr weight_decay) p - lr/(1-beta1^step) * m / (sqrt(v)/sqrt(1-beta2^step) + eps)
+ * formed in float32 without contraction, so that equal inputs give equal bits.
+ *
+ * param_type FDGS_TYPE_BF16: the parameter and the gradient are bfloat16, and `residual` holds, per element, the signed
+ * 16 bits by which the float32 weight's bit pattern lies beside the bfloat16 one's ((param << 16) + residual is the
+ * weight): updates smaller than a bfloat16 step add up.  Zeros to begin with.
+ *
+ * state_bits 8: exp_avg / exp_avg_sq are one byte per element and each has one exponent byte per block of
+ * FDGS_MOMENT8_BLOCK consecutive elements.  With E the block's exponent byte (the biased float32 exponent of its largest
+ * magnitude) a code c > 0 stands for the float32 with bit pattern (c + max(0, 8 (E+1) - 255)) << 20 in the second
+ * moment, for sign (bit 7) and ((c & 127) + max(0, 8 (E+1) - 127)) << 20 in the first; c = 0 is zero, E = 255 makes the
+ * whole block NaN (it was given a value that is not finite).  All zeros to begin with.  Values are rounded
+ * stochastically, by 16 bits each of a hash of the element's index and `round_key`: give every tensor and step a key of
+ * its own, and every replica the same one.  A second moment that is not zero is never rounded to zero.
+ *
+ * The tensors must not overlap, and not two records may name the same one.                          */
+#define FDGS_TYPE_F32 0
+#define FDGS_TYPE_BF16 1
+#define FDGS_TYPE_F16 2
+#define FDGS_MOMENT8_BLOCK 256
+typedef struct {
+    void* param;                     /* [numel] float32 or bfloat16, updated            */
+    const void* grad;                /* [numel], the parameter's type                   */
+    void* exp_avg;                   /* [numel] float32, or bytes with state_bits 8     */
+    void* exp_avg_sq;
+    int16_t* residual;               /* [numel], bfloat16 parameters only               */
+    uint8_t* exp_avg_exponents;      /* [ceil(numel / FDGS_MOMENT8_BLOCK)], state_bits 8 only */
+    uint8_t* exp_avg_sq_exponents;
+    int64_t numel;
+    int64_t grad_row_stride;         /* as in fdgs_adam_args                            */
+    int32_t grad_row_len;
+    int32_t step;                    /* 1-based, the tensor's own count                 */
+    double lr, weight_decay;
+    uint32_t round_key;
+    uint32_t reserved;
+} fdgs_adamw_tensor;
+typedef struct {
+    int32_t num_tensors;
+    int32_t param_type;              /* FDGS_TYPE_F32 or FDGS_TYPE_BF16                 */
+    int32_t state_bits;              /* 32 or 8                                         */
+    int32_t reserved;
+    double beta1, beta2, eps;
+    const fdgs_adamw_tensor* tensors;   /* HOST array, read before the call returns    */
+} fdgs_adamw_args;
+int fdgs_adamw_step(const fdgs_adamw_args* a, void* stream);
+
+/* 8-bit moments to the values they stand for (value_type float32 or bfloat16, both exact), and float32 values to
+ * 8-bit moments: to the nearest (nearest = 1; halves up) or with round_key's random numbers.          */
+typedef struct {
+    uint8_t* codes;                  /* [numel]                                         */
+    uint8_t* exponents;              /* [ceil(numel / FDGS_MOMENT8_BLOCK)]              */
+    void* value;                     /* [numel]                                         */
+    int64_t numel;
+    int32_t is_signed;               /* 1: a first moment's codes, 0: a second's (the sign of its values is dropped) */
+    uint32_t round_key;
+} fdgs_moment8_tensor;
+typedef struct {
+    int32_t num_tensors;
+    int32_t value_type;
+    int32_t nearest;
+    int32_t reserved;
+    const fdgs_moment8_tensor* tensors; /* HOST array, read before the call returns    */
+} fdgs_moment8_args;
+int fdgs_moment8_unpack(const fdgs_moment8_args* a, void* stream);
+int fdgs_moment8_pack(const fdgs_moment8_args* a, void* stream);
+
+/* ---- table lookup with scaling, and its gradient -------------------------------------------------
+ *   out[i, :] = scale * table[ids[i], :]            for the tokens i
+ *   grad_table[r, :] = scale * sum_{i : ids[i] = r} grad_out[i, :]   for every row r; rows no token asks for get zeros
+ * in float32, rounded once to `type` (FDGS_TYPE_F32 / BF16 / F16: table, out and both gradients).  The sums are taken
+ * in an order that the ids alone decide (no atomics): equal inputs give equal bits.
+ * A token has no row - zeros in out, nothing in the gradient - when its id is negative or padding_id; an id of num_rows
+ * or more gives a row of NaN, and nothing in the gradient.                                            */
+#define FDGS_EMBEDDING_MAX_TOKENS (1 << 30)          /* of the gradient; the lookup takes 2^31 - 1 */
+typedef struct {
+    int64_t num_tokens;
+    int32_t num_rows, dim;
+    int32_t type;
+    int32_t id_bytes;                /* 4 (int32) or 8 (int64)                          */
+    const void* ids;                 /* [num_tokens]                                    */
+    const void* table;               /* [num_rows, dim], rows table_row_stride elements apart */
+    int64_t table_row_stride;
+    int64_t padding_id;              /* -1: none                                        */
+    void* out;                       /* [num_tokens, dim]                               */
+    float scale;
+} fdgs_embedding_fwd_args;
+typedef struct {
+    int64_t num_tokens;
+    int32_t num_rows, dim;
+    int32_t type;
+    int32_t id_bytes;
+    const void* ids;
+    const void* grad_out;            /* [num_tokens, dim], rows grad_out_row_stride elements apart (0: one row for all) */
+    int64_t grad_out_row_stride;
+    int64_t padding_id;
+    void* grad_table;                /* [num_rows, dim] out                             */
+    float scale;
+    void* workspace; size_t workspace_bytes;   /* fdgs_embedding_bwd_workspace_bytes(...) */
+} fdgs_embedding_bwd_args;
+int fdgs_embedding_fwd(const fdgs_embedding_fwd_args* a, void* stream);
+size_t fdgs_embedding_bwd_workspace_bytes(int64_t num_tokens, int32_t num_rows, int32_t dim, int32_t type);
+int fdgs_embedding_bwd(const fdgs_embedding_bwd_args* a, void* stream);
+
 /* ---- densification / pruning surgery ------------------------------------------------------------
  * The reference grows and shrinks the six per-Gaussian parameter tensors, their Adam moments and the
  * per-Gaussian statistics with chains of boolean-mask indexing and torch.cat

@@ -1,0 +1,339 @@
+"""GPU: fdgs_adamw_step and the 8-bit moments' conversions against the formula in 64 bits and the format in integers.
+
+Tolerances count roundings (u = 2^-24, half a float32 step): of m three on each of its two terms, of v four, of the
+update twelve beside what m is off by, of the weight four (constant, product, difference, and one to spare)."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import adamw_cases as ac
+
+pytestmark = pytest.mark.gpu
+U = ac.U
+
+
+def _inputs(sizes, seed, spread=4.0):
+    rng = np.random.default_rng(seed)
+    out = []
+    for n in sizes:
+        scale = 10.0 ** rng.uniform(-spread, 0)
+        g = (rng.standard_normal(n) * scale).astype(np.float32)
+        g[rng.random(n) < 0.2] = 0.0
+        m = (0.3 * g + 0.1 * scale * rng.standard_normal(n)).astype(np.float32)
+        v = ((scale * rng.random(n)) ** 2).astype(np.float32)
+        v[rng.random(n) < 0.1] = 0.0
+        w = (0.1 * rng.standard_normal(n)).astype(np.float32)
+        out.append((w, g, m, v))
+    return out
+
+
+def _bf16(x):
+    return torch.from_numpy(np.ascontiguousarray(x)).to(torch.bfloat16)
+
+
+class Arena:
+    """Tensors cut from one array, `skew` elements off its alignment, with a marked gap between them."""
+
+    def __init__(self, arrays, dtype, skew, mark):
+        at, self.at = skew, []
+        for a in arrays:
+            self.at.append(at)
+            at += len(a) + 3
+        self.flat = torch.full((at + 5,), mark, dtype=dtype)
+        for o, a in zip(self.at, arrays):
+            self.flat[o:o + len(a)] = torch.as_tensor(a).to(dtype)
+        self.flat = self.flat.cuda()
+        self.views = [self.flat[o:o + len(a)] for o, a in zip(self.at, arrays)]
+        self.before = self.flat.clone()
+
+    def gaps_untouched(self):
+        inside = torch.zeros(self.flat.numel(), dtype=torch.bool)
+        for o, v in zip(self.at, self.views):
+            inside[o:o + v.numel()] = True
+        return torch.equal(self.flat.cpu()[~inside], self.before.cpu()[~inside])
+
+
+SIZES = [1, 3, 4, 63, 255, 256, 257, 511, 512, 513, 2047, 2048, 2049, 5001, 0, 70001]
+
+
+def _within(got, want, tol, what):
+    err = np.abs(got.astype(np.float64) - want)
+    assert (err <= tol).all(), (what, float((err - tol).max()), int((err > tol).sum()))
+
+
+@pytest.mark.parametrize("skew", [0, 1, 2, 3])
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_step_against_the_formula(dtype, bits, skew):
+    from fdgs import adamw
+    b1, b2, eps = 0.9, 0.999, 1e-8
+    data = _inputs(SIZES, 17 * skew + bits)
+    bf16 = dtype is torch.bfloat16
+    lrs = [1e-3 * (1 + i % 3) for i in range(len(data))]
+    wds = [0.0 if i % 4 == 0 else 0.1 for i in range(len(data))]
+    steps = [1 + 7 * i for i in range(len(data))]
+    keys = [adamw.round_key(5, i, s) for i, s in enumerate(steps)]
+    g_in = [(_bf16(d[1]).float().numpy() if bf16 else d[1]) for d in data]
+    low = Arena([ac.split_bf16(d[0])[1] for d in data], torch.int16, skew, 77) if bf16 else None
+    if bf16:
+        p = Arena([np.zeros(len(d[0])) for d in data], dtype, skew, 9.0)
+        for view, d in zip(p.views, data):
+            view.copy_(torch.from_numpy(ac.split_bf16(d[0])[0].view(np.int16).copy()).view(torch.bfloat16).cuda())
+    else:
+        p = Arena([d[0] for d in data], dtype, skew, 9.0)
+    g = Arena(g_in, dtype, skew, float("nan"))
+    if bits == 32:
+        m = Arena([d[2] for d in data], torch.float32, skew, 9.0)
+        v = Arena([d[3] for d in data], torch.float32, skew, 9.0)
+        old = [(d[2], d[3]) for d in data]
+        adamw.adamw_step(p.views, g.views, m.views, v.views, steps=steps, lr=lrs, betas=(b1, b2), eps=eps, weight_decay=wds,
+                         residuals=low.views if bf16 else None)
+        new = [(a.cpu().numpy(), b.cpu().numpy()) for a, b in zip(m.views, v.views)]
+        states = [m, v]
+    else:
+        em, ev = ([ac.encode(d[k], 0x8000, k == 2) for d in data] for k in (2, 3))
+        old = [(ac.decode(*a, True), ac.decode(*b, False)) for a, b in zip(em, ev)]
+        mc, vc = (Arena([x[0] for x in e], torch.uint8, skew, 201) for e in (em, ev))
+        me, ve = (Arena([x[1] for x in e], torch.uint8, skew, 201) for e in (em, ev))
+        adamw.adamw_step(p.views, g.views, [adamw.Moment8(a, b, True) for a, b in zip(mc.views, me.views)],
+                         [adamw.Moment8(a, b, False) for a, b in zip(vc.views, ve.views)], steps=steps, lr=lrs, betas=(b1, b2),
+                         eps=eps, weight_decay=wds, residuals=low.views if bf16 else None, keys=keys)
+        states = [mc, vc, me, ve]
+    for i, (d, (m0, v0)) in enumerate(zip(data, old)):
+        w64, m64, v64 = ac.adamw64(d[0], g_in[i], m0, v0, steps[i], lrs[i], wds[i], b1, b2, eps)
+        mtol = 3.03 * U * (b1 * np.abs(m0) + (1 - b1) * np.abs(g_in[i])) + 2.0 ** -149
+        vtol = 4.04 * U * v64 + 2.0 ** -147
+        if bits == 32:
+            _within(new[i][0], m64, mtol, "m")
+            _within(new[i][1], v64, vtol, "v")
+        else:       # the codes are those of the format, bit by bit
+            m32, v32 = ac.adamw32(g_in[i], m0, v0, b1, b2)
+            h = ac.hash32(np.arange(len(m32)), keys[i])
+            for got, e, want in ((mc, me, ac.encode(m32, h >> 16, True)), (vc, ve, ac.encode(v32, h & 0xFFFF, False))):
+                assert np.array_equal(got.views[i].cpu().numpy(), want[0]) and np.array_equal(e.views[i].cpu().numpy(), want[1])
+        if bf16:
+            bits_p = p.views[i].cpu().view(torch.int16).numpy().astype(np.int64)
+            w = ((bits_p << 16) + low.views[i].cpu().numpy()).astype(np.int32).view(np.float32)
+            off = np.abs(w.astype(np.float64) - p.views[i].cpu().float().numpy())
+            assert (off <= 2.0 ** -8 * np.abs(w) * (1 + 2.0 ** -8) + 2.0 ** -134).all()     # the parameter is the nearest one
+        else:
+            w = p.views[i].cpu().numpy()
+        lr, bc1, bc2 = lrs[i], 1 - b1 ** steps[i], 1 - b2 ** steps[i]
+        denom = np.sqrt(v64 / bc2) + eps
+        update = np.abs(lr / bc1 * m64 / denom)
+        tol = 12.2 * U * update + 1.01 * lr / bc1 * mtol / denom + 4.04 * U * np.abs(d[0]) + 2.0 ** -149
+        # where v is below the normal numbers its own roundings count for more than u
+        tol += update * np.where(v64 > 0, 2.0 ** -147 / np.maximum(v64, 2.0 ** -149), 0.0)
+        _within(w, w64, tol, "w")
+    for a in [p] + ([low] if bf16 else []) + states:
+        assert a.gaps_untouched()
+    assert torch.equal(g.flat.cpu().isnan(), g.before.cpu().isnan())
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_gradients_as_column_slices_and_other_orders(bits):
+    """Gradients read from the columns of a wider array, expanded from one row or in another order give the bits that
+    a contiguous copy gives."""
+    from fdgs import adamw
+    gen = torch.Generator().manual_seed(3)
+    n = 1037
+    wide = torch.randn(n, 48, generator=gen).cuda()
+    grads = [wide[:, :3], wide[:, 3:], wide[:, 7:8], wide.t()[:5], wide[:1, :8].expand(n, 8), wide[::2, 5:9]]
+
+    def run(copy):
+        ps = [torch.linspace(-1, 1, g.numel(), device="cuda").view(g.shape) for g in grads]
+        make = (lambda p, s: adamw.Moment8.zeros_like(p, s)) if bits == 8 else (lambda p, s: torch.zeros_like(p))
+        ms, vs = [make(p, True) for p in ps], [make(p, False) for p in ps]
+        for t in (1, 2):
+            adamw.adamw_step(ps, [g.contiguous() if copy else g for g in grads], ms, vs, steps=t, lr=1e-2,
+                             keys=[adamw.round_key(1, i, t) for i in range(len(ps))] if bits == 8 else None)
+        return ps + [x for s in ms + vs for x in ((s.codes, s.exponents) if bits == 8 else (s,))]
+    for a, b in zip(run(True), run(False)):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("signed", [True, False])
+def test_pack_and_unpack(signed):
+    from fdgs import adamw
+    rng = np.random.default_rng(8)
+    arrays = []
+    for n in (1, 255, 256, 257, 4099):
+        x = (rng.standard_normal(n) * 10.0 ** rng.uniform(-12, 2, n)).astype(np.float32)
+        arrays.append(np.where(rng.random(n) < 0.2, np.float32(0), x if signed else np.abs(x)).astype(np.float32))
+    arrays.append(np.zeros(300, np.float32))
+    arrays.append((rng.random(700) * 2.0 ** -140).astype(np.float32))            # below the normal numbers
+    arrays.append(np.full(256, np.float32(1.9999999)))                           # rounds up into the next power of two
+    arrays.append(np.where(np.arange(512) == 5, np.float32("inf"), np.float32(1)).astype(np.float32))
+    arrays.append(np.where(np.arange(512) == 300, np.float32("nan"), np.float32(1)).astype(np.float32))
+    arrays.append(np.full(256, np.float32(3e38)))
+    dev = [torch.from_numpy(a).cuda() for a in arrays]
+    keys = [adamw.round_key(2, i, 1) for i in range(len(arrays))]
+    for ks in (None, keys):
+        packed = adamw.pack8(dev, signed, ks)
+        for i, (a, p) in enumerate(zip(arrays, packed)):
+            h = ac.hash32(np.arange(a.size), keys[i])
+            noise = 0x8000 if ks is None else (h >> 16 if signed else h & 0xFFFF)
+            code, e = ac.encode(a, noise, signed)
+            assert np.array_equal(p.codes.cpu().numpy(), code) and np.array_equal(p.exponents.cpu().numpy(), e), i
+        values = adamw.unpack8(packed)
+        halves = adamw.unpack8(packed, torch.bfloat16)
+        for a, p, x, y in zip(arrays, packed, values, halves):
+            want = ac.decode(p.codes.cpu().numpy(), p.exponents.cpu().numpy(), signed)
+            assert np.array_equal(x.cpu().numpy(), want, equal_nan=True)
+            assert np.array_equal(y.float().cpu().numpy(), want, equal_nan=True)           # bfloat16 holds them exactly
+            ok = np.repeat(p.exponents.cpu().numpy() != 255, 256)[:a.size]
+            a64, x64 = np.abs(a[ok].astype(np.float64)), np.abs(want[ok].astype(np.float64))
+            if not signed:
+                assert ((a64 > 0) == (x64 > 0)).all()          # a second moment that is not zero stays so
+            # within one step of the grid (half of one to the nearest): an eighth of the power of two, the block's
+            # largest times 2^-15 or 2^-31 at the small end
+            top = np.repeat(2.0 ** (p.exponents.cpu().numpy().astype(np.float64) - 126), 256)[:a.size][ok]
+            low = np.maximum(top * 2.0 ** (-15.6 if signed else -31.6), 2.0 ** -128.9)
+            step = np.where(a64 > 0, 2.0 ** (np.floor(np.log2(np.maximum(a64, 2.0 ** -149))) - 3), 0)
+            limit = (0.5 if ks is None else 1.0) * np.maximum(step, 2.0 ** -129)
+            far = np.abs(a64 - x64) > limit * (1 + 2.0 ** -15)
+            assert (~far | (a64 <= low)).all() and (np.abs(a64 - x64)[far] <= low[far]).all()
+        again = adamw.pack8(values, signed)                    # what is on the grid stays where it is
+        for x, p, q in zip(values, packed, again):             # (but for the smallest, where the largest has rounded up)
+            same, x = adamw.unpack8([q])[0].cpu().numpy(), x.cpu().numpy()
+            top = np.repeat(2.0 ** (q.exponents.cpu().numpy().astype(np.float64) - 126), 256)[:x.size]
+            there = ~(np.abs(x) < top * 2.0 ** (-14.6 if signed else -30.6))
+            assert np.array_equal(same[there], x[there], equal_nan=True)
+
+
+def test_rounding_keeps_the_mean():
+    """A value between two codes is stored as either, with the mean of what it is: 2^18 elements, five standard
+    deviations of the mean of so many draws plus what 16 random bits cannot resolve."""
+    from fdgs import adamw
+    n = 1 << 18
+    for x in (1.0009, 1.05, 1.1, 1.9):
+        values = torch.full((n,), x, device="cuda")
+        for signed in (True, False):
+            mean = float(adamw.unpack8(adamw.pack8([values], signed, [adamw.round_key(9, 0, 3)]))[0].double().mean())
+            f = (np.float32(x) - 1.0) * 8 % 1
+            sigma = 0.125 * math.sqrt(f * (1 - f) / n)
+            assert abs(mean - float(np.float32(x))) <= 5 * sigma + 0.125 * 2.0 ** -16, (x, signed, mean)
+
+
+def test_second_moment_follows_a_falling_gradient():
+    """With beta2 = 0.999 a moment cut to the nearest code would stay where it is; the drawn cut follows.  v falls as
+    0.999^k; after 2000 steps without gradient the mean over 2^16 elements is 0.135 of the start.  A step that moves v by
+    d between points s apart has a variance of at most s d <= (v / 8) (0.001 v), so the variance relative to the mean
+    squared, r, grows by at most 1.25e-4 (1 + r) a step, to e^0.25 - 1 = 0.284: five deviations of the mean of 65536 are
+    1.04 percent.  16 random bits are off by 2^-16 of s a step, the float32 products by 2 u a step."""
+    from fdgs import adamw
+    n, k = 1 << 16, 2000
+    p, g = torch.zeros(n, device="cuda"), torch.zeros(n, device="cuda")
+    m = adamw.Moment8.zeros_like(p, True)
+    v, = adamw.pack8([torch.full((n,), 0.37, device="cuda")], False)
+    start = float(adamw.unpack8([v])[0][0])
+    for t in range(1, k + 1):
+        adamw.adamw_step([p], [g], [m], [v], steps=t, lr=0.0, keys=[adamw.round_key(4, 0, t)])
+    mean = float(adamw.unpack8([v])[0].double().mean())
+    assert abs(mean / (start * 0.999 ** k) - 1) <= 0.0104 + k * 2.0 ** -16 * 0.125 + 2 * k * U
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_what_is_not_finite_stays_where_it_is(bits):
+    """A NaN or infinite gradient makes its own element NaN, and with 8-bit moments its block of 256 from the next step on;
+    every other element keeps the bits it would have had."""
+    from fdgs import adamw
+    n = 1024
+    gen = torch.Generator().manual_seed(6)
+    g = torch.randn(n, generator=gen).cuda()
+    bad = g.clone()
+    bad[300], bad[301] = float("nan"), float("inf")
+
+    def run(grad):
+        p = torch.ones(n, device="cuda")
+        m = adamw.Moment8.zeros_like(p, True) if bits == 8 else torch.zeros(n, device="cuda")
+        v = adamw.Moment8.zeros_like(p, False) if bits == 8 else torch.zeros(n, device="cuda")
+        for t in (1, 2):
+            adamw.adamw_step([p], [grad if t == 1 else g], [m], [v], steps=t, lr=0.1, keys=[t] if bits == 8 else None)
+        return p.cpu(), [x.cpu() for x in (adamw.unpack8([m, v]) if bits == 8 else (m, v))]
+    pa, sa = run(g)
+    pb, sb = run(bad)
+    hit = torch.zeros(n, dtype=torch.bool)
+    hit[256:512 if bits == 8 else 256] = True
+    hit[300] = hit[301] = True
+    assert torch.equal(pa[~hit], pb[~hit]) and pb[hit].isnan().all()
+    for a, b in zip(sa, sb):
+        assert torch.equal(a[~hit], b[~hit])
+    assert sb[0][hit].isnan().all() if bits == 8 else not sb[0][hit].isfinite().any()
+
+
+def test_bfloat16_weights_gather_small_updates():
+    """1000 steps of 1e-5 on weights of 1, where bfloat16's step is 2^-7: the parameter follows the float32 weight."""
+    from fdgs import adamw
+    n = 513
+    p = torch.ones(n, device="cuda", dtype=torch.bfloat16)
+    low = torch.zeros(n, device="cuda", dtype=torch.int16)
+    g = torch.ones(n, device="cuda", dtype=torch.bfloat16)
+    m, v = torch.zeros(n, device="cuda"), torch.zeros(n, device="cuda")
+    for t in range(1, 1001):
+        adamw.adamw_step([p], [g], [m], [v], steps=t, lr=1e-5, weight_decay=0.0, residuals=[low])
+    w = ((p.view(torch.int16).to(torch.int32) << 16) + low.to(torch.int32)).view(torch.float32).cpu().double()
+    # a step moves by 1e-5 and rounds the weight, which lies between a half and one, by u / 2; the moments gather 3 u a
+    # step for ten steps and 4 u a step for a thousand, half of which the root keeps: 2050 u of each update; eps 1e-8 of it
+    assert (w - (1 - 1e-2)).abs().max() <= 1000 * (0.5 * U + 1e-5 * (2050 * U + 1e-8))
+    assert torch.equal(p.float().cpu(), torch.full((n,), 0.98828125))       # 253.44 / 256, to the nearest
+
+
+def test_bfloat16_parameter_written_from_outside_is_the_new_weight():
+    from fdgs import adamw
+    p = torch.ones(300, device="cuda", dtype=torch.bfloat16)
+    low = torch.full((300,), 123, device="cuda", dtype=torch.int16)
+    p.fill_(-2.5)
+    adamw.adamw_step([p], [torch.zeros_like(p)], [torch.zeros(300, device="cuda")], [torch.zeros(300, device="cuda")],
+                     steps=1, lr=1e-3, weight_decay=0.0, residuals=[low])
+    assert (p.float() + 2.5).abs().max() == 0 and (low == 123).all()
+
+
+def test_same_inputs_same_bits_on_any_stream():
+    from fdgs import adamw
+    data = _inputs([70001, 257, 4096], 2)
+
+    def run(stream):
+        ps, gs = [torch.from_numpy(d[0]).cuda() for d in data], [torch.from_numpy(d[1]).cuda() for d in data]
+        ms, vs = ([f(torch.from_numpy(d[0]).cuda()) for d in data] for f in
+                  (lambda x: adamw.Moment8.zeros_like(x, True), lambda x: adamw.Moment8.zeros_like(x, False)))
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            for t in (1, 2, 3):
+                adamw.adamw_step(ps, gs, ms, vs, steps=t, lr=1e-2, keys=[t, t + 10, t + 20])
+        torch.cuda.synchronize()
+        return ps + [x.codes for x in ms + vs] + [x.exponents for x in ms + vs]
+    for a, b in zip(run(torch.cuda.current_stream()), run(torch.cuda.Stream())):
+        assert torch.equal(a, b)
+
+
+def test_capture_is_refused_and_leaves_the_state_alone():
+    from fdgs import adamw
+    p, g = torch.ones(64, device="cuda"), torch.ones(64, device="cuda")
+    m, v = torch.zeros(64, device="cuda"), torch.zeros(64, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="captured"):
+            adamw.adamw_step([p], [g], [m], [v], steps=1, lr=1e-3)
+        q = p + 1
+    graph.replay()
+    torch.cuda.synchronize()
+    assert (q == 2).all() and (p == 1).all() and (m == 0).all()
+
+
+def test_more_tensors_than_one_launch_takes():
+    from fdgs import adamw
+    rng = np.random.default_rng(0)
+    sizes = [int(n) for n in rng.integers(0, 700, 171)]
+    data = _inputs(sizes, 5)
+    ps, gs, ms, vs = ([torch.from_numpy(d[k]).cuda() for d in data] for k in range(4))
+    adamw.adamw_step(ps, gs, ms, vs, steps=3, lr=1e-3, weight_decay=0.0)
+    for d, p, m in zip(data, ps, ms):
+        w64, m64, v64 = ac.adamw64(*d, 3, 1e-3, 0.0, 0.9, 0.999, 1e-8)
+        tol = 3.03 * U * (0.9 * np.abs(d[2]) + 0.1 * np.abs(d[1])) + 2.0 ** -149
+        _within(m.cpu().numpy(), m64, tol, "m")
+        denom = np.sqrt(v64 / (1 - 0.999 ** 3)) + 1e-8
+        scale = 1e-3 / (1 - 0.9 ** 3) / denom
+        _within(p.cpu().numpy(), w64, 12.2 * U * np.abs(m64) * scale + 1.01 * tol * scale + 4.04 * U * np.abs(d[0]) + 2.0 ** -149, "w")

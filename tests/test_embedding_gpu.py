@@ -1,0 +1,256 @@
+"""GPU: fdgs_embedding_fwd / fdgs_embedding_bwd through fdgs.embedding against the definition in 64 bits.
+
+Tolerances: the lookup rounds a product to float32 (u = 2^-24) and once to the table's type (half a step, h).  The
+gradient adds up to n terms in float32: shares of up to 32 items, then their partial sums, so a term passes through at
+most 32 + n / 8 + 32 additions (a share holds at least 8 items, the groups of a join at most 256)."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+HALF = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+# half a step at the small end, where a type's numbers are evenly spaced
+SMALL = {torch.float32: 2.0 ** -150, torch.bfloat16: 2.0 ** -134, torch.float16: 2.0 ** -25}
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def _ids(t, v, seed, dtype, spread="mixed"):
+    g = torch.Generator().manual_seed(seed)
+    if spread == "one":
+        return torch.full((t,), v // 2, dtype=dtype)
+    if spread == "distinct":
+        return torch.randperm(max(t, v), generator=g)[:t].remainder(v).to(dtype)
+    ids = (v * torch.rand(t, generator=g) ** 3).long().clamp(0, v - 1)
+    if t > 4:
+        ids[torch.rand(t, generator=g) < 0.1] = -1           # without a row
+        ids[torch.rand(t, generator=g) < 0.05] = v           # beyond the table
+        ids[0], ids[-1] = v - 1, 0
+    return ids.to(dtype)
+
+
+def _lookup64(ids, table, scale, padding=None):
+    v = table.shape[0]
+    ids = ids.long()
+    none = (ids < 0) | (torch.zeros_like(ids, dtype=torch.bool) if padding is None else ids == padding)
+    out = torch.zeros(ids.shape + table.shape[1:], dtype=torch.float64)
+    if v:
+        out = scale * table.double()[ids.clamp(0, v - 1)]
+    out[none] = 0.0
+    out[(ids >= v) & ~none] = float("nan")
+    return out
+
+
+def _grad64(gy, ids, v, scale, padding=None):
+    flat = gy.reshape(ids.numel(), math.prod(gy.shape[ids.dim():])).double()
+    ids = ids.reshape(-1).long()
+    ok = (ids >= 0) & (ids < v)
+    if padding is not None:
+        ok &= ids != padding
+    acc = torch.zeros(v, flat.shape[1], dtype=torch.float64)
+    size = torch.zeros(v, flat.shape[1], dtype=torch.float64)
+    acc.index_add_(0, ids[ok], flat[ok])
+    size.index_add_(0, ids[ok], flat[ok].abs())
+    count = torch.bincount(ids[ok], minlength=v).double()[:, None]
+    return scale * acc, abs(scale) * size, count
+
+
+def _check_lookup(y, want, dtype):
+    y = y.cpu().double()
+    assert torch.equal(y.isnan(), want.isnan())
+    err = (y - want).abs().nan_to_num(0.0)
+    assert (err <= want.abs().nan_to_num(0.0) * (HALF[dtype] * (1 + U) + U) + SMALL[dtype]).all(), float(err.max())
+
+
+def _check_grad(got, gy, ids, scale, dtype, padding=None):
+    want, size, count = _grad64(gy.cpu(), ids.cpu(), got.shape[0], scale, padding)
+    got = got.reshape(want.shape).cpu().double()
+    depth = torch.minimum(count, 64 + count / 8) + 1                     # additions a term passes, and the product
+    err = (got - want).abs()
+    tol = U * depth * size + (want.abs() + U * depth * size) * HALF[dtype] + SMALL[dtype]
+    assert (err <= tol).all(), (float((err - tol).max()), int((err > tol).sum()))
+    assert (got[(count == 0).view(-1)] == 0).all()
+
+
+SHAPES = [  # tokens, rows, width
+    (0, 5, 8), (1, 1, 1), (1, 7, 3), (3, 1, 4), (37, 101, 33), (63, 64, 5), (64, 3, 64), (65, 1000, 12), (300, 17, 48),
+    (1000, 5000, 31), (4096, 300, 7), (4097, 11, 256), (5000, 2, 1), (700, 40000, 2), (129, 33, 2056), (40, 9, 9001),
+    (16384, 500, 16), (16385, 500, 16), (50000, 70000, 6), (60000, 255, 48), (40001, 256, 9)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("t,v,d", SHAPES)
+def test_lookup_and_gradient(t, v, d, dtype):
+    from fdgs.embedding import embedding
+    g = torch.Generator().manual_seed(t + v + d)
+    idt = torch.int32 if (t + d) % 2 else torch.int64
+    ids = _ids(t, v, t, idt)
+    table = torch.randn(v, d, generator=g).to(dtype)
+    gy = torch.randn(t, d, generator=g).to(dtype)
+    scale = math.sqrt(d)
+    x = table.cuda().requires_grad_(True)
+    y = embedding(ids.cuda(), x, scale=scale)
+    assert y.dtype is dtype and y.shape == (t, d)
+    _check_lookup(y.detach(), _lookup64(ids, table, float(torch.tensor(scale)), None), dtype)
+    grad, = torch.autograd.grad(y, x, gy.cuda())
+    assert grad.dtype is dtype and grad.shape == x.shape
+    _check_grad(grad, gy, ids, float(torch.tensor(scale)), dtype)
+    # the same bits again
+    again, = torch.autograd.grad(embedding(ids.cuda(), x, scale=scale), x, gy.cuda())
+    assert torch.equal(grad, again)
+
+
+@pytest.mark.parametrize("spread", ["one", "distinct"])
+@pytest.mark.parametrize("t,v,d,dtype", [(20000, 3, 48, torch.float32), (9000, 5, 1000, torch.bfloat16), (33000, 4, 1, torch.float16),
+                                         (2000, 2, 2500, torch.float32), (16000, 20000, 48, torch.float32), (100, 1 << 20, 5, torch.float32)])
+def test_one_row_for_all_and_a_row_for_each(t, v, d, dtype, spread):
+    """A row with every token (its sum is cut over many shares) and none with more than one or two.  Small whole numbers: the
+    sums are exact in float32, so the gradient is the rounded exact value, whatever the order."""
+    from fdgs.embedding import embedding_grad
+    g = torch.Generator().manual_seed(t)
+    ids = _ids(t, v, 5, torch.int32, spread)
+    gy = torch.randint(-4, 5, (t, d), generator=g).to(dtype)
+    got = embedding_grad(gy.cuda(), ids.cuda(), v, scale=0.5).cpu()
+    want, _, _ = _grad64(gy, ids, v, 0.5)
+    assert torch.equal(got, want.to(torch.float32).to(dtype))
+
+
+def test_padding_and_shapes_of_ids():
+    from fdgs.embedding import embedding, embedding_grad
+    g = torch.Generator().manual_seed(4)
+    table = torch.randn(50, 16, 3, generator=g).cuda()
+    ids = torch.randint(-2, 50, (6, 9, 4), generator=g)
+    for use in (ids, ids.transpose(0, 2), ids[::2, 1:], ids[0, 0, 0], ids[:0]):
+        dev = use.cuda() if use.is_contiguous() else ids.cuda().transpose(0, 2) if use.shape[0] == 4 else ids.cuda()[::2, 1:]
+        assert dev.shape == use.shape
+        for padding in (None, 7):
+            x = table.clone().requires_grad_(True)
+            y = embedding(dev, x, scale=2.0, padding_id=padding)
+            assert y.shape == use.shape + (16, 3)
+            _check_lookup(y.detach(), _lookup64(use, table.cpu(), 2.0, padding), torch.float32)
+            gy = torch.randn(y.shape, generator=g)
+            grad, = torch.autograd.grad(y, x, gy.cuda())
+            _check_grad(grad, gy, use, 2.0, torch.float32, padding)
+            assert torch.equal(grad, embedding_grad(gy.cuda(), dev, 50, scale=2.0, padding_id=padding))
+
+
+def test_slices_of_tables_and_gradients_are_read_in_place():
+    from fdgs.embedding import embedding, embedding_grad
+    g = torch.Generator().manual_seed(9)
+    wide = torch.randn(40, 30, generator=g).cuda()
+    ids = torch.randint(0, 40, (5, 21), generator=g).cuda()
+    for table in (wide[:, 3:20], wide[:, 1:2], wide[::3], wide.t(), wide[:1].expand(40, 30)):
+        ok = ids.remainder(table.shape[0])
+        assert torch.equal(embedding(ok, table, scale=1.5), embedding(ok, table.contiguous(), scale=1.5))
+    wide = torch.randn(5, 21, 64, generator=g).cuda()
+    for gy in (wide[..., 5:20], wide[..., :1], wide[:, :1].expand(5, 21, 64), wide[:1, :1, :9].expand(5, 21, 9),
+               torch.ones((), device="cuda").expand(5, 21, 33), wide.transpose(1, 2)[:, :21]):
+        assert torch.equal(embedding_grad(gy, ids, 40), embedding_grad(gy.contiguous(), ids, 40))
+
+
+def test_gradient_against_differences():
+    """The lookup is linear: with whole numbers the difference of two lookups, weighted, is the gradient exactly."""
+    from fdgs.embedding import embedding
+    g = torch.Generator().manual_seed(2)
+    ids = torch.randint(0, 30, (400,), generator=g).cuda()
+    table = torch.randint(-8, 9, (30, 20), generator=g).float().cuda().requires_grad_(True)
+    step = torch.randint(-3, 4, (30, 20), generator=g).float().cuda()
+    gy = torch.randint(-3, 4, (400, 20), generator=g).float().cuda()
+    y = embedding(ids, table, scale=2.0)
+    grad, = torch.autograd.grad(y, table, gy)
+    moved = embedding(ids, (table + step).detach(), scale=2.0)
+    assert float(((moved - y.detach()) * gy).double().sum()) == float((grad * step).double().sum())
+
+
+def test_gradient_twice_is_refused():
+    from fdgs.embedding import embedding
+    table = torch.randn(4, 4, device="cuda", requires_grad=True)
+    y = embedding(torch.tensor([1, 2], device="cuda"), table)
+    with pytest.raises(RuntimeError):
+        g, = torch.autograd.grad((y * y).sum(), table, create_graph=True)
+        torch.autograd.grad(g.sum(), table)
+
+
+def test_two_captured_graphs_with_workspaces_of_their_own():
+    """Lookup and gradient captured twice, replayed in turn with new inputs and eager calls in between."""
+    from fdgs.embedding import embedding, embedding_grad
+    cases = []
+    for t, v, d in ((20000, 300, 24), (500, 900, 40)):
+        cases.append([torch.zeros(t, dtype=torch.int32, device="cuda"), torch.zeros(v, d, device="cuda"),
+                      torch.zeros(t, d, device="cuda"), None, None, torch.cuda.CUDAGraph()])
+    for c in cases:
+        ids, table, gy = c[:3]
+        embedding_grad(gy, ids, table.shape[0])
+        with torch.cuda.graph(c[5]):
+            c[3], c[4] = embedding(ids, table, scale=3.0), embedding_grad(gy, ids, table.shape[0], scale=3.0)
+    for k in range(4):
+        for j, (ids, table, gy, y, grad, graph) in enumerate(cases):
+            g = torch.Generator().manual_seed(10 * k + j)
+            ids.copy_((table.shape[0] * torch.rand(ids.shape, generator=g) ** 2).int())
+            table.copy_(torch.randn(table.shape, generator=g))
+            gy.copy_(torch.randn(gy.shape, generator=g))
+            graph.replay()
+            eager = embedding(ids, table, scale=3.0), embedding_grad(gy, ids, table.shape[0], scale=3.0)
+            torch.cuda.synchronize()
+            assert torch.equal(y, eager[0]) and torch.equal(grad, eager[1])
+
+
+def test_two_streams_at_once():
+    from fdgs.embedding import embedding_grad
+    g = torch.Generator().manual_seed(1)
+    jobs = []
+    for t, v, d in ((30000, 100, 64), (17000, 5000, 33)):
+        ids, gy = torch.randint(0, v, (t,), generator=g).cuda(), torch.randn(t, d, generator=g).cuda()
+        jobs.append((gy, ids, v, torch.cuda.Stream(), embedding_grad(gy, ids, v)))
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(5):
+        for gy, ids, v, stream, want in jobs:
+            with torch.cuda.stream(stream):
+                got.append((embedding_grad(gy, ids, v), want))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in got)
+
+
+def test_offsets_past_32_bits():
+    """Outputs, tables and gradients of more than 2^31 elements: rows and tokens at both ends."""
+    from fdgs.embedding import embedding, embedding_grad
+    d, n = 2048, (1 << 20) + 77                  # 2^31 + 157,696 elements
+    ids = torch.arange(n, device="cuda").flip(0).to(torch.int32)
+    table = torch.zeros(n, d, dtype=torch.bfloat16, device="cuda")
+    for r in (0, 1, n // 2, n - 2, n - 1):
+        table[r] = float(r % 251 + 1)
+    y = embedding(ids, table)
+    for r in (0, 1, n // 2, n - 2, n - 1):
+        assert (y[n - 1 - r] == float(r % 251 + 1)).all()
+    assert int((y[:, 0] != 0).sum()) == 5 and int((y[:, d - 1] != 0).sum()) == 5
+    del table
+    grad = embedding_grad(y, ids, n, scale=2.0)
+    for r in (0, 1, n // 2, n - 2, n - 1):
+        assert (grad[r] == 2.0 * float(r % 251 + 1)).all()
+    assert int((grad[:, 0] != 0).sum()) == 5 and int((grad[:, d - 1] != 0).sum()) == 5
+
+
+def test_refusals_on_the_device():
+    from fdgs.embedding import embedding, embedding_grad
+    table = torch.zeros(4, 4, device="cuda")
+    with pytest.raises(ValueError, match="one device"):
+        embedding(torch.tensor([1]), table)
+    with pytest.raises(ValueError, match="int32 or int64"):
+        embedding(torch.tensor([1.0], device="cuda"), table)
+    with pytest.raises(ValueError, match="float32, bfloat16"):
+        embedding(torch.tensor([1], device="cuda"), table.double())
+    with pytest.raises(ValueError, match="row of the table"):
+        embedding(torch.tensor([1], device="cuda"), table, padding_id=-1)
+    ids = torch.tensor([1, 2], device="cuda")
+    with pytest.raises(ValueError, match="ids.shape"):
+        embedding_grad(torch.zeros(3, 4, device="cuda"), ids, 4)
+    with pytest.raises(ValueError, match="ids.shape"):
+        embedding_grad(torch.zeros(2, device="cuda"), ids, 4)
+    with pytest.raises(ValueError, match="num_rows"):
+        embedding_grad(torch.zeros(2, 4, device="cuda"), ids, -1)
+    assert embedding_grad(torch.zeros(2, 4, device="cuda"), ids, 0).shape == (0, 4)
+    assert embedding(torch.tensor([0, 1], device="cuda"), torch.zeros(0, 4, device="cuda")).isnan().all()
+    assert embedding(ids, torch.zeros(4, 0, device="cuda")).shape == (2, 0)
+    assert embedding_grad(torch.zeros(2, 0, device="cuda"), ids, 4).shape == (4, 0)

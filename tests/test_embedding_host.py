@@ -1,0 +1,73 @@
+"""CPU: what the table lookup and its gradient refuse, and the sizes of the workspace."""
+import ctypes as C
+
+import pytest
+import torch
+
+
+def _fwd(**over):
+    from fdgs import _lib, _records
+    f = dict(num_tokens=2, num_rows=3, dim=4, type=0, id_bytes=4, ids=64, table=64, table_row_stride=4, padding_id=-1, out=64, scale=1.0)
+    f.update(over)
+    return _lib.lib.fdgs_embedding_fwd(C.byref(_records.EmbeddingFwdArgs(**f)), None)
+
+
+def _bwd(**over):
+    from fdgs import _lib, _records
+    f = dict(num_tokens=2, num_rows=3, dim=4, type=0, id_bytes=8, ids=64, grad_out=64, grad_out_row_stride=4, padding_id=-1,
+             grad_table=64, scale=1.0, workspace=64, workspace_bytes=1 << 30)
+    f.update(over)
+    return _lib.lib.fdgs_embedding_bwd(C.byref(_records.EmbeddingBwdArgs(**f)), None)
+
+
+def test_library_refuses_before_any_launch():
+    from fdgs import _lib
+    assert _lib.lib.fdgs_embedding_fwd(None, None) == -1 and _lib.lib.fdgs_embedding_bwd(None, None) == -1
+    for call in (_fwd, _bwd):
+        for bad in (dict(num_tokens=-1), dict(num_rows=-1), dict(dim=-1), dict(type=3), dict(type=-1), dict(id_bytes=2), dict(ids=0)):
+            assert call(**bad) == -1, bad
+        assert call(dim=0) == 0 and call(dim=(1 << 24) + 1) == -4
+    assert _fwd(table=0) == -1 and _fwd(out=0) == -1 and _fwd(table_row_stride=-1) == -1 and _fwd(num_tokens=0) == 0
+    assert _fwd(num_tokens=1 << 31) == -4
+    assert _bwd(grad_out=0) == -1 and _bwd(grad_table=0) == -1 and _bwd(grad_out_row_stride=-1) == -1 and _bwd(num_rows=0) == 0
+    assert _bwd(num_tokens=(1 << 30) + 1) == -4
+    assert _bwd(workspace=0) == -3 and _bwd(workspace_bytes=16) == -3
+
+
+@pytest.mark.parametrize("kind", [0, 1, 2])
+def test_workspace_grows_with_the_work(kind):
+    from fdgs._lib import lib
+    size = lib.fdgs_embedding_bwd_workspace_bytes
+    assert size(-1, 4, 4, kind) == 0 and size(4, 4, 0, kind) == 0 and size(4, 4, 4, 7) == 0
+    for v, d in ((1, 1), (100, 48), (65536, 48), (1000, 5000)):
+        last = 0
+        for t in (0, 1, 100, 16384, 16385, 300000):
+            now = size(t, v, d, kind)
+            assert now >= 8 * t and now >= last * 0.5
+            last = now
+
+
+def test_cpu_tensors_are_refused():
+    from fdgs.embedding import FeatureCodebook, embedding, embedding_grad
+    ids, table = torch.tensor([0, 1]), torch.zeros(3, 4)
+    with pytest.raises(RuntimeError, match="GPU only"):
+        embedding(ids, table)
+    with pytest.raises(RuntimeError, match="GPU only"):
+        embedding_grad(torch.zeros(2, 4), ids, 3)
+    with pytest.raises(ValueError, match="rows, ..."):
+        embedding(ids, torch.zeros(3))
+    with pytest.raises(ValueError, match="per Gaussian"):
+        FeatureCodebook(torch.zeros(3, 16, 3), ids.view(2, 1))
+    book = FeatureCodebook(torch.zeros(3, 16, 3), ids)
+    assert set(book.state_dict()) == {"table", "ids"} and book.table.requires_grad
+
+
+def test_rows_of_strided_gradients():
+    """Which tensors are read in place, and with what distance between their rows."""
+    from fdgs.embedding import _rows
+    base = torch.zeros(6, 5, 8)
+    for t, lead, width, stride in ((base, 2, 8, 8), (base[..., 2:5], 2, 3, 8), (base[:, :1].expand(6, 5, 8), 2, 8, None),
+                                   (base[:1, :1].expand(6, 5, 8), 2, 8, 0), (base[:, ::2, :4], 2, 4, None), (base[::2], 1, 40, 80),
+                                   (base[:, 0], 1, 8, 40), (base.transpose(0, 1), 2, 8, None), (torch.zeros(()).expand(6, 5, 8), 2, 8, None)):
+        got, w, s = _rows(t, lead)
+        assert w == width and (got is t) == (stride is not None) and s == (width if stride is None else stride), (t.shape, t.stride())
