@@ -15,8 +15,9 @@
 #include "moment8.h"
 
 #define AW_MAX 40                                // tensors per launch: their records fill 4 KB of kernel arguments
-#define AW_PER_WAVE 512                          // two blocks of 256 per wave
-#define AW_PER_GROUP 2048                        // elements per workgroup of four waves
+#define AW_BLOCKS 2                               // blocks of 256 per wave
+#define AW_PER_WAVE (AW_BLOCKS * 256)
+#define AW_PER_GROUP (4 * AW_PER_WAVE)           // elements per workgroup of four waves
 
 struct AwTensor {
     void* p; const void* g; void* m; void* v;
@@ -27,7 +28,7 @@ struct AwTensor {
     uint32_t key, pad;
 };
 struct AwPart {
-    int num;
+    int num, exact;                              // exact: eps lies below the normal numbers
     float b1, omb1, b2, omb2, eps;
     int start[AW_MAX];                           // first workgroup of each tensor
     AwTensor t[AW_MAX];
@@ -37,6 +38,8 @@ static_assert(sizeof(AwPart) <= 4096, "kernel arguments of one launch");
 struct __attribute__((packed, aligned(4))) aw_f4 { float x[4]; };
 struct __attribute__((packed, aligned(2))) aw_h4 { uint16_t x[4]; };
 struct __attribute__((packed, aligned(1))) aw_b4 { uint32_t x; };
+struct __attribute__((packed, aligned(1))) aw_b8 { uint32_t x[2]; };
+struct __attribute__((packed, aligned(2))) aw_w4 { uint32_t x[4]; };
 
 // float32 -> bfloat16 to the nearest, halves away from zero, and the signed 16 bits between the two: the pair is the
 // float32 value again exactly, and (unlike rounding halves to even) the difference always fits.
@@ -52,12 +55,19 @@ __device__ __forceinline__ float aw_join(uint16_t hi, int16_t lo) {
 }
 __device__ __forceinline__ float aw_bf16(uint16_t h) { return __uint_as_float((uint32_t)h << 16); }
 
-__device__ __forceinline__ void aw_one(float& w, float g, float& m, float& v, const AwPart& k, const AwTensor& t) {
+// The update with the chip's root and reciprocal (each within 1.6 units of 2^-24 for normal numbers) in place of the
+// correctly rounded root and division, 9 issue slots instead of 32: with 8-bit moments the float32 step is bound by its
+// arithmetic, and the update's rounding is far below the 0.1 by which its moments' codes spread.  The caller keeps
+// numbers below the normal ones, which these instructions take for zero, away from it.
+__device__ __forceinline__ float aw_quick(float w, float m, float v, const AwPart& k, const AwTensor& t) {
 #pragma clang fp contract(off)
-    m = m * k.b1 + g * k.omb1;
-    v = v * k.b2 + (g * g) * k.omb2;
+    const float denom = __builtin_amdgcn_sqrtf(v) * t.inv_root + k.eps;
+    return w * t.decay - (m * t.step_size) * __builtin_amdgcn_rcpf(denom);
+}
+__device__ __forceinline__ float aw_exact(float w, float m, float v, const AwPart& k, const AwTensor& t) {
+#pragma clang fp contract(off)
     const float denom = sqrtf(v) * t.inv_root + k.eps;
-    w = w * t.decay - (m * t.step_size) / denom;
+    return w * t.decay - (m * t.step_size) / denom;
 }
 
 // The tensor that workgroup `b` works on: one look at every tensor's first workgroup, a lane each.
@@ -67,35 +77,13 @@ __device__ __forceinline__ int aw_find(const int* start, int num, int b) {
     return __builtin_amdgcn_readfirstlane(__popcll(__ballot(s <= b)) - 1);
 }
 
-template <bool BF16, bool EIGHT>
-struct AwLane {                                  // a lane's four elements of a block
-    float w[4], g[4], m[4], v[4];
-};
-
-// Gradient element i: i itself, or (rows of L elements, S apart) its place in a column slice of a wider array.
 template <bool BF16>
 __device__ __forceinline__ float aw_grad(const void* g, long long i) {
     return BF16 ? aw_bf16(((const uint16_t*)g)[i]) : ((const float*)g)[i];
 }
+// Four gradient elements from element i on in rows of L elements, S apart: a column slice of a wider array.
 template <bool BF16>
-__device__ __forceinline__ void aw_grad4(const AwTensor& t, long long i, int valid, float* out) {
-    if (t.glen == 0) {
-        if (valid == 4) {
-            if (BF16) {
-                const aw_h4 x = *(const aw_h4*)((const uint16_t*)t.g + i);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) out[j] = aw_bf16(x.x[j]);
-            } else {
-                const aw_f4 x = *(const aw_f4*)((const float*)t.g + i);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) out[j] = x.x[j];
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) out[j] = j < valid ? aw_grad<BF16>(t.g, i + j) : 0.0f;
-        }
-        return;
-    }
+__device__ __forceinline__ void aw_grad_rows(const AwTensor& t, long long i, int valid, float* out) {
     long long row;
     int col;
     if (t.n <= 0xFFFFFFFFLL) {                   // a 32-bit division where the index allows it
@@ -113,66 +101,121 @@ __device__ __forceinline__ void aw_grad4(const AwTensor& t, long long i, int val
     }
 }
 
+// A lane's four elements of a block as they lie in memory.
 template <bool BF16, bool EIGHT>
-__device__ __forceinline__ void aw_load(const AwTensor& t, long long i, int valid, int em, int ev, AwLane<BF16, EIGHT>& x) {
-    aw_grad4<BF16>(t, i, valid, x.g);
-    uint32_t cm = 0, cv = 0;
-    if (valid == 4) {
+struct AwLane {
+    float g[4], w[4], m[4], v[4];                // m, v: float32 moments only
+    uint32_t cm, cv;                             // 8-bit moments' codes
+    int em, ev;                                  // and their block's exponents
+};
+
+// WHOLE: the block has 256 elements.  Else a lane has `valid` (0 to 4) of its four and the rest are zeros.
+template <bool BF16, bool EIGHT, bool WHOLE>
+__device__ __forceinline__ void aw_load(const AwTensor& t, long long block, int valid, AwLane<BF16, EIGHT>& x) {
+    const uint32_t o = 4u * (threadIdx.x & 63);  // the block is the wave's: its address is scalar, the lane's part 32 bits
+    if (t.glen != 0) {
+        aw_grad_rows<BF16>(t, block + o, WHOLE ? 4 : valid, x.g);
+    } else if (WHOLE) {
         if (BF16) {
-            const aw_h4 h = *(const aw_h4*)((const uint16_t*)t.p + i), l = *(const aw_h4*)(t.low + i);
+            const aw_h4 g = *(const aw_h4*)((const uint16_t*)t.g + block + o);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x.g[j] = aw_bf16(g.x[j]);
+        } else {
+            const aw_f4 g = *(const aw_f4*)((const float*)t.g + block + o);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x.g[j] = g.x[j];
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x.g[j] = j < valid ? aw_grad<BF16>(t.g, block + o + j) : 0.0f;
+    }
+    if (EIGHT) {
+        x.em = t.me[block / M8_BLOCK];
+        x.ev = t.ve[block / M8_BLOCK];
+    }
+    if (WHOLE) {
+        if (BF16) {
+            const aw_h4 h = *(const aw_h4*)((const uint16_t*)t.p + block + o), l = *(const aw_h4*)(t.low + block + o);
 #pragma unroll
             for (int j = 0; j < 4; ++j) x.w[j] = aw_join(h.x[j], (int16_t)l.x[j]);
         } else {
-            const aw_f4 p = *(const aw_f4*)((const float*)t.p + i);
+            const aw_f4 p = *(const aw_f4*)((const float*)t.p + block + o);
 #pragma unroll
             for (int j = 0; j < 4; ++j) x.w[j] = p.x[j];
         }
         if (EIGHT) {
-            cm = ((const aw_b4*)((const uint8_t*)t.m + i))->x;
-            cv = ((const aw_b4*)((const uint8_t*)t.v + i))->x;
+            x.cm = ((const aw_b4*)((const uint8_t*)t.m + block + o))->x;
+            x.cv = ((const aw_b4*)((const uint8_t*)t.v + block + o))->x;
         } else {
-            const aw_f4 m = *(const aw_f4*)((const float*)t.m + i), v = *(const aw_f4*)((const float*)t.v + i);
+            const aw_f4 m = *(const aw_f4*)((const float*)t.m + block + o), v = *(const aw_f4*)((const float*)t.v + block + o);
 #pragma unroll
             for (int j = 0; j < 4; ++j) { x.m[j] = m.x[j]; x.v[j] = v.x[j]; }
         }
-    } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const bool ok = j < valid;
-            if (BF16) x.w[j] = ok ? aw_join(((const uint16_t*)t.p)[i + j], t.low[i + j]) : 0.0f;
-            else x.w[j] = ok ? ((const float*)t.p)[i + j] : 0.0f;
-            if (EIGHT) {
-                cm |= (ok ? (uint32_t)((const uint8_t*)t.m)[i + j] : 0u) << (8 * j);
-                cv |= (ok ? (uint32_t)((const uint8_t*)t.v)[i + j] : 0u) << (8 * j);
-            } else {
-                x.m[j] = ok ? ((const float*)t.m)[i + j] : 0.0f;
-                x.v[j] = ok ? ((const float*)t.v)[i + j] : 0.0f;
-            }
-        }
+        return;
     }
-    if (EIGHT) {
-        const int bm = m8_base<true>(em), bv = m8_base<false>(ev);
+    x.cm = x.cv = 0;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            x.m[j] = m8_decode<true>((cm >> (8 * j)) & 255u, em, bm);
-            x.v[j] = m8_decode<false>((cv >> (8 * j)) & 255u, ev, bv);
+    for (int j = 0; j < 4; ++j) {
+        const bool ok = j < valid;
+        const long long i = block + o + j;
+        if (BF16) x.w[j] = ok ? aw_join(((const uint16_t*)t.p)[i], t.low[i]) : 0.0f;
+        else x.w[j] = ok ? ((const float*)t.p)[i] : 0.0f;
+        if (EIGHT) {
+            x.cm |= (ok ? (uint32_t)((const uint8_t*)t.m)[i] : 0u) << (8 * j);
+            x.cv |= (ok ? (uint32_t)((const uint8_t*)t.v)[i] : 0u) << (8 * j);
+        } else {
+            x.m[j] = ok ? ((const float*)t.m)[i] : 0.0f;
+            x.v[j] = ok ? ((const float*)t.v)[i] : 0.0f;
         }
     }
 }
 
-template <bool BF16, bool EIGHT>
+template <bool BF16, bool EIGHT, bool WHOLE>
 __device__ __forceinline__ void aw_finish(const AwPart& k, const AwTensor& t, long long block, int valid, AwLane<BF16, EIGHT>& x) {
-    const int lane = threadIdx.x & 63;
-    const long long i = block + 4 * lane;
+    const uint32_t lane = threadIdx.x & 63, o = 4 * lane;
+    float b1 = k.b1, b2 = k.b2;
+    if (EIGHT) {
+        const int em = __builtin_amdgcn_readfirstlane(x.em), ev = __builtin_amdgcn_readfirstlane(x.ev);
+        const int bm = m8_base<true>(em), bv = m8_base<false>(ev);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) aw_one(x.w[j], x.g[j], x.m[j], x.v[j], k, t);
+        for (int j = 0; j < 4; ++j) {
+            x.m[j] = __uint_as_float(m8_decode<true>((x.cm >> (8 * j)) & 255u, bm));
+            x.v[j] = __uint_as_float(m8_decode<false>((x.cv >> (8 * j)) & 255u, bv));
+        }
+        if (em == 255) b1 = __builtin_nanf("");  // the block stands for NaN
+        if (ev == 255) b2 = __builtin_nanf("");
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+#pragma clang fp contract(off)
+        x.m[j] = x.m[j] * b1 + x.g[j] * k.omb1;
+        x.v[j] = x.v[j] * b2 + (x.g[j] * x.g[j]) * k.omb2;
+    }
+    if (EIGHT && !BF16) {
+        uint32_t least = 0xFFFFFFFFu;            // (pattern - 1) of the smallest v that is not zero
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t b = __float_as_uint(x.v[j]) - 1u;
+            least = b < least ? b : least;
+        }
+        if (__ballot(least < 0x007FFFFFu) == 0 && !k.exact) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x.w[j] = aw_quick(x.w[j], x.m[j], x.v[j], k, t);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x.w[j] = aw_exact(x.w[j], x.m[j], x.v[j], k, t);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x.w[j] = aw_exact(x.w[j], x.m[j], x.v[j], k, t);
+    }
     uint32_t cm = 0, cv = 0;
     if (EIGHT) {
         uint32_t tm = 0, tv = 0;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const uint32_t a = __float_as_uint(x.m[j]) & 0x7FFFFFFFu, b = __float_as_uint(x.v[j]) & 0x7FFFFFFFu;
-            if (j < valid) {
+            if (WHOLE || j < valid) {
                 tm = a > tm ? a : tm;
                 tv = b > tv ? b : tv;
             }
@@ -180,19 +223,22 @@ __device__ __forceinline__ void aw_finish(const AwPart& k, const AwTensor& t, lo
         const uint32_t e2 = m8_wave_max2((tm >> 23) | ((tv >> 23) << 16));
         const int em = (int)(e2 & 0xFFFFu), ev = (int)(e2 >> 16);
         const int bm = m8_base<true>(em), bv = m8_base<false>(ev);
-        const uint32_t key = m8_key(t.key, i);
+        // the hash's first product, once: the elements follow one another
+        const uint32_t x0 = ((uint32_t)block + o + m8_key(t.key, block)) * M8_C1;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const uint32_t h = m8_hash((uint32_t)i + j, key);
-            cm |= m8_encode<true>(x.m[j], m8_noise_m(h), em, bm) << (8 * j);
-            cv |= m8_encode<false>(x.v[j], m8_noise_v(h), ev, bv) << (8 * j);
+            const uint32_t h = m8_hash(x0 + (uint32_t)j * M8_C1);
+            cm |= m8_encode<true>(x.m[j], m8_noise_m(h), bm) << (8 * j);
+            cv |= m8_encode<false>(x.v[j], m8_noise_v(h), bv) << (8 * j);
         }
+        cm = em == 255 ? 0u : cm;
+        cv = ev == 255 ? 0u : cv;
         if (lane == 0) {
             t.me[block / M8_BLOCK] = (uint8_t)em;
             t.ve[block / M8_BLOCK] = (uint8_t)ev;
         }
     }
-    if (valid == 4) {
+    if (WHOLE) {
         if (BF16) {
             aw_h4 h, l;
 #pragma unroll
@@ -201,44 +247,45 @@ __device__ __forceinline__ void aw_finish(const AwPart& k, const AwTensor& t, lo
                 aw_split(x.w[j], h.x[j], lo);
                 l.x[j] = (uint16_t)lo;
             }
-            *(aw_h4*)((uint16_t*)t.p + i) = h;
-            *(aw_h4*)(t.low + i) = l;
+            *(aw_h4*)((uint16_t*)t.p + block + o) = h;
+            *(aw_h4*)(t.low + block + o) = l;
         } else {
             aw_f4 p;
 #pragma unroll
             for (int j = 0; j < 4; ++j) p.x[j] = x.w[j];
-            *(aw_f4*)((float*)t.p + i) = p;
+            *(aw_f4*)((float*)t.p + block + o) = p;
         }
         if (EIGHT) {
-            ((aw_b4*)((uint8_t*)t.m + i))->x = cm;
-            ((aw_b4*)((uint8_t*)t.v + i))->x = cv;
+            ((aw_b4*)((uint8_t*)t.m + block + o))->x = cm;
+            ((aw_b4*)((uint8_t*)t.v + block + o))->x = cv;
         } else {
             aw_f4 m, v;
 #pragma unroll
             for (int j = 0; j < 4; ++j) { m.x[j] = x.m[j]; v.x[j] = x.v[j]; }
-            *(aw_f4*)((float*)t.m + i) = m;
-            *(aw_f4*)((float*)t.v + i) = v;
+            *(aw_f4*)((float*)t.m + block + o) = m;
+            *(aw_f4*)((float*)t.v + block + o) = v;
         }
-    } else {
+        return;
+    }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if (j >= valid) break;
-            if (BF16) {
-                uint16_t hi;
-                int16_t lo;
-                aw_split(x.w[j], hi, lo);
-                ((uint16_t*)t.p)[i + j] = hi;
-                t.low[i + j] = lo;
-            } else {
-                ((float*)t.p)[i + j] = x.w[j];
-            }
-            if (EIGHT) {
-                ((uint8_t*)t.m)[i + j] = (uint8_t)(cm >> (8 * j));
-                ((uint8_t*)t.v)[i + j] = (uint8_t)(cv >> (8 * j));
-            } else {
-                ((float*)t.m)[i + j] = x.m[j];
-                ((float*)t.v)[i + j] = x.v[j];
-            }
+    for (int j = 0; j < 4; ++j) {
+        if (j >= valid) break;
+        const long long i = block + o + j;
+        if (BF16) {
+            uint16_t hi;
+            int16_t lo;
+            aw_split(x.w[j], hi, lo);
+            ((uint16_t*)t.p)[i] = hi;
+            t.low[i] = lo;
+        } else {
+            ((float*)t.p)[i] = x.w[j];
+        }
+        if (EIGHT) {
+            ((uint8_t*)t.m)[i] = (uint8_t)(cm >> (8 * j));
+            ((uint8_t*)t.v)[i] = (uint8_t)(cv >> (8 * j));
+        } else {
+            ((float*)t.m)[i] = x.m[j];
+            ((float*)t.v)[i] = x.v[j];
         }
     }
 }
@@ -248,29 +295,24 @@ __global__ void __launch_bounds__(256)
 adamw_kernel(AwPart k) {
     const int ti = aw_find(k.start, k.num, (int)blockIdx.x);
     const AwTensor& t = k.t[ti];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const long long base = (long long)((int)blockIdx.x - k.start[ti]) * AW_PER_GROUP + wave * AW_PER_WAVE;
-    AwLane<BF16, EIGHT> x[2];
-    if (base + AW_PER_WAVE <= t.n) {             // both blocks whole: all loads before the first use
+    AwLane<BF16, EIGHT> x[AW_BLOCKS];
+    if (base + AW_PER_WAVE <= t.n) {             // whole blocks: all loads before the first use
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const long long b = base + u * M8_BLOCK;
-            const int em = EIGHT ? t.me[b / M8_BLOCK] : 0, ev = EIGHT ? t.ve[b / M8_BLOCK] : 0;
-            aw_load<BF16, EIGHT>(t, b + 4 * lane, 4, em, ev, x[u]);
-        }
+        for (int u = 0; u < AW_BLOCKS; ++u) aw_load<BF16, EIGHT, true>(t, base + u * M8_BLOCK, 4, x[u]);
 #pragma unroll
-        for (int u = 0; u < 2; ++u) aw_finish<BF16, EIGHT>(k, t, base + u * M8_BLOCK, 4, x[u]);
+        for (int u = 0; u < AW_BLOCKS; ++u) aw_finish<BF16, EIGHT, true>(k, t, base + u * M8_BLOCK, 4, x[u]);
         return;
     }
 #pragma unroll 1
-    for (int u = 0; u < 2; ++u) {
+    for (int u = 0; u < AW_BLOCKS; ++u) {
         const long long b = base + u * M8_BLOCK;
         if (b >= t.n) return;
-        const long long left = t.n - (b + 4 * lane);
+        const long long left = t.n - (b + 4 * (threadIdx.x & 63));
         const int valid = left >= 4 ? 4 : left > 0 ? (int)left : 0;
-        const int em = EIGHT ? t.me[b / M8_BLOCK] : 0, ev = EIGHT ? t.ve[b / M8_BLOCK] : 0;
-        aw_load<BF16, EIGHT>(t, b + 4 * lane, valid, em, ev, x[0]);
-        aw_finish<BF16, EIGHT>(k, t, b, valid, x[0]);
+        aw_load<BF16, EIGHT, false>(t, b, valid, x[0]);
+        aw_finish<BF16, EIGHT, false>(k, t, b, valid, x[0]);
     }
 }
 
@@ -293,6 +335,7 @@ extern "C" int fdgs_adamw_step(const fdgs_adamw_args* a, void* stream) {
     k.b1 = (float)a->beta1; k.omb1 = (float)(1.0 - a->beta1);
     k.b2 = (float)a->beta2; k.omb2 = (float)(1.0 - a->beta2);
     k.eps = (float)a->eps;
+    k.exact = k.eps > 0.0f && k.eps < 1.17549435e-38f;
     for (int i = 0; i < a->num_tensors;) {
         int blocks = 0;
         k.num = 0;
@@ -332,45 +375,54 @@ struct M8Part {
 };
 static_assert(sizeof(M8Part) <= 4096, "kernel arguments of one launch");
 
+// Eight consecutive values from element i on.  Eight to a lane: 8 bytes in and, as bfloat16, 16 out.
 template <bool BF16, bool SIGNED>
-__device__ __forceinline__ void m8_unpack_block(const M8Tensor& t, long long b) {
-    const int lane = threadIdx.x & 63;
-    const long long i = b + 4 * lane;
+__device__ __forceinline__ void m8_unpack8(const M8Tensor& t, long long i) {
     if (i >= t.n) return;
-    const int e = t.exps[b / M8_BLOCK], base = m8_base<SIGNED>(e);
-    if (i + 4 <= t.n) {
-        const uint32_t c = ((const aw_b4*)(t.codes + i))->x;
+    const int e = t.exps[i / M8_BLOCK], base = m8_base<SIGNED>(e);
+    const uint32_t nan = 0x7FC00000u;
+    if (i + 8 <= t.n) {
+        const aw_b8 c = *(const aw_b8*)(t.codes + i);
+        uint32_t b[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            b[j] = m8_decode<SIGNED>((c.x[j / 4] >> (8 * (j & 3))) & 255u, base);
+            b[j] = e == 255 ? nan : b[j];
+        }
         if (BF16) {                              // four significant bits: bfloat16 holds them exactly
-            aw_h4 h;
+            aw_w4 h;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) h.x[j] = (uint16_t)(__float_as_uint(m8_decode<SIGNED>((c >> (8 * j)) & 255u, e, base)) >> 16);
-            *(aw_h4*)((uint16_t*)t.value + i) = h;
+            for (int j = 0; j < 4; ++j) h.x[j] = (b[2 * j] >> 16) | (b[2 * j + 1] & 0xFFFF0000u);
+            *(aw_w4*)((uint16_t*)t.value + i) = h;
         } else {
-            aw_f4 f;
+            aw_f4 f[2];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) f.x[j] = m8_decode<SIGNED>((c >> (8 * j)) & 255u, e, base);
-            *(aw_f4*)((float*)t.value + i) = f;
+            for (int j = 0; j < 8; ++j) f[j / 4].x[j & 3] = __uint_as_float(b[j]);
+            *(aw_f4*)((float*)t.value + i) = f[0];
+            *(aw_f4*)((float*)t.value + i + 4) = f[1];
         }
     } else {
         for (long long j = i; j < t.n; ++j) {
-            const float f = m8_decode<SIGNED>(t.codes[j], e, base);
-            if (BF16) ((uint16_t*)t.value)[j] = (uint16_t)(__float_as_uint(f) >> 16);
-            else ((float*)t.value)[j] = f;
+            const uint32_t b = e == 255 ? nan : m8_decode<SIGNED>(t.codes[j], base);
+            if (BF16) ((uint16_t*)t.value)[j] = (uint16_t)(b >> 16);
+            else ((float*)t.value)[j] = __uint_as_float(b);
         }
     }
 }
 
+#define M8_PER_GROUP 8192                        // elements per workgroup
 template <bool BF16>
 __global__ void __launch_bounds__(256)
 moment8_unpack_kernel(M8Part k) {
     const int ti = aw_find(k.start, k.num, (int)blockIdx.x);
     const M8Tensor& t = k.t[ti];
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const long long base = (long long)((int)blockIdx.x - k.start[ti]) * AW_PER_GROUP + wave * AW_PER_WAVE;
+    const long long base = (long long)((int)blockIdx.x - k.start[ti]) * M8_PER_GROUP + 8 * (int)threadIdx.x;
+    if (t.is_signed) {
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-        if (t.is_signed) m8_unpack_block<BF16, true>(t, base + u * M8_BLOCK);
-        else m8_unpack_block<BF16, false>(t, base + u * M8_BLOCK);
+        for (int u = 0; u < 4; ++u) m8_unpack8<BF16, true>(t, base + u * 2048);
+    } else {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) m8_unpack8<BF16, false>(t, base + u * 2048);
     }
 }
 
@@ -392,8 +444,8 @@ __device__ __forceinline__ void m8_pack_block(const M8Part& k, const M8Tensor& t
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         if (i + j >= t.n) break;
-        const uint32_t h = k.nearest ? 0x80008000u : m8_hash((uint32_t)i + j, key);
-        t.codes[i + j] = (uint8_t)m8_encode<SIGNED>(x[j], SIGNED ? m8_noise_m(h) : m8_noise_v(h), e, base);
+        const uint32_t h = k.nearest ? 0x80008000u : m8_hash(((uint32_t)i + j + key) * M8_C1);
+        t.codes[i + j] = (uint8_t)(e == 255 ? 0u : m8_encode<SIGNED>(x[j], SIGNED ? m8_noise_m(h) : m8_noise_v(h), base));
     }
     if (lane == 0) t.exps[b / M8_BLOCK] = (uint8_t)e;
 }
@@ -403,9 +455,9 @@ moment8_pack_kernel(M8Part k) {
     const int ti = aw_find(k.start, k.num, (int)blockIdx.x);
     const M8Tensor& t = k.t[ti];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const long long base = (long long)((int)blockIdx.x - k.start[ti]) * AW_PER_GROUP + wave * AW_PER_WAVE;
+    const long long base = (long long)((int)blockIdx.x - k.start[ti]) * M8_PER_GROUP + wave * (M8_PER_GROUP / 4);
 #pragma unroll 1
-    for (int u = 0; u < 2; ++u) {
+    for (int u = 0; u < M8_PER_GROUP / 4 / M8_BLOCK; ++u) {
         if (t.is_signed) m8_pack_block<true>(k, t, base + u * M8_BLOCK);
         else m8_pack_block<false>(k, t, base + u * M8_BLOCK);
     }
@@ -420,7 +472,7 @@ static int moment8_launch(const fdgs_moment8_args* a, void* stream, bool pack) {
         if (s.numel < 0) return FDGS_EINVAL;
         if (s.numel == 0) continue;
         if (!s.codes || !s.exponents || !s.value) return FDGS_EINVAL;
-        if ((s.numel - 1) / AW_PER_GROUP >= 0x7fffffffLL / M8_MAX) return FDGS_ETOOLARGE;
+        if ((s.numel - 1) / M8_PER_GROUP >= 0x7fffffffLL / M8_MAX) return FDGS_ETOOLARGE;
     }
     M8Part k;
     k.nearest = a->nearest != 0;
@@ -431,7 +483,7 @@ static int moment8_launch(const fdgs_moment8_args* a, void* stream, bool pack) {
             const fdgs_moment8_tensor& s = a->tensors[i];
             if (s.numel == 0) continue;
             k.start[k.num] = blocks;
-            blocks += (int)((s.numel + AW_PER_GROUP - 1) / AW_PER_GROUP);
+            blocks += (int)((s.numel + M8_PER_GROUP - 1) / M8_PER_GROUP);
             M8Tensor& t = k.t[k.num++];
             t.codes = s.codes; t.exps = s.exponents; t.value = s.value;
             t.n = s.numel; t.key = s.round_key; t.is_signed = s.is_signed != 0;

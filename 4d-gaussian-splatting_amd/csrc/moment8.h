@@ -25,9 +25,10 @@
 
 // 32 bits from an element's index and a tensor's key of the step.  Three odd multipliers from the fractions of the
 // golden ratio and of the roots of 2 and 3, with shifts in between that bring the high bits back down.
-__device__ __forceinline__ uint32_t m8_hash(uint32_t index_lo, uint32_t key_and_hi) {
-    uint32_t x = index_lo + key_and_hi;
-    x *= 0x9E3779B9u;
+// x0: (index + key) * M8_C1 of the element (the next element's is M8_C1 more)
+#define M8_C1 0x9E3779B9u
+__device__ __forceinline__ uint32_t m8_hash(uint32_t x0) {
+    uint32_t x = x0;
     x ^= x >> 16;
     x *= 0x6A09E667u;
     x ^= x >> 15;
@@ -49,36 +50,37 @@ __device__ __forceinline__ int m8_base(int e) {
     return b > 0 ? b : 0;
 }
 
+// The float32 pattern that a code stands for, in a block whose exponent is not 255 (the caller's NaN).
 template <bool SIGNED>
-__device__ __forceinline__ float m8_decode(uint32_t code, int e, int base) {
+__device__ __forceinline__ uint32_t m8_decode(uint32_t code, int base) {
     const uint32_t size = SIGNED ? (code & 127u) : code;
-    uint32_t bits = size ? (size + (uint32_t)base) << 20 : 0u;
-    if (SIGNED) bits |= (code & 128u) << 24;
-    return __uint_as_float(e == 255 ? 0x7FC00000u : bits);
+    const uint32_t bits = size ? (size + (uint32_t)base) << 20 : 0u;
+    return SIGNED ? bits | ((code & 128u) << 24) : bits;
 }
 
+// The code of x; the caller stores 0 in a block whose exponent is 255.
 template <bool SIGNED>
-__device__ __forceinline__ uint32_t m8_encode(float x, uint32_t noise, int e, int base) {
+__device__ __forceinline__ uint32_t m8_encode(float x, uint32_t noise, int base) {
     const uint32_t all = __float_as_uint(x), bits = all & 0x7FFFFFFFu;
-    int code = (int)((bits + noise) >> 20) - base;
-    if (SIGNED) {
-        code = code > 0 ? code : 0;
-        code |= (int)(all >> 24) & 128;
-    } else {
-        const int least = bits ? 1 : 0;
-        code = code > least ? code : least;
-    }
-    return e == 255 ? 0u : (uint32_t)code;
+    const int code = (int)((bits + noise) >> 20) - base;
+    if (SIGNED) return (uint32_t)(code > 0 ? code : 0) | ((all >> 24) & 128u);
+    const int least = (int)(bits < 1u ? bits : 1u);
+    return (uint32_t)(code > least ? code : least);
 }
 
 typedef unsigned short m8_u16x2 __attribute__((ext_vector_type(2)));
-// Largest of two 16-bit fields over a wave, in every lane: the exponents of both moments in one reduction.
+__device__ __forceinline__ uint32_t m8_max2(uint32_t v, uint32_t w) {
+    const m8_u16x2 a = __builtin_bit_cast(m8_u16x2, v), b = __builtin_bit_cast(m8_u16x2, w);
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(a, b));
+}
+// Largest of two 16-bit fields over the wave, the exponents of both moments in one reduction: neighbours, quads, rows of
+// 16 (a lane reads another of its row without going through LDS), then rows into the rows above; the last lane has it.
 __device__ __forceinline__ uint32_t m8_wave_max2(uint32_t v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        const uint32_t w = (uint32_t)__shfl_xor((int)v, o);
-        const m8_u16x2 a = __builtin_bit_cast(m8_u16x2, v), b = __builtin_bit_cast(m8_u16x2, w);
-        v = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(a, b));
-    }
-    return v;
+    v = m8_max2(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, true));    // quad: 1 0 3 2
+    v = m8_max2(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, true));    // quad: 2 3 0 1
+    v = m8_max2(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xF, 0xF, true));   // mirrored half rows
+    v = m8_max2(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xF, 0xF, true));   // mirrored rows
+    v = m8_max2(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xA, 0xF, true));   // rows 1 and 3: from 0 and 2
+    v = m8_max2(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xC, 0xF, true));   // rows 2 and 3: from row 1
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }

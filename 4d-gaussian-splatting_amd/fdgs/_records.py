@@ -1,18 +1,10 @@
 """Argument structures of the entry points over lists of tensors and over tables (fdgs_adamw_step, fdgs_moment8_*,
-fdgs_embedding_*): the ctypes side of include/fdgs.h, and the packed records of the per-tensor arrays.
-
-An array of records goes to the library in one piece: `struct` packs all its fields at once, which takes a fraction of
-the time of setting them one by one (a step over 200 tensors has 3000 of them)."""
+fdgs_embedding_*): the ctypes side of include/fdgs.h.  The arrays of per-tensor records that the list calls take are
+formed by fdgs._host (csrc/host.cpp) and handed over as bytes."""
 import ctypes as C
-import struct
 
 TYPE_F32, TYPE_BF16, TYPE_F16 = 0, 1, 2
 MOMENT8_BLOCK = 256
-
-# fdgs_adamw_tensor: seven pointers, numel, grad_row_stride, grad_row_len, step, lr, weight_decay, round_key, reserved
-ADAMW_TENSOR = "7Qqqiidd2I"
-# fdgs_moment8_tensor: codes, exponents, value, numel, is_signed, round_key
-MOMENT8_TENSOR = "3QqiI"
 
 
 class AdamWTensor(C.Structure):
@@ -52,17 +44,3 @@ class EmbeddingBwdArgs(C.Structure):
                 ("id_bytes", C.c_int32), ("ids", C.c_void_p), ("grad_out", C.c_void_p),
                 ("grad_out_row_stride", C.c_int64), ("padding_id", C.c_int64), ("grad_table", C.c_void_p),
                 ("scale", C.c_float), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
-
-
-_PACKERS = {}
-
-
-def pack(fmt, count, fields):
-    """A host array of `count` records with the format `fmt`, from the flat list of their fields."""
-    key = (fmt, count)
-    packer = _PACKERS.get(key)
-    if packer is None:
-        if len(_PACKERS) > 256:         # a program has a handful of list lengths
-            _PACKERS.clear()
-        packer = _PACKERS[key] = struct.Struct("=" + fmt * count)
-    return packer.pack(*fields)
