@@ -1,10 +1,13 @@
-// fdgs._host: the per-tensor host work of the entry points over lists of tensors.
+// fdgs._host: the host work of the entry points over lists of tensors, and the table lookup with its autograd function.
 //
 // A step over 200 tensors looks at 1400 tensors' types, sizes, layouts, devices and addresses.  From Python each look
 // costs 0.1 to 0.4 us, 5 to 7 us a tensor, several times what the GPU needs for the step; here the whole list costs
-// about 0.3 us a tensor.  Every check raises the Python exception that a caller sees; nothing is launched from here.
+// about 0.3 us a tensor.  Every check raises the Python exception that a caller sees.
+// The lookup of one token takes the GPU 4 us; its checks, output and call take 12 from Python, its training pass 130.
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <ATen/ATen.h>
+#include <c10/hip/HIPStream.h>
 #include <algorithm>
 #include <cstring>
 #include <stdexcept>
@@ -223,6 +226,252 @@ PyObject* moment8_records(PyObject* a) {
     return Py_BuildValue("Ni", bytes.give(), type == at::kBFloat16 ? FDGS_TYPE_BF16 : FDGS_TYPE_F32);
 }
 
+// ---- the table lookup ----
+using at::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+// The library that fdgs._lib has loaded (its functions' addresses), and that module: where its PROFILE is set every call
+// goes through its call_address(), which brackets it with events.
+struct Library {
+    int (*fwd)(const fdgs_embedding_fwd_args*, void*) = nullptr;
+    size_t (*ws)(int64_t, int32_t, int32_t, int32_t) = nullptr;
+    int (*bwd)(const fdgs_embedding_bwd_args*, void*) = nullptr;
+    const char* (*strerror)(int) = nullptr;
+    PyObject* module = nullptr;
+} library;
+
+template <class Args>
+void launch(const char* name, int (*fn)(const Args*, void*), const Args& a, const at::Device& device) {
+    const c10::DeviceGuard guard(device);
+    {
+        const PyGILState_STATE gil = PyGILState_Ensure();
+        PyObject* on = PyObject_GetAttrString(library.module, "PROFILE");
+        const bool profiled = on && on != Py_None;
+        Py_XDECREF(on);
+        PyObject* r = nullptr;
+        if (profiled) r = PyObject_CallMethod(library.module, "call_address", "sK", name, (unsigned long long)(uintptr_t)&a);
+        const bool failed = profiled && !r;
+        Py_XDECREF(r);
+        if (failed) PyErr_Clear();
+        PyGILState_Release(gil);
+        if (failed) throw std::runtime_error(std::string(name) + " failed in its profiled call");
+        if (profiled) return;
+    }
+    const int rc = fn(&a, (void*)c10::hip::getCurrentHIPStream(device.index()).stream());
+    if (rc != FDGS_OK) throw std::runtime_error(std::string(name) + ": " + library.strerror(rc) + " (" + std::to_string(rc) + ")");
+}
+
+int type_of(const Tensor& t, const char* what) {
+    switch (t.scalar_type()) {
+        case at::kFloat: return FDGS_TYPE_F32;
+        case at::kBFloat16: return FDGS_TYPE_BF16;
+        case at::kHalf: return FDGS_TYPE_F16;
+        default: value_error(std::string(what) + " is float32, bfloat16 or float16");
+    }
+}
+
+Tensor ids_of(const Tensor& ids, const at::Device& device) {
+    if (ids.scalar_type() != at::kInt && ids.scalar_type() != at::kLong) value_error("ids are int32 or int64");
+    if (ids.device() != device) value_error("ids and table have to be on one device");
+    return ids.contiguous();
+}
+
+// t [lead..., row...] with rows that are contiguous runs a constant, not negative distance apart: t itself where it is
+// laid out so, else a copy.
+Tensor rows_of(const Tensor& t, int64_t lead, int64_t& width, int64_t& stride) {
+    width = 1;
+    for (int64_t d = lead; d < t.dim(); ++d) width *= t.size(d);
+    stride = width;
+    if (t.is_contiguous()) return t;
+    int64_t run = 1;
+    bool ok = true;
+    for (int64_t d = t.dim() - 1; ok && d >= lead; --d) {
+        ok = t.size(d) == 1 || t.stride(d) == run;
+        run *= t.size(d);
+    }
+    int64_t step = -1, span = 0;                     // of the leading dimensions, those of one element left out
+    for (int64_t d = lead - 1; ok && d >= 0; --d) {
+        if (t.size(d) == 1) continue;
+        if (step < 0) step = t.stride(d);
+        else ok = t.stride(d) == span;
+        span = t.stride(d) * t.size(d);
+    }
+    if (!ok) return t.contiguous();
+    stride = step < 0 ? width : step;
+    return t;
+}
+
+Tensor lookup(const Tensor& ids0, const Tensor& table0, double scale, int64_t padding) {
+    const int type = type_of(table0, "the table");
+    const Tensor ids = ids_of(ids0, table0.device());
+    int64_t width, stride;
+    const Tensor table = rows_of(table0, 1, width, stride);
+    if (table.size(0) > INT32_MAX || width > INT32_MAX) value_error("the table has at most 2^31 - 1 rows and columns");
+    std::vector<int64_t> shape(ids.sizes().begin(), ids.sizes().end());
+    shape.insert(shape.end(), table.sizes().begin() + 1, table.sizes().end());
+    Tensor out = at::empty(shape, table.options());
+    fdgs_embedding_fwd_args a;
+    memset(&a, 0, sizeof(a));
+    a.num_tokens = ids.numel();
+    a.num_rows = (int32_t)table.size(0);
+    a.dim = (int32_t)width;
+    a.type = type;
+    a.id_bytes = (int32_t)ids.element_size();
+    a.ids = ids.data_ptr();
+    a.table = table.data_ptr();
+    a.table_row_stride = stride;
+    a.padding_id = padding;
+    a.out = out.data_ptr();
+    a.scale = (float)scale;
+    launch("fdgs_embedding_fwd", library.fwd, a, table.device());
+    return out;
+}
+
+Tensor table_grad(const Tensor& grad_out0, const Tensor& ids0, int64_t rows, double scale, int64_t padding) {
+    on_gpu(grad_out0);
+    const int type = type_of(grad_out0, "grad_out");
+    const Tensor ids = ids_of(ids0, grad_out0.device());
+    int64_t lead = ids.dim();
+    if (grad_out0.dim() <= lead || grad_out0.sizes().slice(0, lead) != ids.sizes()) value_error("grad_out has to be [*ids.shape, ...]");
+    if (rows < 0 || rows > INT32_MAX) value_error("num_rows is between 0 and 2^31 - 1");
+    std::vector<int64_t> shape{rows};
+    shape.insert(shape.end(), grad_out0.sizes().begin() + lead, grad_out0.sizes().end());
+    Tensor view = grad_out0;
+    if (lead == 0) {
+        view = grad_out0.unsqueeze(0);
+        lead = 1;
+    }
+    int64_t width, stride;
+    const Tensor g = rows_of(view, lead, width, stride);
+    if (width > INT32_MAX) value_error("a row has at most 2^31 - 1 columns");
+    Tensor out = at::empty(shape, g.options());
+    if (rows == 0 || width == 0) return out;
+    fdgs_embedding_bwd_args a;
+    memset(&a, 0, sizeof(a));
+    const size_t bytes = library.ws(ids.numel(), (int32_t)rows, (int32_t)width, type);
+    const Tensor workspace = at::empty({(int64_t)bytes}, g.options().dtype(at::kByte));
+    a.num_tokens = ids.numel();
+    a.num_rows = (int32_t)rows;
+    a.dim = (int32_t)width;
+    a.type = type;
+    a.id_bytes = (int32_t)ids.element_size();
+    a.ids = ids.data_ptr();
+    a.grad_out = g.data_ptr();
+    a.grad_out_row_stride = stride;
+    a.padding_id = padding;
+    a.grad_table = out.data_ptr();
+    a.scale = (float)scale;
+    a.workspace = workspace.data_ptr();
+    a.workspace_bytes = bytes;
+    launch("fdgs_embedding_bwd", library.bwd, a, g.device());
+    return out;
+}
+
+// The lookup is linear in the table and its gradient linear in grad_out, each the other's transpose: two functions that
+// are each other's backward pass, to any order.
+struct Lookup : torch::autograd::Function<Lookup> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& table, const Tensor& ids, double scale, int64_t padding);
+    static variable_list backward(AutogradContext* ctx, variable_list grads);
+};
+struct TableGrad : torch::autograd::Function<TableGrad> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& grad_out, const Tensor& ids, int64_t rows, double scale, int64_t padding);
+    static variable_list backward(AutogradContext* ctx, variable_list grads);
+};
+
+Tensor Lookup::forward(AutogradContext* ctx, const Tensor& table, const Tensor& ids, double scale, int64_t padding) {
+    ctx->save_for_backward({ids});
+    ctx->saved_data["rows"] = table.size(0);
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["padding"] = padding;
+    return lookup(ids, table, scale, padding);
+}
+variable_list Lookup::backward(AutogradContext* ctx, variable_list grads) {
+    const Tensor ids = ctx->get_saved_variables()[0];
+    const int64_t rows = ctx->saved_data["rows"].toInt(), padding = ctx->saved_data["padding"].toInt();
+    const double scale = ctx->saved_data["scale"].toDouble();
+    const bool graph = at::GradMode::is_enabled() && grads[0].requires_grad();
+    return {graph ? TableGrad::apply(grads[0], ids, rows, scale, padding) : table_grad(grads[0], ids, rows, scale, padding), Tensor(), Tensor(), Tensor()};
+}
+Tensor TableGrad::forward(AutogradContext* ctx, const Tensor& grad_out, const Tensor& ids, int64_t rows, double scale, int64_t padding) {
+    ctx->save_for_backward({ids});
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["padding"] = padding;
+    return table_grad(grad_out, ids, rows, scale, padding);
+}
+variable_list TableGrad::backward(AutogradContext* ctx, variable_list grads) {
+    const Tensor ids = ctx->get_saved_variables()[0];
+    const int64_t padding = ctx->saved_data["padding"].toInt();
+    const double scale = ctx->saved_data["scale"].toDouble();
+    const bool graph = at::GradMode::is_enabled() && grads[0].requires_grad();
+    return {graph ? Lookup::apply(grads[0], ids, scale, padding) : lookup(ids, grads[0], scale, padding), Tensor(), Tensor(), Tensor(), Tensor()};
+}
+
+int64_t padding_of(PyObject* o) {
+    if (o == Py_None) return -1;
+    Ref n(PyNumber_Index(o));
+    const long long v = PyLong_AsLongLong(n.p);
+    if (v == -1 && PyErr_Occurred()) throw Raised();
+    if (v < 0) value_error("padding_id is a row of the table; negative ids are padding always");
+    return v;
+}
+
+// embedding(ids, table, scale, padding_id | None)
+PyObject* embedding(PyObject* a) {
+    PyObject *io, *to, *po;
+    double scale;
+    if (!PyArg_ParseTuple(a, "OOdO", &io, &to, &scale, &po)) throw Raised();
+    const Tensor &ids = tensor(io, "ids"), &table = tensor(to, "the table");
+    if (table.dim() < 2) value_error("the table is [rows, ...] in float32, bfloat16 or float16");
+    type_of(table, "the table");
+    on_gpu(table);
+    const int64_t padding = padding_of(po);
+    Tensor out;
+    if (table.requires_grad() && at::GradMode::is_enabled()) {
+        ids_of(ids, table.device());                 // refused here, as the type that a caller expects
+        out = Lookup::apply(table, ids, scale, padding);
+    } else {
+        out = lookup(ids, table, scale, padding);
+    }
+    return THPVariable_Wrap(std::move(out));
+}
+
+// embedding_grad(grad_out, ids, num_rows, scale, padding_id | None)
+PyObject* embedding_grad(PyObject* a) {
+    PyObject *go, *io, *po;
+    long long rows;
+    double scale;
+    if (!PyArg_ParseTuple(a, "OOLdO", &go, &io, &rows, &scale, &po)) throw Raised();
+    const Tensor &g = tensor(go, "grad_out"), &ids = tensor(io, "ids");
+    return THPVariable_Wrap(table_grad(g, ids, rows, scale, padding_of(po)));
+}
+
+// rows_layout(tensor, lead) -> (read in place, width, stride): what rows_of() makes of a tensor
+PyObject* rows_layout(PyObject* a) {
+    PyObject* o;
+    long long lead;
+    if (!PyArg_ParseTuple(a, "OL", &o, &lead)) throw Raised();
+    const Tensor& t = tensor(o, "tensor");
+    int64_t width, stride;
+    const Tensor r = rows_of(t, lead, width, stride);
+    return Py_BuildValue("NLL", PyBool_FromLong(r.is_same(t)), (long long)width, (long long)stride);
+}
+
+// bind(module, addresses of fdgs_embedding_fwd, _bwd_workspace_bytes, _bwd and fdgs_strerror)
+PyObject* bind(PyObject* a) {
+    unsigned long long fwd, ws, bwd, err;
+    PyObject* module;
+    if (!PyArg_ParseTuple(a, "OKKKK", &module, &fwd, &ws, &bwd, &err)) throw Raised();
+    Py_INCREF(module);
+    Py_XDECREF(library.module);
+    library.module = module;
+    library.fwd = (decltype(library.fwd))(uintptr_t)fwd;
+    library.ws = (decltype(library.ws))(uintptr_t)ws;
+    library.bwd = (decltype(library.bwd))(uintptr_t)bwd;
+    library.strerror = (decltype(library.strerror))(uintptr_t)err;
+    Py_RETURN_NONE;
+}
+
 template <PyObject* (*F)(PyObject*)>
 PyObject* guarded(PyObject*, PyObject* args) {
     try {
@@ -232,6 +481,8 @@ PyObject* guarded(PyObject*, PyObject* args) {
         PyErr_SetString(r.type, r.what.c_str());
     } catch (const std::bad_alloc&) {
         PyErr_NoMemory();
+    } catch (const c10::Error& e) {
+        PyErr_SetString(PyExc_RuntimeError, e.what_without_backtrace());
     } catch (const std::exception& e) {
         PyErr_SetString(PyExc_RuntimeError, e.what());
     }
@@ -241,8 +492,12 @@ PyObject* guarded(PyObject*, PyObject* args) {
 PyMethodDef methods[] = {
     {"adamw_records", guarded<adamw_records>, METH_VARARGS, "the records of fdgs_adamw_step for lists of tensors"},
     {"moment8_records", guarded<moment8_records>, METH_VARARGS, "the records of fdgs_moment8_pack / unpack for lists of tensors"},
+    {"embedding", guarded<embedding>, METH_VARARGS, "the table lookup, with its gradient where the table wants one"},
+    {"embedding_grad", guarded<embedding_grad>, METH_VARARGS, "the gradient of the table alone"},
+    {"rows_layout", guarded<rows_layout>, METH_VARARGS, "how the rows of a tensor are read"},
+    {"bind", guarded<bind>, METH_VARARGS, "the library's entry points"},
     {nullptr, nullptr, 0, nullptr}};
-PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", "argument records of libfdgs's list calls", -1, methods, nullptr, nullptr, nullptr, nullptr};
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", "host work of libfdgs's calls over lists of tensors and tables", -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace
 

@@ -6,6 +6,7 @@ module raises.
 """
 import ctypes as C
 import os
+import sys
 
 import torch
 
@@ -298,6 +299,11 @@ def call_on(device, name, args):
             call(name, args)
 
 
+def call_address(name, address):
+    """call() with the address of an argument struct that stays valid for the call."""
+    call(name, getattr(lib, name).argtypes[0]._type_.from_address(address))
+
+
 def ptr(t):
     """Device pointer of a contiguous tensor (None -> NULL)."""
     if t is None:
@@ -336,3 +342,13 @@ def side_resources():
         res = _SIDE[key] = (side, fork, join)
     side, fork, join = res
     return side.cuda_stream, fork.cuda_event, join.cuda_event
+
+
+def _bind_host():
+    """Gives fdgs._host (csrc/host.cpp) the entry points it calls itself."""
+    from . import _host
+    _host.bind(sys.modules[__name__], *(C.cast(getattr(lib, n), c_p).value for n in (
+        "fdgs_embedding_fwd", "fdgs_embedding_bwd_workspace_bytes", "fdgs_embedding_bwd", "fdgs_strerror")))
+
+
+_bind_host()

@@ -163,13 +163,37 @@ def test_gradient_against_differences():
     assert float(((moved - y.detach()) * gy).double().sum()) == float((grad * step).double().sum())
 
 
-def test_gradient_twice_is_refused():
+def test_second_derivatives():
+    """sum(y^2 w) has the Hessian 2 scale^2 diag(sum of w): whole numbers, so exact."""
     from fdgs.embedding import embedding
-    table = torch.randn(4, 4, device="cuda", requires_grad=True)
-    y = embedding(torch.tensor([1, 2], device="cuda"), table)
-    with pytest.raises(RuntimeError):
-        g, = torch.autograd.grad((y * y).sum(), table, create_graph=True)
-        torch.autograd.grad(g.sum(), table)
+    g = torch.Generator().manual_seed(3)
+    ids = torch.randint(-1, 6, (50,), generator=g).cuda()
+    table = torch.randint(-4, 5, (6, 5), generator=g).float().cuda().requires_grad_(True)
+    w = torch.randint(-3, 4, (50, 5), generator=g).float().cuda()
+    u = torch.randint(-3, 4, (6, 5), generator=g).float().cuda()
+    y = embedding(ids, table, scale=2.0)
+    first, = torch.autograd.grad((y * y * w).sum(), table, create_graph=True)
+    second, = torch.autograd.grad((first * u).sum(), table, create_graph=True)
+    sums = torch.zeros(6, 5, device="cuda").index_add_(0, ids.clamp_min(0), w * (ids >= 0)[:, None])
+    assert torch.equal(first, 8 * sums * table) and torch.equal(second, 8 * sums * u)
+
+
+def test_profiled_calls():
+    """With _lib.PROFILE set the calls are bracketed with events, forward and backward."""
+    from fdgs import _lib
+    from fdgs.embedding import embedding
+    table = torch.randn(9, 4, device="cuda", requires_grad=True)
+    ids = torch.tensor([3, 3, 1], device="cuda")
+    plain = embedding(ids, table)
+    _lib.PROFILE = {}
+    try:
+        y = embedding(ids, table)
+        y.sum().backward()
+        seen = {k: len(v) for k, v in _lib.PROFILE.items()}
+    finally:
+        _lib.PROFILE = None
+    assert seen == {"fdgs_embedding_fwd": 1, "fdgs_embedding_bwd": 1}
+    assert torch.equal(y, plain) and table.grad.sum() == 12
 
 
 def test_two_captured_graphs_with_workspaces_of_their_own():

@@ -64,10 +64,9 @@ def test_cpu_tensors_are_refused():
 
 def test_rows_of_strided_gradients():
     """Which tensors are read in place, and with what distance between their rows."""
-    from fdgs.embedding import _rows
+    from fdgs._host import rows_layout
     base = torch.zeros(6, 5, 8)
     for t, lead, width, stride in ((base, 2, 8, 8), (base[..., 2:5], 2, 3, 8), (base[:, :1].expand(6, 5, 8), 2, 8, None),
                                    (base[:1, :1].expand(6, 5, 8), 2, 8, 0), (base[:, ::2, :4], 2, 4, None), (base[::2], 1, 40, 80),
                                    (base[:, 0], 1, 8, 40), (base.transpose(0, 1), 2, 8, None), (torch.zeros(()).expand(6, 5, 8), 2, 8, None)):
-        got, w, s = _rows(t, lead)
-        assert w == width and (got is t) == (stride is not None) and s == (width if stride is None else stride), (t.shape, t.stride())
+        assert rows_layout(t, lead) == (stride is not None, width, width if stride is None else stride), (t.shape, t.stride())
