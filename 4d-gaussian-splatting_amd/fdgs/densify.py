@@ -106,8 +106,8 @@ def surgery_apply(src, rows_after, rows_carried, arrays):
 class GaussianSurgery:
     """Binds the objects the reference's trainer edits: `gaussians` (attributes _xyz, _features_dc,
     _features_rest, _opacity, _scaling, _rotation, percent_dense), the optimizer (parameter groups named
-    xyz / f_dc / f_rest / opacity / scaling / rotation with one tensor each, torch.optim.Adam or
-    fdgs.adam.FusedAdam), `deforms` (deformation_table, deformation_accum; optional) and the holder of the
+    xyz / f_dc / f_rest / opacity / scaling / rotation with one tensor each, torch.optim.Adam,
+    fdgs.adam.FusedAdam or fdgs.adamw.FusedAdamW), `deforms` (deformation_table, deformation_accum; optional) and the holder of the
     statistics xyz_gradient_accum / denom / max_radii2D (the reference keeps them on `gaussians`)."""
 
     def __init__(self, gaussians, optimizer, deforms=None, stats=None, percent_dense=None, noise_fn=None):
@@ -137,13 +137,18 @@ class GaussianSurgery:
         new = nn.Parameter(tensor.requires_grad_(True))
         group["params"][0] = new
         if st is not None:
-            st["exp_avg"], st["exp_avg_sq"] = exp_avg, exp_avg_sq
+            if hasattr(self.optimizer, "set_moments"):      # fdgs.adamw.FusedAdamW: it may keep them in 8 bits
+                self.optimizer.set_moments(st, exp_avg, exp_avg_sq)
+            else:
+                st["exp_avg"], st["exp_avg_sq"] = exp_avg, exp_avg_sq
             self.optimizer.state[new] = st
         setattr(self.gaussians, _ATTR[name], new)
         return new
 
     def _moments(self, group):
         p = group["params"][0]
+        if hasattr(self.optimizer, "moments"):
+            return self.optimizer.moments(p)
         st = self.optimizer.state.get(p) if p in self.optimizer.state else None
         if st is None or "exp_avg" not in st:
             return None

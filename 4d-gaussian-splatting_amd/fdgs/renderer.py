@@ -5,7 +5,9 @@
 `pc` is any object with the GaussianModel tensor layout
 (src/model/gaussian_model.py:70-89: get_xyz, _scaling, _rotation, _opacity,
 get_features, active_sh_degree, the three activation callables); `deforms` is
-any object whose `deformation_fields` is callable like DeformationFields.
+any object whose `deformation_fields` is callable like DeformationFields.  A model
+with a `feature_codebook` (fdgs.embedding.FeatureCodebook) has its SH coefficients
+from there, in place of get_features.
 
 The reference forwards `shs` together with `colors_precomp` when
 `override_color` / `convert_SHs_python` are used (:89-113), which its
@@ -18,6 +20,7 @@ import torch
 
 from . import _lib
 from . import deformation as _deformation
+from .embedding import FeatureCodebook
 from .rasterizer import GaussianRasterizationSettings, GaussianRasterizer
 
 
@@ -53,15 +56,18 @@ def prepare(viewpoint_camera, pc, deforms, bg_color: torch.Tensor, scaling_modif
 
     means2D = screenspace_points
     opacity = pc._opacity
+    codebook = getattr(pc, "feature_codebook", None)
+    codebook = codebook if isinstance(codebook, FeatureCodebook) else None
     # Without gradients, with this package's deformation field and a model that keeps the SH coefficients as the
     # reference's GaussianModel does, the two tensors go to the deformation kernel as they are: get_features is a
     # concatenation into a fresh [N,16,3] tensor on every call (gaussian_model.py:86-89)
     split_sh = ("fine" in stage and not torch.is_grad_enabled() and override_color is None and not convert_SHs_python
-                and isinstance(getattr(deforms, "deformation_fields", None), _deformation.DeformationFields)
+                and codebook is None and isinstance(getattr(deforms, "deformation_fields", None), _deformation.DeformationFields)
                 and isinstance(getattr(pc, "_features_dc", None), torch.Tensor)
                 and isinstance(getattr(pc, "_features_rest", None), torch.Tensor)
                 and pc._features_dc.dim() == 3 and pc._features_dc.shape[1] == 1 and pc._features_rest.shape[1] == 15)
-    shs = _deformation.SplitSH(pc._features_dc, pc._features_rest) if split_sh else pc.get_features
+    shs = _deformation.SplitSH(pc._features_dc, pc._features_rest) if split_sh else \
+        pc.get_features if codebook is None else codebook()
     scales = None
     rotations = None
     cov3D_precomp = None
@@ -108,8 +114,8 @@ def prepare(viewpoint_camera, pc, deforms, bg_color: torch.Tensor, scaling_modif
     if override_color is None:
         if convert_SHs_python:      # SH -> RGB on the host side, as gaussian_renderer/__init__.py:91-96
             from .sh import eval_sh
-            shs_view = pc.get_features.transpose(1, 2).view(-1, 3, (pc.max_sh_degree + 1) ** 2)
-            dir_pp = pc.get_xyz - viewpoint_camera.camera_center.to(dev).repeat(pc.get_features.shape[0], 1)
+            shs_view = shs.transpose(1, 2).view(-1, 3, (pc.max_sh_degree + 1) ** 2)
+            dir_pp = pc.get_xyz - viewpoint_camera.camera_center.to(dev).repeat(shs.shape[0], 1)
             dir_pp_normalized = dir_pp / dir_pp.norm(dim=1, keepdim=True)
             sh2rgb = eval_sh(pc.active_sh_degree, shs_view, dir_pp_normalized)
             colors_precomp = torch.clamp_min(sh2rgb + 0.5, 0.0)

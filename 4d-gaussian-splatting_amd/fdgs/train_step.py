@@ -9,6 +9,7 @@ import os
 import torch
 
 from . import _lib, dp, losses, schedule
+from .embedding import FeatureCodebook
 from .renderer import render
 
 
@@ -25,7 +26,12 @@ class TrainStep:
     DYNERF_REGULATION = (0.001, 0.0001, 0.0002)
 
     def __init__(self, gaussians, deforms, background, lr_scale=1.0, stage="fine", fused_adam=True,
-                 regulation=DYNERF_REGULATION, lambda_dssim=0.0):
+                 regulation=DYNERF_REGULATION, lambda_dssim=0.0, adamw=None):
+        """adamw: None for the reference's Adam, or a dict of fdgs.adamw.FusedAdamW's arguments (state_bits, weight_decay,
+        betas, eps, seed; weight_decay 0 and eps 1e-15 unless given) to step the same groups with it.  A model with a
+        `feature_codebook` (fdgs.embedding.FeatureCodebook) has one group "codebook" in place of f_dc and f_rest."""
+        codebook = getattr(gaussians, "feature_codebook", None)
+        self.codebook = codebook if isinstance(codebook, FeatureCodebook) else None
         self.g, self.deforms, self.bg, self.stage = gaussians, deforms, background, stage
         self.lambda_dssim = float(lambda_dssim)     # configs/train/dynerf.yaml:36 ships 0
         self.last_psnr = None                       # fdgs_trainer.py:131: mean PSNR of the local views, on device
@@ -37,14 +43,18 @@ class TrainStep:
             {"params": [gaussians._xyz], "lr": 0.00016 * lr_scale, "name": "xyz"},
             {"params": list(df.get_mlp_parameters()), "lr": 0.00016 * lr_scale, "name": "deformation"},
             {"params": list(df.get_grid_parameters()), "lr": 0.0016 * lr_scale, "name": "grid"},
-            {"params": [gaussians._features_dc], "lr": 0.0025, "name": "f_dc"},
-            {"params": [gaussians._features_rest], "lr": 0.0025 / 20.0, "name": "f_rest"},
+            *([{"params": [gaussians._features_dc], "lr": 0.0025, "name": "f_dc"},
+               {"params": [gaussians._features_rest], "lr": 0.0025 / 20.0, "name": "f_rest"}] if self.codebook is None else
+              [{"params": [self.codebook.table], "lr": 0.0025, "name": "codebook"}]),
             {"params": [gaussians._opacity], "lr": 0.05, "name": "opacity"},
             {"params": [gaussians._scaling], "lr": 0.005, "name": "scaling"},
             {"params": [gaussians._rotation], "lr": 0.001, "name": "rotation"},
         ]
         _lib.require_gpu(gaussians._xyz)    # every kernel of the step lives in libfdgs.so: there is no CPU path
-        if fused_adam:                      # one launch for all 40 tensors
+        if adamw is not None:
+            from .adamw import FusedAdamW
+            self.optimizer = FusedAdamW(groups, **{"lr": 0.0, "eps": 1e-15, "weight_decay": 0.0, **adamw})
+        elif fused_adam:                    # one launch for all 40 tensors
             from .adam import FusedAdam
             self.optimizer = FusedAdam(groups, lr=0.0, eps=1e-15)
         else:
@@ -70,7 +80,7 @@ class TrainStep:
         self.params = [p for grp in self.optimizer.param_groups for p in grp["params"]]
         self.bucket = dp.GradBucket(self.params)
         # the SH gradients can be exchanged early (fdgs.deformation.RESIDUAL_GRAD_HOOK); the rest then goes here
-        sh_ids = {id(self.g._features_dc), id(self.g._features_rest)}
+        sh_ids = {id(getattr(self.g, k, None)) for k in ("_features_dc", "_features_rest")}
         self.bucket_without_sh = dp.GradBucket([p for p in self.params if id(p) not in sh_ids])
 
     # -- densification / pruning between steps (fdgs_trainer.py:191-200) --------------------------------
@@ -239,7 +249,9 @@ class TrainStep:
         # the same number of views on every rank (so all ranks take this branch together): after a rank's last
         # view's rasterizer backward everything but the deformation field's and the positions' gradients is complete
         # and is exchanged while that view's deformation backward runs
-        if views and dp.is_dist() and len(global_views) % dp.rank_world()[1] == 0 and self.early_exchange:
+        # (not with a codebook: its gradient is [V,16,3], formed behind the [N,16,3] one that the hook would exchange)
+        if views and dp.is_dist() and len(global_views) % dp.rank_world()[1] == 0 and self.early_exchange \
+                and self.codebook is None:
             def hook(g_sh):             # autograd route (one view per rank): the SH gradient
                 try:
                     work = dp.all_reduce_async(g_sh)
@@ -259,7 +271,7 @@ class TrainStep:
                     return None
                 early.append(("range", buf, r, work_r))
                 return work
-        direct = (self.use_pipeline and self.lambda_dssim == 0 and self.pipeline.usable(self.stage)
+        direct = (self.use_pipeline and self.codebook is None and self.lambda_dssim == 0 and self.pipeline.usable(self.stage)
                   and all(getattr(c, "original_image", None) is not None for c in views))
         if direct:
             # the regulariser depends on no view: it is enqueued inside the first view's forward, where the host

@@ -119,3 +119,29 @@ def test_split_of_a_weight_is_exact():
     hi, lo = ac.split_bf16(w)
     back = ((hi.astype(np.int64) << 16) + lo.astype(np.int64)).astype(np.uint32).view(np.float32)
     assert np.array_equal(back.view(np.uint32), w.view(np.uint32))
+
+
+def test_optimizer_refuses_what_it_does_not_do():
+    from fdgs.adamw import FusedAdamW
+    p = torch.zeros(4, requires_grad=True)
+    for bad, match in ((dict(state_bits=16), "8 or 32"), (dict(betas=(1.0, 0.9)), "betas"), (dict(eps=-1.0), "betas")):
+        with pytest.raises(ValueError, match=match):
+            FusedAdamW([p], **bad)
+    for key in ("amsgrad", "maximize"):
+        with pytest.raises(ValueError, match="amsgrad"):
+            FusedAdamW([{"params": [p], key: True}])
+    with pytest.raises(ValueError, match="twice"):
+        FusedAdamW([{"params": [p]}, {"params": [p]}])
+    opt = FusedAdamW([p])
+    opt.step()                                   # nothing has a gradient
+    p.grad = torch.ones(4)
+    with pytest.raises(RuntimeError, match="GPU only"):
+        opt.step()
+    assert opt.state == {} and opt.state_dict()["state"] == {}
+    with pytest.raises(ValueError, match="different parameter groups"):
+        opt.load_state_dict({"state": {}, "param_groups": []})
+    opt.zero_grad(set_to_none=False)
+    assert (p.grad == 0).all()
+    half = torch.zeros(4, dtype=torch.float16)
+    with pytest.raises(ValueError, match="float32 and bfloat16"):
+        FusedAdamW([half])._new_state(half)
