@@ -1,4 +1,4 @@
-// fdgs._host: the host work of the entry points over lists of tensors, and the table lookup with its autograd function.
+// fdgs._host: the calls over lists of tensors from the lists on, and the table lookup with its autograd function.
 //
 // A step over 200 tensors looks at 1400 tensors' types, sizes, layouts, devices and addresses.  From Python each look
 // costs 0.1 to 0.4 us, 5 to 7 us a tensor, several times what the GPU needs for the step; here the whole list costs
@@ -7,6 +7,7 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <ATen/ATen.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <algorithm>
 #include <cstring>
@@ -93,15 +94,52 @@ void on_gpu(const at::Tensor& t) {
     if (!t.is_cuda()) throw Refused{PyExc_RuntimeError, "libfdgs kernels run on the GPU only; got a tensor on " + t.device().str()};
 }
 
-// adamw_records(params, grads, exp_avgs, exp_avg_sqs, residuals | None, steps, lr, weight_decay, keys | None, Moment8)
-//   -> (records, param type, state bits, copies of gradients to keep until the launch)
-PyObject* adamw_records(PyObject* a) {
+using at::Tensor;
+
+// The library that fdgs._lib has loaded (its functions' addresses), and that module: where its PROFILE is set every call
+// goes through its call_address(), which brackets it with events.
+struct Library {
+    int (*fwd)(const fdgs_embedding_fwd_args*, void*) = nullptr;
+    size_t (*ws)(int64_t, int32_t, int32_t, int32_t) = nullptr;
+    int (*bwd)(const fdgs_embedding_bwd_args*, void*) = nullptr;
+    int (*adamw)(const fdgs_adamw_args*, void*) = nullptr;
+    int (*unpack8)(const fdgs_moment8_args*, void*) = nullptr;
+    int (*pack8)(const fdgs_moment8_args*, void*) = nullptr;
+    const char* (*strerror)(int) = nullptr;
+    PyObject* module = nullptr;
+} library;
+
+template <class Args>
+void launch(const char* name, int (*fn)(const Args*, void*), const Args& a, const at::Device& device) {
+    const c10::DeviceGuard guard(device);
+    {
+        const PyGILState_STATE gil = PyGILState_Ensure();
+        PyObject* on = PyObject_GetAttrString(library.module, "PROFILE");
+        const bool profiled = on && on != Py_None;
+        Py_XDECREF(on);
+        PyObject* r = nullptr;
+        if (profiled) r = PyObject_CallMethod(library.module, "call_address", "sK", name, (unsigned long long)(uintptr_t)&a);
+        const bool failed = profiled && !r;
+        Py_XDECREF(r);
+        if (failed) PyErr_Clear();
+        PyGILState_Release(gil);
+        if (failed) throw std::runtime_error(std::string(name) + " failed in its profiled call");
+        if (profiled) return;
+    }
+    const int rc = fn(&a, (void*)c10::hip::getCurrentHIPStream(device.index()).stream());
+    if (rc != FDGS_OK) throw std::runtime_error(std::string(name) + ": " + library.strerror(rc) + " (" + std::to_string(rc) + ")");
+}
+
+// adamw_step(params, grads, exp_avgs, exp_avg_sqs, residuals | None, steps, lr, weight_decay, keys | None, Moment8,
+//            beta1, beta2, eps)
+PyObject* adamw_step(PyObject* a) {
     PyObject *po, *go, *mo, *vo, *ro, *so, *lo, *wo, *ko, *cls;
-    if (!PyArg_ParseTuple(a, "OOOOOOOOOO", &po, &go, &mo, &vo, &ro, &so, &lo, &wo, &ko, &cls)) throw Raised();
+    double beta1, beta2, eps;
+    if (!PyArg_ParseTuple(a, "OOOOOOOOOOddd", &po, &go, &mo, &vo, &ro, &so, &lo, &wo, &ko, &cls, &beta1, &beta2, &eps)) throw Raised();
     List p(po), g(go), m(mo), v(vo);
     const Py_ssize_t n = p.size();
     if (g.size() != n || m.size() != n || v.size() != n) value_error("params, grads and moments have to be lists of the same length");
-    if (n == 0) value_error("no tensors");
+    if (n == 0) Py_RETURN_NONE;
     const Each steps(so, n, "steps"), lr(lo, n, "lr"), wd(wo, n, "weight_decay");
     const at::Tensor& first = tensor(p.at(0), "params");
     const at::ScalarType type = first.scalar_type();
@@ -109,17 +147,16 @@ PyObject* adamw_records(PyObject* a) {
     const bool bf16 = type == at::kBFloat16;
     if (!bf16 && type != at::kFloat) value_error("adamw_step takes float32 and bfloat16 parameters, not " + name_of(first));
     on_gpu(first);
-    Py_ssize_t nr = 0;
-    std::vector<PyObject*> low;
+    const c10::DeviceGuard guard(device);
+    if (c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None)
+        throw Refused{PyExc_RuntimeError, "adamw_step reads its step counts on the host and cannot be captured into a graph"};
     Ref rseq(ro == Py_None ? PyTuple_New(0) : PySequence_Fast(ro, "residuals: a list of tensors is needed"));
-    nr = PySequence_Fast_GET_SIZE(rseq.p);
-    if (bf16 && nr != n) value_error("bfloat16 parameters need residuals: an int16 tensor for each");
+    if (bf16 && PySequence_Fast_GET_SIZE(rseq.p) != n) value_error("bfloat16 parameters need residuals: an int16 tensor for each");
     const bool eight = is_moment(m.at(0), cls);
     if (eight && (ko == Py_None || !(PyList_Check(ko) || PyTuple_Check(ko)) || PySequence_Fast_GET_SIZE(ko) != n))
         value_error("8-bit moments need keys: a number for each tensor, others at every step");
-    Ref hold(PyList_New(0));
-    Ref bytes(PyBytes_FromStringAndSize(nullptr, n * (Py_ssize_t)sizeof(fdgs_adamw_tensor)));
-    fdgs_adamw_tensor* out = (fdgs_adamw_tensor*)PyBytes_AS_STRING(bytes.p);
+    std::vector<Tensor> hold;                        // copies of gradients, kept until the kernels are on the stream
+    std::vector<fdgs_adamw_tensor> out(n);
     std::vector<uintptr_t> written;
     written.reserve(3 * n);
     for (Py_ssize_t i = 0; i < n; ++i) {
@@ -144,10 +181,8 @@ PyObject* adamw_records(PyObject* a) {
                 r.grad_row_len = (int32_t)len;
                 r.grad_row_stride = gt.stride(0);
             } else {
-                const at::Tensor copy = gt.detach().contiguous();
-                r.grad = copy.data_ptr();
-                Ref held(THPVariable_Wrap(copy));
-                if (PyList_Append(hold.p, held.p) < 0) throw Raised();
+                hold.push_back(gt.detach().contiguous());
+                r.grad = hold.back().data_ptr();
             }
         }
         if (eight) {
@@ -191,13 +226,24 @@ PyObject* adamw_records(PyObject* a) {
     }
     std::sort(written.begin(), written.end());
     if (std::adjacent_find(written.begin(), written.end()) != written.end()) value_error("a tensor is in the lists twice");
-    return Py_BuildValue("NiiN", bytes.give(), bf16 ? FDGS_TYPE_BF16 : FDGS_TYPE_F32, eight ? 8 : 32, hold.give());
+    fdgs_adamw_args args;
+    memset(&args, 0, sizeof(args));
+    args.num_tensors = (int32_t)n;
+    args.param_type = bf16 ? FDGS_TYPE_BF16 : FDGS_TYPE_F32;
+    args.state_bits = eight ? 8 : 32;
+    args.beta1 = beta1;
+    args.beta2 = beta2;
+    args.eps = eps;
+    args.tensors = out.data();
+    launch("fdgs_adamw_step", library.adamw, args, device);
+    Py_RETURN_NONE;
 }
 
-// moment8_records(moments, values, keys | None, Moment8) -> (records, value type)
-PyObject* moment8_records(PyObject* a) {
+// moment8(pack, moments, values, keys | None, Moment8): values -> moments (to the nearest without keys), or back
+PyObject* moment8_convert(PyObject* a) {
     PyObject *mo, *vo, *ko, *cls;
-    if (!PyArg_ParseTuple(a, "OOOO", &mo, &vo, &ko, &cls)) throw Raised();
+    int pack;
+    if (!PyArg_ParseTuple(a, "pOOOO", &pack, &mo, &vo, &ko, &cls)) throw Raised();
     List m(mo), v(vo);
     const Py_ssize_t n = m.size();
     if (n == 0 || v.size() != n) value_error("a tensor of values is needed for each moment");
@@ -206,8 +252,7 @@ PyObject* moment8_records(PyObject* a) {
     const at::ScalarType type = first.scalar_type();
     if (type != at::kFloat && type != at::kBFloat16) value_error("the values of 8-bit moments are float32 or bfloat16");
     on_gpu(first);
-    Ref bytes(PyBytes_FromStringAndSize(nullptr, n * (Py_ssize_t)sizeof(fdgs_moment8_tensor)));
-    fdgs_moment8_tensor* out = (fdgs_moment8_tensor*)PyBytes_AS_STRING(bytes.p);
+    std::vector<fdgs_moment8_tensor> out(n);
     for (Py_ssize_t i = 0; i < n; ++i) {
         const at::Tensor& t = tensor(v.at(i), "values");
         if (t.scalar_type() != type || t.device() != first.device() || !t.is_contiguous())
@@ -223,44 +268,19 @@ PyObject* moment8_records(PyObject* a) {
         r.round_key = ko == Py_None ? 0u : keys.low32(i);
         out[i] = r;
     }
-    return Py_BuildValue("Ni", bytes.give(), type == at::kBFloat16 ? FDGS_TYPE_BF16 : FDGS_TYPE_F32);
+    fdgs_moment8_args args;
+    memset(&args, 0, sizeof(args));
+    args.num_tensors = (int32_t)n;
+    args.value_type = type == at::kBFloat16 ? FDGS_TYPE_BF16 : FDGS_TYPE_F32;
+    args.nearest = ko == Py_None;
+    args.tensors = out.data();
+    launch(pack ? "fdgs_moment8_pack" : "fdgs_moment8_unpack", pack ? library.pack8 : library.unpack8, args, first.device());
+    Py_RETURN_NONE;
 }
 
 // ---- the table lookup ----
-using at::Tensor;
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
-
-// The library that fdgs._lib has loaded (its functions' addresses), and that module: where its PROFILE is set every call
-// goes through its call_address(), which brackets it with events.
-struct Library {
-    int (*fwd)(const fdgs_embedding_fwd_args*, void*) = nullptr;
-    size_t (*ws)(int64_t, int32_t, int32_t, int32_t) = nullptr;
-    int (*bwd)(const fdgs_embedding_bwd_args*, void*) = nullptr;
-    const char* (*strerror)(int) = nullptr;
-    PyObject* module = nullptr;
-} library;
-
-template <class Args>
-void launch(const char* name, int (*fn)(const Args*, void*), const Args& a, const at::Device& device) {
-    const c10::DeviceGuard guard(device);
-    {
-        const PyGILState_STATE gil = PyGILState_Ensure();
-        PyObject* on = PyObject_GetAttrString(library.module, "PROFILE");
-        const bool profiled = on && on != Py_None;
-        Py_XDECREF(on);
-        PyObject* r = nullptr;
-        if (profiled) r = PyObject_CallMethod(library.module, "call_address", "sK", name, (unsigned long long)(uintptr_t)&a);
-        const bool failed = profiled && !r;
-        Py_XDECREF(r);
-        if (failed) PyErr_Clear();
-        PyGILState_Release(gil);
-        if (failed) throw std::runtime_error(std::string(name) + " failed in its profiled call");
-        if (profiled) return;
-    }
-    const int rc = fn(&a, (void*)c10::hip::getCurrentHIPStream(device.index()).stream());
-    if (rc != FDGS_OK) throw std::runtime_error(std::string(name) + ": " + library.strerror(rc) + " (" + std::to_string(rc) + ")");
-}
 
 int type_of(const Tensor& t, const char* what) {
     switch (t.scalar_type()) {
@@ -457,17 +477,21 @@ PyObject* rows_layout(PyObject* a) {
     return Py_BuildValue("NLL", PyBool_FromLong(r.is_same(t)), (long long)width, (long long)stride);
 }
 
-// bind(module, addresses of fdgs_embedding_fwd, _bwd_workspace_bytes, _bwd and fdgs_strerror)
+// bind(module, addresses of fdgs_embedding_fwd, _bwd_workspace_bytes, _bwd, fdgs_adamw_step, fdgs_moment8_unpack, _pack and
+// fdgs_strerror)
 PyObject* bind(PyObject* a) {
-    unsigned long long fwd, ws, bwd, err;
+    unsigned long long fwd, ws, bwd, adamw, unpack, pack, err;
     PyObject* module;
-    if (!PyArg_ParseTuple(a, "OKKKK", &module, &fwd, &ws, &bwd, &err)) throw Raised();
+    if (!PyArg_ParseTuple(a, "OKKKKKKK", &module, &fwd, &ws, &bwd, &adamw, &unpack, &pack, &err)) throw Raised();
     Py_INCREF(module);
     Py_XDECREF(library.module);
     library.module = module;
     library.fwd = (decltype(library.fwd))(uintptr_t)fwd;
     library.ws = (decltype(library.ws))(uintptr_t)ws;
     library.bwd = (decltype(library.bwd))(uintptr_t)bwd;
+    library.adamw = (decltype(library.adamw))(uintptr_t)adamw;
+    library.unpack8 = (decltype(library.unpack8))(uintptr_t)unpack;
+    library.pack8 = (decltype(library.pack8))(uintptr_t)pack;
     library.strerror = (decltype(library.strerror))(uintptr_t)err;
     Py_RETURN_NONE;
 }
@@ -490,8 +514,8 @@ PyObject* guarded(PyObject*, PyObject* args) {
 }
 
 PyMethodDef methods[] = {
-    {"adamw_records", guarded<adamw_records>, METH_VARARGS, "the records of fdgs_adamw_step for lists of tensors"},
-    {"moment8_records", guarded<moment8_records>, METH_VARARGS, "the records of fdgs_moment8_pack / unpack for lists of tensors"},
+    {"adamw_step", guarded<adamw_step>, METH_VARARGS, "fdgs_adamw_step for lists of tensors"},
+    {"moment8", guarded<moment8_convert>, METH_VARARGS, "fdgs_moment8_pack / unpack for lists of tensors"},
     {"embedding", guarded<embedding>, METH_VARARGS, "the table lookup, with its gradient where the table wants one"},
     {"embedding_grad", guarded<embedding_grad>, METH_VARARGS, "the gradient of the table alone"},
     {"rows_layout", guarded<rows_layout>, METH_VARARGS, "how the rows of a tensor are read"},

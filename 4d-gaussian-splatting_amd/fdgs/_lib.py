@@ -290,15 +290,6 @@ def call(name, args):
     check(rc, name)
 
 
-def call_on(device, name, args):
-    """call() with `device` as the current one: the stream is then a stream of the device the tensors are on."""
-    if device.index == torch.cuda.current_device():
-        call(name, args)
-    else:
-        with torch.cuda.device(device):
-            call(name, args)
-
-
 def call_address(name, address):
     """call() with the address of an argument struct that stays valid for the call."""
     call(name, getattr(lib, name).argtypes[0]._type_.from_address(address))
@@ -348,7 +339,8 @@ def _bind_host():
     """Gives fdgs._host (csrc/host.cpp) the entry points it calls itself."""
     from . import _host
     _host.bind(sys.modules[__name__], *(C.cast(getattr(lib, n), c_p).value for n in (
-        "fdgs_embedding_fwd", "fdgs_embedding_bwd_workspace_bytes", "fdgs_embedding_bwd", "fdgs_strerror")))
+        "fdgs_embedding_fwd", "fdgs_embedding_bwd_workspace_bytes", "fdgs_embedding_bwd", "fdgs_adamw_step", "fdgs_moment8_unpack",
+        "fdgs_moment8_pack", "fdgs_strerror")))
 
 
 _bind_host()

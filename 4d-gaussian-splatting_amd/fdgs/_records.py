@@ -1,6 +1,6 @@
 """Argument structures of the entry points over lists of tensors and over tables (fdgs_adamw_step, fdgs_moment8_*,
-fdgs_embedding_*): the ctypes side of include/fdgs.h.  The arrays of per-tensor records that the list calls take are
-formed by fdgs._host (csrc/host.cpp) and handed over as bytes."""
+fdgs_embedding_*): the ctypes side of include/fdgs.h.  The package makes these calls from fdgs._host (csrc/host.cpp);
+the structures here are for a caller of the C ABI, and for calls that are profiled."""
 import ctypes as C
 
 TYPE_F32, TYPE_BF16, TYPE_F16 = 0, 1, 2

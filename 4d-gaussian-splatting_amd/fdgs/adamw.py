@@ -57,34 +57,8 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, steps, lr, betas=(0.9, 0
     All tensors are on one GPU, have one type, do not overlap, and the step runs on its current stream.  Tensors
     without elements are passed over.  The call reads steps, lr and keys on the host: a captured graph would replay
     the ones it was captured with, so a stream that is being captured is refused."""
-    if not len(params) == len(grads) == len(exp_avgs) == len(exp_avg_sqs):
-        raise ValueError("params, grads and moments have to be lists of the same length")
-    if not len(params):
-        return
-    device = params[0].device
-    if device.type == "cuda":
-        _no_capture(device, "adamw_step")
-    records, kind, bits, hold = _host.adamw_records(params, grads, exp_avgs, exp_avg_sqs, residuals, steps, lr, weight_decay,
-                                                    keys, Moment8)
-    b1, b2 = betas
-    _lib.call_on(device, "fdgs_adamw_step", _records.AdamWArgs(len(params), kind, bits, 0, b1, b2, eps, records))
+    _host.adamw_step(params, grads, exp_avgs, exp_avg_sqs, residuals, steps, lr, weight_decay, keys, Moment8, *betas, eps)
     GENERATION[0] += 1
-    del hold                                     # copies of gradients: kept until the kernels were on the stream
-
-
-def _no_capture(device, what):
-    if device.index == torch.cuda.current_device():
-        capturing = torch.cuda.is_current_stream_capturing()
-    else:
-        with torch.cuda.device(device):
-            capturing = torch.cuda.is_current_stream_capturing()
-    if capturing:
-        raise RuntimeError(f"{what} reads its step counts on the host and cannot be captured into a graph")
-
-
-def _moment8_call(name, moments, values, nearest, keys):
-    records, kind = _host.moment8_records(moments, values, keys, Moment8)
-    _lib.call_on(values[0].device, name, _records.Moment8Args(len(moments), kind, 1 if nearest else 0, 0, records))
 
 
 def unpack8(moments, dtype=torch.float32, out=None):
@@ -95,7 +69,7 @@ def unpack8(moments, dtype=torch.float32, out=None):
         return []
     if out is None:
         out = [torch.empty(x.codes.shape, dtype=dtype, device=x.codes.device) for x in moments]
-    _moment8_call("fdgs_moment8_unpack", moments, out, False, None)
+    _host.moment8(False, moments, out, None, Moment8)
     return list(out)
 
 
@@ -116,7 +90,7 @@ def pack8(values, signed, keys=None):
             raise ValueError("pack8 takes float32 tensors on one device")
         out.append(Moment8(torch.empty_like(t, dtype=torch.uint8),
                            torch.empty(-(-t.numel() // BLOCK), dtype=torch.uint8, device=device), bool(s)))
-    _moment8_call("fdgs_moment8_pack", out, values, keys is None, keys)
+    _host.moment8(True, out, values, keys, Moment8)
     return out
 
 
