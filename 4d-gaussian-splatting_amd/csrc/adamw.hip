@@ -15,9 +15,11 @@
 #include "moment8.h"
 
 #define AW_MAX 40                                // tensors per launch: their records fill 4 KB of kernel arguments
-#define AW_BLOCKS 2                               // blocks of 256 per wave
-#define AW_PER_WAVE (AW_BLOCKS * 256)
-#define AW_PER_GROUP (4 * AW_PER_WAVE)           // elements per workgroup of four waves
+// Blocks of 256 per wave, and elements per workgroup of four waves.  One block with float32 moments (97 bfloat16 tensors:
+// 203 us, 213 with two, 232 with four), two with 8-bit ones (2,000,000 Gaussians: 405 us, 418 with one, 405 with four; 211
+// bfloat16 tensors 157, 157, 198).
+static constexpr int aw_blocks(bool eight) { return eight ? 2 : 1; }
+static constexpr int aw_per_group(bool eight) { return 4 * 256 * aw_blocks(eight); }
 
 struct AwTensor {
     void* p; const void* g; void* m; void* v;
@@ -36,22 +38,61 @@ struct AwPart {
 static_assert(sizeof(AwPart) <= 4096, "kernel arguments of one launch");
 
 struct __attribute__((packed, aligned(4))) aw_f4 { float x[4]; };
-struct __attribute__((packed, aligned(2))) aw_h4 { uint16_t x[4]; };
-struct __attribute__((packed, aligned(1))) aw_b4 { uint32_t x; };
+struct __attribute__((packed, aligned(2))) aw_h4 { uint32_t x[2]; };   // four 16-bit numbers, two to a word
 struct __attribute__((packed, aligned(1))) aw_b8 { uint32_t x[2]; };
 struct __attribute__((packed, aligned(2))) aw_w4 { uint32_t x[4]; };
 
+// Streaming accesses for what only the optimizer touches (moments, residuals) and for the gradient, which is used up:
+// they leave the caches to the parameters, which the next forward pass reads.  At 300,000 Gaussians 108 -> 99 us.
+typedef uint32_t aw_u4 __attribute__((ext_vector_type(4)));
+typedef uint32_t aw_u2 __attribute__((ext_vector_type(2)));
+typedef aw_u4 aw_u4_at4 __attribute__((aligned(4)));
+typedef aw_u2 aw_u2_at2 __attribute__((aligned(2)));
+typedef uint32_t aw_u1_at1 __attribute__((aligned(1)));
+__device__ __forceinline__ aw_f4 aw_take(const float* p) { return __builtin_bit_cast(aw_f4, __builtin_nontemporal_load((const aw_u4_at4*)p)); }
+__device__ __forceinline__ aw_h4 aw_take(const uint16_t* p) { return __builtin_bit_cast(aw_h4, __builtin_nontemporal_load((const aw_u2_at2*)p)); }
+__device__ __forceinline__ uint32_t aw_take(const uint8_t* p) { return __builtin_nontemporal_load((const aw_u1_at1*)p); }
+__device__ __forceinline__ void aw_put(float* p, const aw_f4& x) { __builtin_nontemporal_store(__builtin_bit_cast(aw_u4, x), (aw_u4_at4*)p); }
+__device__ __forceinline__ void aw_put(uint16_t* p, const aw_h4& x) { __builtin_nontemporal_store(__builtin_bit_cast(aw_u2, x), (aw_u2_at2*)p); }
+__device__ __forceinline__ void aw_put(uint8_t* p, uint32_t x) { __builtin_nontemporal_store(x, (aw_u1_at1*)p); }
+
 // float32 -> bfloat16 to the nearest, halves away from zero, and the signed 16 bits between the two: the pair is the
-// float32 value again exactly, and (unlike rounding halves to even) the difference always fits.
+// float32 value again exactly, and (unlike rounding halves to even) the difference always fits: it is the pattern's low half.
 __device__ __forceinline__ void aw_split(float w, uint16_t& hi, int16_t& lo) {
     const uint32_t b = __float_as_uint(w);
     const bool nan = w != w;
-    const uint32_t h = (b + 0x8000u) >> 16;
-    hi = (uint16_t)(nan ? 0x7FC0u : h);
-    lo = (int16_t)(nan ? 0u : b - (h << 16));
+    hi = (uint16_t)(nan ? 0x7FC0u : (b + 0x8000u) >> 16);
+    lo = (int16_t)(nan ? 0u : b);
 }
 __device__ __forceinline__ float aw_join(uint16_t hi, int16_t lo) {
     return __uint_as_float(((uint32_t)hi << 16) + (uint32_t)(int)lo);
+}
+__device__ __forceinline__ void aw_split4(const float* w, aw_h4& h, aw_h4& l) {
+    if (__ballot(__builtin_isunordered(w[0], w[1]) || __builtin_isunordered(w[2], w[3])) == 0) {     // no NaN in the wave
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const uint32_t a = __float_as_uint(w[2 * j]), b = __float_as_uint(w[2 * j + 1]);
+            h.x[j] = __builtin_amdgcn_perm(b + 0x8000u, a + 0x8000u, 0x07060302u);
+            l.x[j] = __builtin_amdgcn_perm(b, a, 0x05040100u);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            uint16_t h0, h1;
+            int16_t l0, l1;
+            aw_split(w[2 * j], h0, l0);
+            aw_split(w[2 * j + 1], h1, l1);
+            h.x[j] = h0 | ((uint32_t)h1 << 16);
+            l.x[j] = (uint16_t)l0 | ((uint32_t)(uint16_t)l1 << 16);
+        }
+    }
+}
+__device__ __forceinline__ void aw_join4(const aw_h4& h, const aw_h4& l, float* w) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        w[2 * j] = __uint_as_float((h.x[j] << 16) + (uint32_t)((int)(l.x[j] << 16) >> 16));
+        w[2 * j + 1] = __uint_as_float((h.x[j] & 0xFFFF0000u) + (uint32_t)((int)l.x[j] >> 16));
+    }
 }
 __device__ __forceinline__ float aw_bf16(uint16_t h) { return __uint_as_float((uint32_t)h << 16); }
 
@@ -70,11 +111,15 @@ __device__ __forceinline__ float aw_exact(float w, float m, float v, const AwPar
     return w * t.decay - (m * t.step_size) / denom;
 }
 
-// The tensor that workgroup `b` works on: one look at every tensor's first workgroup, a lane each.
+// The tensor that workgroup `b` works on (scalar; six steps for 40 tensors.  Comparing with every start is more work than
+// the waiting it saves: 405 -> 436 us for the 8-bit step over 2,000,000 Gaussians, a lane each through vector loads 413.)
 __device__ __forceinline__ int aw_find(const int* start, int num, int b) {
-    const int lane = threadIdx.x & 63;
-    const int s = lane < num ? start[lane] : 0x7FFFFFFF;
-    return __builtin_amdgcn_readfirstlane(__popcll(__ballot(s <= b)) - 1);
+    int lo = 0, hi = num;
+    while (hi - lo > 1) {
+        const int m = (lo + hi) >> 1;
+        if (start[m] <= b) lo = m; else hi = m;
+    }
+    return lo;
 }
 
 template <bool BF16>
@@ -117,11 +162,14 @@ __device__ __forceinline__ void aw_load(const AwTensor& t, long long block, int 
         aw_grad_rows<BF16>(t, block + o, WHOLE ? 4 : valid, x.g);
     } else if (WHOLE) {
         if (BF16) {
-            const aw_h4 g = *(const aw_h4*)((const uint16_t*)t.g + block + o);
+            const aw_h4 g = aw_take((const uint16_t*)t.g + block + o);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) x.g[j] = aw_bf16(g.x[j]);
+            for (int j = 0; j < 2; ++j) {
+                x.g[2 * j] = __uint_as_float(g.x[j] << 16);
+                x.g[2 * j + 1] = __uint_as_float(g.x[j] & 0xFFFF0000u);
+            }
         } else {
-            const aw_f4 g = *(const aw_f4*)((const float*)t.g + block + o);
+            const aw_f4 g = aw_take((const float*)t.g + block + o);
 #pragma unroll
             for (int j = 0; j < 4; ++j) x.g[j] = g.x[j];
         }
@@ -135,19 +183,18 @@ __device__ __forceinline__ void aw_load(const AwTensor& t, long long block, int 
     }
     if (WHOLE) {
         if (BF16) {
-            const aw_h4 h = *(const aw_h4*)((const uint16_t*)t.p + block + o), l = *(const aw_h4*)(t.low + block + o);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) x.w[j] = aw_join(h.x[j], (int16_t)l.x[j]);
+            const aw_h4 h = *(const aw_h4*)((const uint16_t*)t.p + block + o), l = aw_take((const uint16_t*)t.low + block + o);
+            aw_join4(h, l, x.w);
         } else {
             const aw_f4 p = *(const aw_f4*)((const float*)t.p + block + o);
 #pragma unroll
             for (int j = 0; j < 4; ++j) x.w[j] = p.x[j];
         }
         if (EIGHT) {
-            x.cm = ((const aw_b4*)((const uint8_t*)t.m + block + o))->x;
-            x.cv = ((const aw_b4*)((const uint8_t*)t.v + block + o))->x;
+            x.cm = aw_take((const uint8_t*)t.m + block + o);
+            x.cv = aw_take((const uint8_t*)t.v + block + o);
         } else {
-            const aw_f4 m = *(const aw_f4*)((const float*)t.m + block + o), v = *(const aw_f4*)((const float*)t.v + block + o);
+            const aw_f4 m = aw_take((const float*)t.m + block + o), v = aw_take((const float*)t.v + block + o);
 #pragma unroll
             for (int j = 0; j < 4; ++j) { x.m[j] = m.x[j]; x.v[j] = v.x[j]; }
         }
@@ -228,9 +275,10 @@ __device__ __forceinline__ void aw_finish(const AwPart& k, const AwTensor& t, lo
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const uint32_t h = m8_hash(x0 + (uint32_t)j * M8_C1);
-            cm |= m8_encode<true>(x.m[j], m8_noise_m(h), bm) << (8 * j);
-            cv |= m8_encode<false>(x.v[j], m8_noise_v(h), bv) << (8 * j);
+            cm |= m8_encode<true>(__float_as_uint(x.m[j]) & 0x7FFFFFFFu, m8_noise_m(h), bm) << (8 * j);
+            cv |= m8_encode<false>(__float_as_uint(x.v[j]) & 0x7FFFFFFFu, m8_noise_v(h), bv) << (8 * j);
         }
+        cm |= m8_signs(x.m);
         cm = em == 255 ? 0u : cm;
         cv = ev == 255 ? 0u : cv;
         if (lane == 0) {
@@ -241,14 +289,9 @@ __device__ __forceinline__ void aw_finish(const AwPart& k, const AwTensor& t, lo
     if (WHOLE) {
         if (BF16) {
             aw_h4 h, l;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                int16_t lo;
-                aw_split(x.w[j], h.x[j], lo);
-                l.x[j] = (uint16_t)lo;
-            }
+            aw_split4(x.w, h, l);
             *(aw_h4*)((uint16_t*)t.p + block + o) = h;
-            *(aw_h4*)(t.low + block + o) = l;
+            aw_put((uint16_t*)t.low + block + o, l);
         } else {
             aw_f4 p;
 #pragma unroll
@@ -256,14 +299,14 @@ __device__ __forceinline__ void aw_finish(const AwPart& k, const AwTensor& t, lo
             *(aw_f4*)((float*)t.p + block + o) = p;
         }
         if (EIGHT) {
-            ((aw_b4*)((uint8_t*)t.m + block + o))->x = cm;
-            ((aw_b4*)((uint8_t*)t.v + block + o))->x = cv;
+            aw_put((uint8_t*)t.m + block + o, cm);
+            aw_put((uint8_t*)t.v + block + o, cv);
         } else {
             aw_f4 m, v;
 #pragma unroll
             for (int j = 0; j < 4; ++j) { m.x[j] = x.m[j]; v.x[j] = x.v[j]; }
-            *(aw_f4*)((float*)t.m + block + o) = m;
-            *(aw_f4*)((float*)t.v + block + o) = v;
+            aw_put((float*)t.m + block + o, m);
+            aw_put((float*)t.v + block + o, v);
         }
         return;
     }
@@ -296,9 +339,10 @@ adamw_kernel(AwPart k) {
     const int ti = aw_find(k.start, k.num, (int)blockIdx.x);
     const AwTensor& t = k.t[ti];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const long long base = (long long)((int)blockIdx.x - k.start[ti]) * AW_PER_GROUP + wave * AW_PER_WAVE;
+    constexpr int AW_BLOCKS = aw_blocks(EIGHT);
+    const long long base = (long long)((int)blockIdx.x - k.start[ti]) * aw_per_group(EIGHT) + wave * (AW_BLOCKS * M8_BLOCK);
     AwLane<BF16, EIGHT> x[AW_BLOCKS];
-    if (base + AW_PER_WAVE <= t.n) {             // whole blocks: all loads before the first use
+    if (base + AW_BLOCKS * M8_BLOCK <= t.n) {    // whole blocks: all loads before the first use
 #pragma unroll
         for (int u = 0; u < AW_BLOCKS; ++u) aw_load<BF16, EIGHT, true>(t, base + u * M8_BLOCK, 4, x[u]);
 #pragma unroll
@@ -322,12 +366,13 @@ extern "C" int fdgs_adamw_step(const fdgs_adamw_args* a, void* stream) {
     if (!bf16 && a->param_type != FDGS_TYPE_F32) return FDGS_EINVAL;
     if (!eight && a->state_bits != 32) return FDGS_EINVAL;
     if (!(a->beta1 >= 0.0 && a->beta1 < 1.0 && a->beta2 >= 0.0 && a->beta2 < 1.0 && a->eps >= 0.0)) return FDGS_EINVAL;
+    const int per_group = aw_per_group(eight);
     for (int i = 0; i < a->num_tensors; ++i) {   // all of them before the first launch: no step is half done
         const fdgs_adamw_tensor& s = a->tensors[i];
         if (s.numel < 0 || s.step < 1 || s.grad_row_len < 0) return FDGS_EINVAL;
         if (s.grad_row_len > 0 && s.grad_row_stride < s.grad_row_len) return FDGS_EINVAL;
         if (s.numel == 0) continue;
-        if ((s.numel - 1) / AW_PER_GROUP >= 0x7fffffffLL / AW_MAX) return FDGS_ETOOLARGE;
+        if ((s.numel - 1) / per_group >= 0x7fffffffLL / AW_MAX) return FDGS_ETOOLARGE;
         if (!s.param || !s.grad || !s.exp_avg || !s.exp_avg_sq || (bf16 && !s.residual)) return FDGS_EINVAL;
         if (eight && (!s.exp_avg_exponents || !s.exp_avg_sq_exponents)) return FDGS_EINVAL;
     }
@@ -343,7 +388,7 @@ extern "C" int fdgs_adamw_step(const fdgs_adamw_args* a, void* stream) {
             const fdgs_adamw_tensor& s = a->tensors[i];
             if (s.numel == 0) continue;
             k.start[k.num] = blocks;
-            blocks += (int)((s.numel + AW_PER_GROUP - 1) / AW_PER_GROUP);
+            blocks += (int)((s.numel + per_group - 1) / per_group);
             AwTensor& t = k.t[k.num++];
             t.p = s.param; t.g = s.grad; t.m = s.exp_avg; t.v = s.exp_avg_sq;
             t.low = s.residual; t.me = s.exp_avg_exponents; t.ve = s.exp_avg_sq_exponents;
@@ -366,7 +411,7 @@ extern "C" int fdgs_adamw_step(const fdgs_adamw_args* a, void* stream) {
 }
 
 // ---- 8-bit moments to values and back ----
-#define M8_MAX 64                                // tensors per launch
+#define M8_MAX 92                                // tensors per launch
 struct M8Tensor { uint8_t* codes; uint8_t* exps; void* value; long long n; uint32_t key; int is_signed; };
 struct M8Part {
     int num, nearest;
@@ -419,10 +464,10 @@ moment8_unpack_kernel(M8Part k) {
     const long long base = (long long)((int)blockIdx.x - k.start[ti]) * M8_PER_GROUP + 8 * (int)threadIdx.x;
     if (t.is_signed) {
 #pragma unroll
-        for (int u = 0; u < 4; ++u) m8_unpack8<BF16, true>(t, base + u * 2048);
+        for (int u = 0; u < M8_PER_GROUP / 2048; ++u) m8_unpack8<BF16, true>(t, base + u * 2048);
     } else {
 #pragma unroll
-        for (int u = 0; u < 4; ++u) m8_unpack8<BF16, false>(t, base + u * 2048);
+        for (int u = 0; u < M8_PER_GROUP / 2048; ++u) m8_unpack8<BF16, false>(t, base + u * 2048);
     }
 }
 
@@ -445,7 +490,10 @@ __device__ __forceinline__ void m8_pack_block(const M8Part& k, const M8Tensor& t
     for (int j = 0; j < 4; ++j) {
         if (i + j >= t.n) break;
         const uint32_t h = k.nearest ? 0x80008000u : m8_hash(((uint32_t)i + j + key) * M8_C1);
-        t.codes[i + j] = (uint8_t)(e == 255 ? 0u : m8_encode<SIGNED>(x[j], SIGNED ? m8_noise_m(h) : m8_noise_v(h), base));
+        const uint32_t all = __float_as_uint(x[j]);
+        uint32_t code = m8_encode<SIGNED>(all & 0x7FFFFFFFu, SIGNED ? m8_noise_m(h) : m8_noise_v(h), base);
+        if (SIGNED) code |= (all >> 24) & 128u;
+        t.codes[i + j] = (uint8_t)(e == 255 ? 0u : code);
     }
     if (lane == 0) t.exps[b / M8_BLOCK] = (uint8_t)e;
 }

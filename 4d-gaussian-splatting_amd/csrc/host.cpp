@@ -236,6 +236,11 @@ PyObject* adamw_step(PyObject* a) {
     args.eps = eps;
     args.tensors = out.data();
     launch("fdgs_adamw_step", library.adamw, args, device);
+    // written in place: a graph that has saved a parameter is to notice, as after torch's own steps
+    for (Py_ssize_t i = 0; i < n; ++i) {
+        const Tensor& t = THPVariable_Unpack(p.at(i));
+        if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+    }
     Py_RETURN_NONE;
 }
 
@@ -436,11 +441,19 @@ int64_t padding_of(PyObject* o) {
     return v;
 }
 
+// A tensor here would lose its gradient without a word.
+double scale_of(PyObject* o) {
+    if (THPVariable_Check(o)) throw Refused{PyExc_TypeError, "scale is a number, not a tensor: it gets no gradient"};
+    const double v = PyFloat_AsDouble(o);
+    if (v == -1.0 && PyErr_Occurred()) throw Raised();
+    return v;
+}
+
 // embedding(ids, table, scale, padding_id | None)
 PyObject* embedding(PyObject* a) {
-    PyObject *io, *to, *po;
-    double scale;
-    if (!PyArg_ParseTuple(a, "OOdO", &io, &to, &scale, &po)) throw Raised();
+    PyObject *io, *to, *so, *po;
+    if (!PyArg_ParseTuple(a, "OOOO", &io, &to, &so, &po)) throw Raised();
+    const double scale = scale_of(so);
     const Tensor &ids = tensor(io, "ids"), &table = tensor(to, "the table");
     if (table.dim() < 2) value_error("the table is [rows, ...] in float32, bfloat16 or float16");
     type_of(table, "the table");
@@ -458,10 +471,10 @@ PyObject* embedding(PyObject* a) {
 
 // embedding_grad(grad_out, ids, num_rows, scale, padding_id | None)
 PyObject* embedding_grad(PyObject* a) {
-    PyObject *go, *io, *po;
+    PyObject *go, *io, *so, *po;
     long long rows;
-    double scale;
-    if (!PyArg_ParseTuple(a, "OOLdO", &go, &io, &rows, &scale, &po)) throw Raised();
+    if (!PyArg_ParseTuple(a, "OOLOO", &go, &io, &rows, &so, &po)) throw Raised();
+    const double scale = scale_of(so);
     const Tensor &g = tensor(go, "grad_out"), &ids = tensor(io, "ids");
     return THPVariable_Wrap(table_grad(g, ids, rows, scale, padding_of(po)));
 }

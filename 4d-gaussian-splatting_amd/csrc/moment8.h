@@ -40,9 +40,9 @@ __device__ __forceinline__ uint32_t m8_key(uint32_t key, long long index) {
     return key + (uint32_t)((unsigned long long)index >> 32) * 0x6A09E667u;
 }
 
-// What the two fields of the hash add below the kept bits.
-__device__ __forceinline__ uint32_t m8_noise_m(uint32_t h) { return (h >> 12) & 0xFFFF0u; }
-__device__ __forceinline__ uint32_t m8_noise_v(uint32_t h) { return (h << 4) & 0xFFFF0u; }
+// The two fields of the hash; 16 times such a field is what is added below the kept bits.
+__device__ __forceinline__ uint32_t m8_noise_m(uint32_t h) { return h >> 16; }
+__device__ __forceinline__ uint32_t m8_noise_v(uint32_t h) { return h & 0xFFFFu; }
 
 template <bool SIGNED>
 __device__ __forceinline__ int m8_base(int e) {
@@ -58,14 +58,20 @@ __device__ __forceinline__ uint32_t m8_decode(uint32_t code, int base) {
     return SIGNED ? bits | ((code & 128u) << 24) : bits;
 }
 
-// The code of x; the caller stores 0 in a block whose exponent is 255.
+// The code of a magnitude's pattern, without a sign; the caller stores 0 in a block whose exponent is 255.
 template <bool SIGNED>
-__device__ __forceinline__ uint32_t m8_encode(float x, uint32_t noise, int base) {
-    const uint32_t all = __float_as_uint(x), bits = all & 0x7FFFFFFFu;
-    const int code = (int)((bits + noise) >> 20) - base;
-    if (SIGNED) return (uint32_t)(code > 0 ? code : 0) | ((all >> 24) & 128u);
-    const int least = (int)(bits < 1u ? bits : 1u);
-    return (uint32_t)(code > least ? code : least);
+__device__ __forceinline__ uint32_t m8_encode(uint32_t bits, uint32_t noise, int base) {
+    // the subtraction saturates: what lies below the base gets code 0
+    const uint32_t code = __builtin_elementwise_sub_sat(bits + (noise << 4), (uint32_t)base << 20) >> 20;
+    if (SIGNED) return code;
+    const uint32_t least = bits < 1u ? bits : 1u;
+    return code > least ? code : least;
+}
+// Bit 7 of each byte: the signs of four values.
+__device__ __forceinline__ uint32_t m8_signs(const float* x) {
+    const uint32_t lo = __builtin_amdgcn_perm(__float_as_uint(x[1]), __float_as_uint(x[0]), 0x0C0C0703u);
+    const uint32_t hi = __builtin_amdgcn_perm(__float_as_uint(x[3]), __float_as_uint(x[2]), 0x07030C0Cu);
+    return (lo | hi) & 0x80808080u;
 }
 
 typedef unsigned short m8_u16x2 __attribute__((ext_vector_type(2)));

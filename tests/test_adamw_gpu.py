@@ -264,6 +264,34 @@ def test_what_is_not_finite_stays_where_it_is(bits):
     assert sb[0][hit].isnan().all() if bits == 8 else not sb[0][hit].isfinite().any()
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("eps", [0.0, 1e-40, 1e-30, 1e-15])
+def test_moments_below_the_normal_numbers(bits, eps):
+    """Gradients whose squares are below the smallest normal float32 (and, in the first block, ordinary ones beside them): the
+    update is the formula's, with what v's evenly spaced numbers there leave of it (2^-148 for each of four roundings)."""
+    from fdgs import adamw
+    rng = np.random.default_rng(3)
+    n = 1024
+    g = (10.0 ** rng.uniform(-22, -19, n) * np.where(rng.random(n) < 0.5, -1, 1)).astype(np.float32)
+    g[:100] = rng.standard_normal(100)
+    p, m, v = (torch.zeros(n, device="cuda") for _ in range(3))
+    if bits == 8:
+        m, v = adamw.Moment8.zeros_like(p, True), adamw.Moment8.zeros_like(p, False)
+    adamw.adamw_step([p], [torch.from_numpy(g).cuda()], [m], [v], steps=1, lr=1e-3, eps=eps, keys=[1] if bits == 8 else None)
+    zero = np.zeros(n)
+    w64, m64, v64 = ac.adamw64(zero, g, zero, zero, 1, 1e-3, 0.01, 0.9, 0.999, eps)
+    off = 4 * 2.0 ** -148
+    lo, hi = (1e-3 * np.abs(g) / (np.sqrt(np.maximum(v64 + s * off, 0.0) / (1 - 0.999)) + eps * (1 - s * U) - s * 2.0 ** -149)
+              for s in (1, -1))
+    hi = np.where((hi > 0) & (v64 > off), hi, np.inf)       # v itself may be rounded to nothing
+    got = np.abs(p.cpu().numpy().astype(np.float64))
+    rel = 15.3 * U
+    ok = got >= lo * (1 - rel) - 2.0 ** -149
+    ok &= (got <= hi * (1 + rel)) | ~np.isfinite(got)
+    assert ok.all() and np.isfinite(got[v64 > 2 * off]).all(), int((~ok).sum())
+    assert (np.sign(p.cpu().numpy())[v64 > 2 * off] == -np.sign(g)[v64 > 2 * off]).all()
+
+
 def test_bfloat16_weights_gather_small_updates():
     """1000 steps of 1e-5 on weights of 1, where bfloat16's step is 2^-7: the parameter follows the float32 weight."""
     from fdgs import adamw

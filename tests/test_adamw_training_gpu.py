@@ -121,6 +121,18 @@ def test_states_of_other_optimizers_are_taken():
     assert all(torch.equal(theirs.state[p]["exp_avg"], src.state[p]["exp_avg"]) for p in ps)
 
 
+def test_a_step_is_seen_by_saved_graphs():
+    """A backward pass over a parameter that was stepped after its forward pass raises, as with torch's optimizers."""
+    from fdgs.adamw import FusedAdamW
+    p = torch.ones(8, device="cuda", requires_grad=True)
+    opt = FusedAdamW([p])
+    loss = (p * p).sum()
+    loss.backward(retain_graph=True)
+    opt.step()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+
 def _scene(n=3000, w=96, h=64):
     from fdgs import scene_synth as ss
     from fdgs.deformation import DeformationFields

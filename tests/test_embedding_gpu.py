@@ -104,7 +104,9 @@ def test_lookup_and_gradient(t, v, d, dtype):
 
 @pytest.mark.parametrize("spread", ["one", "distinct"])
 @pytest.mark.parametrize("t,v,d,dtype", [(20000, 3, 48, torch.float32), (9000, 5, 1000, torch.bfloat16), (33000, 4, 1, torch.float16),
-                                         (2000, 2, 2500, torch.float32), (16000, 20000, 48, torch.float32), (100, 1 << 20, 5, torch.float32)])
+                                         (2000, 2, 2500, torch.float32), (16000, 20000, 48, torch.float32), (100, 1 << 20, 5, torch.float32),
+                                         (100, 3, 48, torch.float32), (128, 2, 1000, torch.bfloat16), (129, 2, 1000, torch.bfloat16),
+                                         (4096, 9, 64, torch.float16), (4097, 9, 64, torch.float16), (300000, 2, 4, torch.float32)])
 def test_one_row_for_all_and_a_row_for_each(t, v, d, dtype, spread):
     """A row with every token (its sum is cut over many shares) and none with more than one or two.  Small whole numbers: the
     sums are exact in float32, so the gradient is the rounded exact value, whatever the order."""
@@ -134,6 +136,27 @@ def test_padding_and_shapes_of_ids():
             grad, = torch.autograd.grad(y, x, gy.cuda())
             _check_grad(grad, gy, use, 2.0, torch.float32, padding)
             assert torch.equal(grad, embedding_grad(gy.cuda(), dev, 50, scale=2.0, padding_id=padding))
+
+
+@pytest.mark.parametrize("t", [60, 3000, 9000, 40000])
+def test_what_padded_tokens_hold_does_not_matter(t):
+    """NaN and infinities in the gradients of padded tokens, and in the padding row of the table."""
+    from fdgs.embedding import embedding, embedding_grad
+    g = torch.Generator().manual_seed(t)
+    ids = torch.randint(0, 50, (t,), generator=g)
+    ids[torch.rand(t, generator=g) < 0.4] = -1
+    ids[torch.rand(t, generator=g) < 0.2] = 49
+    none = (ids == -1) | (ids == 49)
+    gy = torch.randint(-3, 4, (t, 24), generator=g).float()
+    bad = gy.clone()
+    bad[none] = float("nan")
+    bad[none.nonzero()[::2, 0]] = float("inf")
+    table = torch.randn(50, 24, generator=g)
+    table[49] = float("nan")
+    got = embedding_grad(bad.cuda(), ids.cuda(), 50, padding_id=49).cpu()
+    assert torch.equal(got, _grad64(gy, ids, 50, 1.0, 49)[0].float()) and (got[49] == 0).all()
+    assert (embedding(ids.cuda(), table.cuda(), padding_id=49).cpu()[none] == 0).all()
+    assert (embedding_grad(bad.cuda(), torch.full_like(ids, -5).cuda(), 50).cpu() == 0).all()
 
 
 def test_slices_of_tables_and_gradients_are_read_in_place():
@@ -201,7 +224,7 @@ def test_two_captured_graphs_with_workspaces_of_their_own():
     """Lookup and gradient captured twice, replayed in turn with new inputs and eager calls in between."""
     from fdgs.embedding import embedding, embedding_grad
     cases = []
-    for t, v, d in ((20000, 300, 24), (500, 900, 40)):
+    for t, v, d in ((20000, 300, 24), (500, 900, 40), (9000, 70, 16), (100, 30, 8)):
         cases.append([torch.zeros(t, dtype=torch.int32, device="cuda"), torch.zeros(v, d, device="cuda"),
                       torch.zeros(t, d, device="cuda"), None, None, torch.cuda.CUDAGraph()])
     for c in cases:
@@ -219,6 +242,36 @@ def test_two_captured_graphs_with_workspaces_of_their_own():
             eager = embedding(ids, table, scale=3.0), embedding_grad(gy, ids, table.shape[0], scale=3.0)
             torch.cuda.synchronize()
             assert torch.equal(y, eager[0]) and torch.equal(grad, eager[1])
+
+
+def test_captured_training_pass():
+    """Lookup and backward through autograd in one graph, replayed with other inputs and eager passes in between."""
+    from fdgs.embedding import embedding
+    ids = torch.zeros(5000, dtype=torch.int64, device="cuda")
+    table = torch.zeros(40, 12, device="cuda", requires_grad=True)
+    gy = torch.zeros(5000, 12, device="cuda")
+
+    def once():
+        y = embedding(ids, table, scale=0.5)
+        return y, torch.autograd.grad(y, table, gy)[0]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        once()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = once()
+    for k in range(3):
+        g = torch.Generator().manual_seed(k)
+        ids.copy_(torch.randint(-1, 40, (5000,), generator=g))
+        with torch.no_grad():
+            table.copy_(torch.randn(40, 12, generator=g))
+        gy.copy_(torch.randn(5000, 12, generator=g))
+        graph.replay()
+        want = once()
+        torch.cuda.synchronize()
+        assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
 
 
 def test_two_streams_at_once():
@@ -266,6 +319,8 @@ def test_refusals_on_the_device():
         embedding(torch.tensor([1.0], device="cuda"), table)
     with pytest.raises(ValueError, match="float32, bfloat16"):
         embedding(torch.tensor([1], device="cuda"), table.double())
+    with pytest.raises(TypeError, match="scale is a number"):
+        embedding(torch.tensor([1], device="cuda"), table, scale=torch.ones(()))
     with pytest.raises(ValueError, match="row of the table"):
         embedding(torch.tensor([1], device="cuda"), table, padding_id=-1)
     ids = torch.tensor([1, 2], device="cuda")
