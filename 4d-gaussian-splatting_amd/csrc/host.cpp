@@ -441,6 +441,20 @@ int64_t padding_of(PyObject* o) {
     return v;
 }
 
+// A backward pass that is captured while a graph of the same leaf made on another stream lives waits for that stream, from
+// autograd's own thread, where the error that the capture makes of it ends the process.  Refused here, where it can be.
+void capture_alone(const Tensor& table) {
+    if (!table.is_leaf()) return;
+    const c10::DeviceGuard guard(table.device());
+    if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(table);
+    if (!node) return;
+    const auto made_on = node->stream();
+    if (made_on.has_value() && made_on->id() == c10::hip::getCurrentHIPStream(table.device().index()).id()) return;
+    throw Refused{PyExc_RuntimeError, "embedding: an autograd graph of this table from outside the capture is alive; delete its "
+                                      "outputs before capturing a pass that wants gradients"};
+}
+
 // A tensor here would lose its gradient without a word.
 double scale_of(PyObject* o) {
     if (THPVariable_Check(o)) throw Refused{PyExc_TypeError, "scale is a number, not a tensor: it gets no gradient"};
@@ -462,6 +476,7 @@ PyObject* embedding(PyObject* a) {
     Tensor out;
     if (table.requires_grad() && at::GradMode::is_enabled()) {
         ids_of(ids, table.device());                 // refused here, as the type that a caller expects
+        capture_alone(table);
         out = Lookup::apply(table, ids, scale, padding);
     } else {
         out = lookup(ids, table, scale, padding);

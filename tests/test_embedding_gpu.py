@@ -245,8 +245,8 @@ def test_two_captured_graphs_with_workspaces_of_their_own():
 
 
 def test_captured_training_pass():
-    """Lookup and backward through autograd in one graph, replayed with other inputs and eager passes in between."""
-    from fdgs.embedding import embedding
+    """Lookup and backward through autograd in one graph, replayed with other inputs and eager calls in between."""
+    from fdgs.embedding import embedding, embedding_grad
     ids = torch.zeros(5000, dtype=torch.int64, device="cuda")
     table = torch.zeros(40, 12, device="cuda", requires_grad=True)
     gy = torch.zeros(5000, 12, device="cuda")
@@ -269,9 +269,36 @@ def test_captured_training_pass():
             table.copy_(torch.randn(40, 12, generator=g))
         gy.copy_(torch.randn(5000, 12, generator=g))
         graph.replay()
-        want = once()
+        y = embedding(ids, table.detach(), scale=0.5)
+        want = embedding_grad(gy, ids, 40, scale=0.5)
         torch.cuda.synchronize()
-        assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+        assert torch.equal(out[0], y) and torch.equal(out[1], want)
+
+
+def test_capture_beside_a_living_eager_graph_is_refused():
+    """Such a backward pass would end the process; without gradients, or with the eager graph gone, the capture works."""
+    from fdgs.embedding import embedding
+    ids = torch.tensor([1, 0, 1], device="cuda")
+    table = torch.randn(2, 8, device="cuda", requires_grad=True)
+    eager = embedding(ids, table)
+    first = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(first):
+        with pytest.raises(RuntimeError, match="outside the capture"):
+            embedding(ids, table)
+        plain = embedding(ids, table.detach())
+    first.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(plain, eager)
+    want = eager.detach().clone()
+    del eager
+    second = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(second):
+        y = embedding(ids, table) + embedding(ids, table)        # twice in one capture
+        grad, = torch.autograd.grad(y, table, torch.ones_like(y))
+    for _ in range(3):
+        second.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, 2 * want) and torch.equal(grad, torch.tensor([[2.0], [4.0]], device="cuda").expand(2, 8))
 
 
 def test_two_streams_at_once():
