@@ -1,4 +1,4 @@
-// AdamW over many tensors in one launch per 40 tensors (moments in float32 or in 8 bits, parameters in float32 or in
+// AdamW over many tensors in one launch (moments in float32 or in 8 bits, parameters in float32 or in
 // bfloat16), and the 8-bit moments' conversions.
 //
 //   m = beta1 m + (1 - beta1) g;   v = beta2 v + (1 - beta2) g^2
@@ -13,8 +13,9 @@
 // The products and sums are not contracted to fused multiply-adds: which code an 8-bit moment gets then depends on
 // the formula alone and not on the compiler's choices, and the same step is the same bits on every replica.
 #include "moment8.h"
+#include <type_traits>
 
-#define AW_MAX 40                                // tensors per launch: their records fill 4 KB of kernel arguments
+#define AW_MAX 40                                // tensors whose records fill 4 KB of kernel arguments
 // Blocks of 256 per wave, and elements per workgroup of four waves.  One block with float32 moments (97 bfloat16 tensors:
 // 203 us, 213 with two, 232 with four), two with 8-bit ones (2,000,000 Gaussians: 405 us, 418 with one, 405 with four; 211
 // bfloat16 tensors 157, 157, 198).
@@ -29,13 +30,99 @@ struct AwTensor {
     float step_size, inv_root, decay;
     uint32_t key, pad;
 };
-struct AwPart {
-    int num, exact;                              // exact: eps lies below the normal numbers
+struct AwStep {
+    int exact;                                   // eps lies below the normal numbers
     float b1, omb1, b2, omb2, eps;
-    int start[AW_MAX];                           // first workgroup of each tensor
-    AwTensor t[AW_MAX];
 };
-static_assert(sizeof(AwPart) <= 4096, "kernel arguments of one launch");
+template <class Record, int MAX>
+struct AwPart {
+    Record t[MAX];
+    int start[MAX];                              // first workgroup of each tensor
+    int num;
+};
+static_assert(sizeof(AwStep) + sizeof(AwPart<AwTensor, AW_MAX>) <= 4096, "kernel arguments of one launch");
+
+// Where the records of a launch lie: in its arguments, or (more tensors than two launches' arguments hold) in a table in
+// device memory that small launches before it have filled from theirs.  211 bfloat16 tensors with 8-bit moments and the
+// conversion of these: 244 us in six launches and five, 199 in one each and as many that fill; 97 bfloat16 tensors 198 us
+// in three launches, 199 in one and three that fill.
+template <class Record, int MAX>
+struct AwInArgs {
+    AwPart<Record, MAX> part;
+    __device__ __forceinline__ int num() const { return part.num; }
+    __device__ __forceinline__ const int* starts() const { return part.start; }
+    __device__ __forceinline__ const Record& record(int i) const { return part.t[i]; }
+};
+// (The table is read through the constant address space: nothing in the launch writes it, so a record is loaded once and into
+// scalar registers like the arguments.  As ordinary memory the 8-bit step reads it again behind every store: 131 us, not 94, for
+// 40,000,000 elements.)
+template <class Record, int MAX>
+struct AwInTable {
+    const Record* t;
+    const int* start;
+    int n;
+    typedef const __attribute__((address_space(4))) int* Ints;
+    __device__ __forceinline__ int num() const { return n; }
+    __device__ __forceinline__ Ints starts() const { return (Ints)(uintptr_t)start; }
+    __device__ __forceinline__ Record record(int i) const {
+        int words[sizeof(Record) / 4];
+        const Ints from = (Ints)(uintptr_t)(t + i);
+#pragma unroll
+        for (int k = 0; k < (int)(sizeof(Record) / 4); ++k) words[k] = from[k];
+        return __builtin_bit_cast(Record, words);
+    }
+};
+template <class Record, int MAX>
+__global__ void __launch_bounds__(256)
+list_table_kernel(AwPart<Record, MAX> part, Record* table, int* start) {
+    // one load a thread: the arguments are far away (with four after one another a fill took 4.8 us)
+    struct __attribute__((packed, aligned(4))) W4 { uint32_t x[4]; };
+    static_assert(MAX * sizeof(Record) <= 256 * sizeof(W4) && MAX * sizeof(Record) % sizeof(W4) == 0 && MAX <= 256, "one load a thread");
+    const int i = threadIdx.x;
+    const W4 x = i < (int)(MAX * sizeof(Record) / sizeof(W4)) ? ((const W4*)part.t)[i] : W4{};
+    const int first = i < MAX ? part.start[i] : 0;
+    uint32_t* to = (uint32_t*)table;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (4 * i + j < part.num * (int)(sizeof(Record) / 4)) to[4 * i + j] = x.x[j];
+    if (i < part.num) start[i] = first;
+}
+static size_t list_table_bytes(int num, size_t record) { return (size_t)num * (record + sizeof(int)) + 512; }
+
+// Runs `launch(source, workgroups)` for all the records that `next(record, workgroups)` gives (false: no more): in one launch
+// over the table where there is a workspace and more of them than the arguments hold, else in as many launches as it takes.
+template <class Record, int MAX, class Next, class Launch>
+static int list_launch(int count, void* workspace, size_t bytes, hipStream_t s, Next next, Launch launch) {
+    const bool table = count > 2 * MAX && workspace && bytes >= list_table_bytes(count, sizeof(Record));
+    Record* records = (Record*)(((uintptr_t)workspace + 255) / 256 * 256);
+    int* starts = (int*)(records + count);
+    int blocks = 0, filled = 0;
+    for (bool more = true; more;) {
+        AwInArgs<Record, MAX> args;
+        args.part.num = 0;
+        if (!table) blocks = 0;
+        while (args.part.num < MAX) {
+            int groups = 0;
+            more = next(args.part.t[args.part.num], groups);
+            if (!more) break;
+            args.part.start[args.part.num++] = blocks;
+            blocks += groups;
+        }
+        if (args.part.num == 0) break;
+        if (table) {
+            hipLaunchKernelGGL((list_table_kernel<Record, MAX>), dim3(1), dim3(256), 0, s, args.part, records + filled, starts + filled);
+            filled += args.part.num;
+        } else {
+            launch(args, blocks);
+        }
+        FDGS_CHECK_LAUNCH();
+    }
+    if (table && filled) {
+        launch(AwInTable<Record, MAX>{records, starts, filled}, blocks);
+        FDGS_CHECK_LAUNCH();
+    }
+    return FDGS_OK;
+}
 
 struct __attribute__((packed, aligned(4))) aw_f4 { float x[4]; };
 struct __attribute__((packed, aligned(2))) aw_h4 { uint32_t x[2]; };   // four 16-bit numbers, two to a word
@@ -100,12 +187,12 @@ __device__ __forceinline__ float aw_bf16(uint16_t h) { return __uint_as_float((u
 // correctly rounded root and division, 9 issue slots instead of 32: with 8-bit moments the float32 step is bound by its
 // arithmetic, and the update's rounding is far below the 0.1 by which its moments' codes spread.  The caller keeps
 // numbers below the normal ones, which these instructions take for zero, away from it.
-__device__ __forceinline__ float aw_quick(float w, float m, float v, const AwPart& k, const AwTensor& t) {
+__device__ __forceinline__ float aw_quick(float w, float m, float v, const AwStep& k, const AwTensor& t) {
 #pragma clang fp contract(off)
     const float denom = __builtin_amdgcn_sqrtf(v) * t.inv_root + k.eps;
     return w * t.decay - (m * t.step_size) * __builtin_amdgcn_rcpf(denom);
 }
-__device__ __forceinline__ float aw_exact(float w, float m, float v, const AwPart& k, const AwTensor& t) {
+__device__ __forceinline__ float aw_exact(float w, float m, float v, const AwStep& k, const AwTensor& t) {
 #pragma clang fp contract(off)
     const float denom = sqrtf(v) * t.inv_root + k.eps;
     return w * t.decay - (m * t.step_size) / denom;
@@ -113,7 +200,8 @@ __device__ __forceinline__ float aw_exact(float w, float m, float v, const AwPar
 
 // The tensor that workgroup `b` works on (scalar; six steps for 40 tensors.  Comparing with every start is more work than
 // the waiting it saves: 405 -> 436 us for the 8-bit step over 2,000,000 Gaussians, a lane each through vector loads 413.)
-__device__ __forceinline__ int aw_find(const int* start, int num, int b) {
+template <class Ints>
+__device__ __forceinline__ int aw_find(Ints start, int num, int b) {
     int lo = 0, hi = num;
     while (hi - lo > 1) {
         const int m = (lo + hi) >> 1;
@@ -218,7 +306,7 @@ __device__ __forceinline__ void aw_load(const AwTensor& t, long long block, int 
 }
 
 template <bool BF16, bool EIGHT, bool WHOLE>
-__device__ __forceinline__ void aw_finish(const AwPart& k, const AwTensor& t, long long block, int valid, AwLane<BF16, EIGHT>& x) {
+__device__ __forceinline__ void aw_finish(const AwStep& k, const AwTensor& t, long long block, int valid, AwLane<BF16, EIGHT>& x) {
     const uint32_t lane = threadIdx.x & 63, o = 4 * lane;
     float b1 = k.b1, b2 = k.b2;
     if (EIGHT) {
@@ -333,14 +421,14 @@ __device__ __forceinline__ void aw_finish(const AwPart& k, const AwTensor& t, lo
     }
 }
 
-template <bool BF16, bool EIGHT>
+template <bool BF16, bool EIGHT, class Source>
 __global__ void __launch_bounds__(256)
-adamw_kernel(AwPart k) {
-    const int ti = aw_find(k.start, k.num, (int)blockIdx.x);
-    const AwTensor& t = k.t[ti];
+adamw_kernel(AwStep k, Source source) {
+    const int ti = aw_find(source.starts(), source.num(), (int)blockIdx.x);
+    const AwTensor& t = source.record(ti);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     constexpr int AW_BLOCKS = aw_blocks(EIGHT);
-    const long long base = (long long)((int)blockIdx.x - k.start[ti]) * aw_per_group(EIGHT) + wave * (AW_BLOCKS * M8_BLOCK);
+    const long long base = (long long)((int)blockIdx.x - source.starts()[ti]) * aw_per_group(EIGHT) + wave * (AW_BLOCKS * M8_BLOCK);
     AwLane<BF16, EIGHT> x[AW_BLOCKS];
     if (base + AW_BLOCKS * M8_BLOCK <= t.n) {    // whole blocks: all loads before the first use
 #pragma unroll
@@ -367,58 +455,57 @@ extern "C" int fdgs_adamw_step(const fdgs_adamw_args* a, void* stream) {
     if (!eight && a->state_bits != 32) return FDGS_EINVAL;
     if (!(a->beta1 >= 0.0 && a->beta1 < 1.0 && a->beta2 >= 0.0 && a->beta2 < 1.0 && a->eps >= 0.0)) return FDGS_EINVAL;
     const int per_group = aw_per_group(eight);
+    long long total = 0;                         // workgroups
     for (int i = 0; i < a->num_tensors; ++i) {   // all of them before the first launch: no step is half done
         const fdgs_adamw_tensor& s = a->tensors[i];
         if (s.numel < 0 || s.step < 1 || s.grad_row_len < 0) return FDGS_EINVAL;
         if (s.grad_row_len > 0 && s.grad_row_stride < s.grad_row_len) return FDGS_EINVAL;
         if (s.numel == 0) continue;
-        if ((s.numel - 1) / per_group >= 0x7fffffffLL / AW_MAX) return FDGS_ETOOLARGE;
+        total += (s.numel - 1) / per_group + 1;
+        if (total > 0x7fffffffLL) return FDGS_ETOOLARGE;
         if (!s.param || !s.grad || !s.exp_avg || !s.exp_avg_sq || (bf16 && !s.residual)) return FDGS_EINVAL;
         if (eight && (!s.exp_avg_exponents || !s.exp_avg_sq_exponents)) return FDGS_EINVAL;
     }
-    AwPart k;
+    AwStep k;
     k.b1 = (float)a->beta1; k.omb1 = (float)(1.0 - a->beta1);
     k.b2 = (float)a->beta2; k.omb2 = (float)(1.0 - a->beta2);
     k.eps = (float)a->eps;
     k.exact = k.eps > 0.0f && k.eps < 1.17549435e-38f;
-    for (int i = 0; i < a->num_tensors;) {
-        int blocks = 0;
-        k.num = 0;
-        for (; i < a->num_tensors && k.num < AW_MAX; ++i) {
-            const fdgs_adamw_tensor& s = a->tensors[i];
-            if (s.numel == 0) continue;
-            k.start[k.num] = blocks;
-            blocks += (int)((s.numel + per_group - 1) / per_group);
-            AwTensor& t = k.t[k.num++];
-            t.p = s.param; t.g = s.grad; t.m = s.exp_avg; t.v = s.exp_avg_sq;
-            t.low = s.residual; t.me = s.exp_avg_exponents; t.ve = s.exp_avg_sq_exponents;
-            t.n = s.numel; t.gstride = s.grad_row_stride; t.glen = s.grad_row_len;
-            t.step_size = (float)(s.lr / (1.0 - pow(a->beta1, (double)s.step)));
-            t.inv_root = (float)(1.0 / sqrt(1.0 - pow(a->beta2, (double)s.step)));
-            t.decay = (float)(1.0 - s.lr * s.weight_decay);
-            t.key = s.round_key; t.pad = 0;
-        }
-        if (k.num == 0) break;
+    int i = 0;
+    auto next = [&](AwTensor& t, int& groups) {
+        while (i < a->num_tensors && a->tensors[i].numel == 0) ++i;
+        if (i == a->num_tensors) return false;
+        const fdgs_adamw_tensor& s = a->tensors[i++];
+        groups = (int)((s.numel + per_group - 1) / per_group);
+        t.p = s.param; t.g = s.grad; t.m = s.exp_avg; t.v = s.exp_avg_sq;
+        t.low = s.residual; t.me = s.exp_avg_exponents; t.ve = s.exp_avg_sq_exponents;
+        t.n = s.numel; t.gstride = s.grad_row_stride; t.glen = s.grad_row_len;
+        t.step_size = (float)(s.lr / (1.0 - pow(a->beta1, (double)s.step)));
+        t.inv_root = (float)(1.0 / sqrt(1.0 - pow(a->beta2, (double)s.step)));
+        t.decay = (float)(1.0 - s.lr * s.weight_decay);
+        t.key = s.round_key; t.pad = 0;
+        return true;
+    };
+    hipStream_t st = (hipStream_t)stream;
+    auto launch = [&](const auto& source, int blocks) {
+        typedef std::remove_cv_t<std::remove_reference_t<decltype(source)>> Source;
         const dim3 grid((unsigned)blocks), threads(256);
-        hipStream_t st = (hipStream_t)stream;
-        if (bf16 && eight) hipLaunchKernelGGL((adamw_kernel<true, true>), grid, threads, 0, st, k);
-        else if (bf16) hipLaunchKernelGGL((adamw_kernel<true, false>), grid, threads, 0, st, k);
-        else if (eight) hipLaunchKernelGGL((adamw_kernel<false, true>), grid, threads, 0, st, k);
-        else hipLaunchKernelGGL((adamw_kernel<false, false>), grid, threads, 0, st, k);
-        FDGS_CHECK_LAUNCH();
-    }
-    return FDGS_OK;
+        if (bf16 && eight) hipLaunchKernelGGL((adamw_kernel<true, true, Source>), grid, threads, 0, st, k, source);
+        else if (bf16) hipLaunchKernelGGL((adamw_kernel<true, false, Source>), grid, threads, 0, st, k, source);
+        else if (eight) hipLaunchKernelGGL((adamw_kernel<false, true, Source>), grid, threads, 0, st, k, source);
+        else hipLaunchKernelGGL((adamw_kernel<false, false, Source>), grid, threads, 0, st, k, source);
+    };
+    return list_launch<AwTensor, AW_MAX>(a->num_tensors, a->workspace, a->workspace_bytes, st, next, launch);
+}
+
+extern "C" size_t fdgs_adamw_workspace_bytes(int32_t num_tensors) {
+    return num_tensors > 2 * AW_MAX ? list_table_bytes(num_tensors, sizeof(AwTensor)) : 0;
 }
 
 // ---- 8-bit moments to values and back ----
-#define M8_MAX 92                                // tensors per launch
+#define M8_MAX 92                                // tensors whose records fill 4 KB of kernel arguments
 struct M8Tensor { uint8_t* codes; uint8_t* exps; void* value; long long n; uint32_t key; int is_signed; };
-struct M8Part {
-    int num, nearest;
-    int start[M8_MAX];
-    M8Tensor t[M8_MAX];
-};
-static_assert(sizeof(M8Part) <= 4096, "kernel arguments of one launch");
+static_assert(sizeof(AwPart<M8Tensor, M8_MAX>) + 8 <= 4096, "kernel arguments of one launch");
 
 // Eight consecutive values from element i on.  Eight to a lane: 8 bytes in and, as bfloat16, 16 out.
 template <bool BF16, bool SIGNED>
@@ -456,12 +543,12 @@ __device__ __forceinline__ void m8_unpack8(const M8Tensor& t, long long i) {
 }
 
 #define M8_PER_GROUP 8192                        // elements per workgroup
-template <bool BF16>
+template <bool BF16, class Source>
 __global__ void __launch_bounds__(256)
-moment8_unpack_kernel(M8Part k) {
-    const int ti = aw_find(k.start, k.num, (int)blockIdx.x);
-    const M8Tensor& t = k.t[ti];
-    const long long base = (long long)((int)blockIdx.x - k.start[ti]) * M8_PER_GROUP + 8 * (int)threadIdx.x;
+moment8_unpack_kernel(Source source) {
+    const int ti = aw_find(source.starts(), source.num(), (int)blockIdx.x);
+    const M8Tensor& t = source.record(ti);
+    const long long base = (long long)((int)blockIdx.x - source.starts()[ti]) * M8_PER_GROUP + 8 * (int)threadIdx.x;
     if (t.is_signed) {
 #pragma unroll
         for (int u = 0; u < M8_PER_GROUP / 2048; ++u) m8_unpack8<BF16, true>(t, base + u * 2048);
@@ -472,7 +559,7 @@ moment8_unpack_kernel(M8Part k) {
 }
 
 template <bool SIGNED>
-__device__ __forceinline__ void m8_pack_block(const M8Part& k, const M8Tensor& t, long long b) {
+__device__ __forceinline__ void m8_pack_block(bool nearest, const M8Tensor& t, long long b) {
     const int lane = threadIdx.x & 63;
     const long long i = b + 4 * lane;
     if (b >= t.n) return;                        // the whole wave
@@ -489,7 +576,7 @@ __device__ __forceinline__ void m8_pack_block(const M8Part& k, const M8Tensor& t
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         if (i + j >= t.n) break;
-        const uint32_t h = k.nearest ? 0x80008000u : m8_hash(((uint32_t)i + j + key) * M8_C1);
+        const uint32_t h = nearest ? 0x80008000u : m8_hash(((uint32_t)i + j + key) * M8_C1);
         const uint32_t all = __float_as_uint(x[j]);
         uint32_t code = m8_encode<SIGNED>(all & 0x7FFFFFFFu, SIGNED ? m8_noise_m(h) : m8_noise_v(h), base);
         if (SIGNED) code |= (all >> 24) & 128u;
@@ -498,16 +585,17 @@ __device__ __forceinline__ void m8_pack_block(const M8Part& k, const M8Tensor& t
     if (lane == 0) t.exps[b / M8_BLOCK] = (uint8_t)e;
 }
 
+template <class Source>
 __global__ void __launch_bounds__(256)
-moment8_pack_kernel(M8Part k) {
-    const int ti = aw_find(k.start, k.num, (int)blockIdx.x);
-    const M8Tensor& t = k.t[ti];
+moment8_pack_kernel(int nearest, Source source) {
+    const int ti = aw_find(source.starts(), source.num(), (int)blockIdx.x);
+    const M8Tensor& t = source.record(ti);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const long long base = (long long)((int)blockIdx.x - k.start[ti]) * M8_PER_GROUP + wave * (M8_PER_GROUP / 4);
+    const long long base = (long long)((int)blockIdx.x - source.starts()[ti]) * M8_PER_GROUP + wave * (M8_PER_GROUP / 4);
 #pragma unroll 1
     for (int u = 0; u < M8_PER_GROUP / 4 / M8_BLOCK; ++u) {
-        if (t.is_signed) m8_pack_block<true>(k, t, base + u * M8_BLOCK);
-        else m8_pack_block<false>(k, t, base + u * M8_BLOCK);
+        if (t.is_signed) m8_pack_block<true>(nearest != 0, t, base + u * M8_BLOCK);
+        else m8_pack_block<false>(nearest != 0, t, base + u * M8_BLOCK);
     }
 }
 
@@ -515,36 +603,38 @@ static int moment8_launch(const fdgs_moment8_args* a, void* stream, bool pack) {
     if (!a || a->num_tensors < 0 || (a->num_tensors > 0 && !a->tensors)) return FDGS_EINVAL;
     const bool bf16 = a->value_type == FDGS_TYPE_BF16;
     if ((bf16 && pack) || (!bf16 && a->value_type != FDGS_TYPE_F32)) return FDGS_EINVAL;
+    long long total = 0;                         // workgroups
     for (int i = 0; i < a->num_tensors; ++i) {
         const fdgs_moment8_tensor& s = a->tensors[i];
         if (s.numel < 0) return FDGS_EINVAL;
         if (s.numel == 0) continue;
         if (!s.codes || !s.exponents || !s.value) return FDGS_EINVAL;
-        if ((s.numel - 1) / M8_PER_GROUP >= 0x7fffffffLL / M8_MAX) return FDGS_ETOOLARGE;
+        total += (s.numel - 1) / M8_PER_GROUP + 1;
+        if (total > 0x7fffffffLL) return FDGS_ETOOLARGE;
     }
-    M8Part k;
-    k.nearest = a->nearest != 0;
-    for (int i = 0; i < a->num_tensors;) {
-        int blocks = 0;
-        k.num = 0;
-        for (; i < a->num_tensors && k.num < M8_MAX; ++i) {
-            const fdgs_moment8_tensor& s = a->tensors[i];
-            if (s.numel == 0) continue;
-            k.start[k.num] = blocks;
-            blocks += (int)((s.numel + M8_PER_GROUP - 1) / M8_PER_GROUP);
-            M8Tensor& t = k.t[k.num++];
-            t.codes = s.codes; t.exps = s.exponents; t.value = s.value;
-            t.n = s.numel; t.key = s.round_key; t.is_signed = s.is_signed != 0;
-        }
-        if (k.num == 0) break;
+    int i = 0;
+    auto next = [&](M8Tensor& t, int& groups) {
+        while (i < a->num_tensors && a->tensors[i].numel == 0) ++i;
+        if (i == a->num_tensors) return false;
+        const fdgs_moment8_tensor& s = a->tensors[i++];
+        groups = (int)((s.numel + M8_PER_GROUP - 1) / M8_PER_GROUP);
+        t.codes = s.codes; t.exps = s.exponents; t.value = s.value;
+        t.n = s.numel; t.key = s.round_key; t.is_signed = s.is_signed != 0;
+        return true;
+    };
+    hipStream_t st = (hipStream_t)stream;
+    auto launch = [&](const auto& source, int blocks) {
+        typedef std::remove_cv_t<std::remove_reference_t<decltype(source)>> Source;
         const dim3 grid((unsigned)blocks), threads(256);
-        hipStream_t st = (hipStream_t)stream;
-        if (pack) hipLaunchKernelGGL(moment8_pack_kernel, grid, threads, 0, st, k);
-        else if (bf16) hipLaunchKernelGGL(moment8_unpack_kernel<true>, grid, threads, 0, st, k);
-        else hipLaunchKernelGGL(moment8_unpack_kernel<false>, grid, threads, 0, st, k);
-        FDGS_CHECK_LAUNCH();
-    }
-    return FDGS_OK;
+        if (pack) hipLaunchKernelGGL((moment8_pack_kernel<Source>), grid, threads, 0, st, (int)(a->nearest != 0), source);
+        else if (bf16) hipLaunchKernelGGL((moment8_unpack_kernel<true, Source>), grid, threads, 0, st, source);
+        else hipLaunchKernelGGL((moment8_unpack_kernel<false, Source>), grid, threads, 0, st, source);
+    };
+    return list_launch<M8Tensor, M8_MAX>(a->num_tensors, a->workspace, a->workspace_bytes, st, next, launch);
+}
+
+extern "C" size_t fdgs_moment8_workspace_bytes(int32_t num_tensors) {
+    return num_tensors > 2 * M8_MAX ? list_table_bytes(num_tensors, sizeof(M8Tensor)) : 0;
 }
 
 extern "C" int fdgs_moment8_unpack(const fdgs_moment8_args* a, void* stream) { return moment8_launch(a, stream, false); }

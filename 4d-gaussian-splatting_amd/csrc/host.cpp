@@ -106,6 +106,8 @@ struct Library {
     int (*unpack8)(const fdgs_moment8_args*, void*) = nullptr;
     int (*pack8)(const fdgs_moment8_args*, void*) = nullptr;
     const char* (*strerror)(int) = nullptr;
+    size_t (*adamw_ws)(int32_t) = nullptr;
+    size_t (*moment8_ws)(int32_t) = nullptr;
     PyObject* module = nullptr;
 } library;
 
@@ -235,6 +237,9 @@ PyObject* adamw_step(PyObject* a) {
     args.beta2 = beta2;
     args.eps = eps;
     args.tensors = out.data();
+    args.workspace_bytes = library.adamw_ws(args.num_tensors);
+    const Tensor workspace = args.workspace_bytes ? at::empty({(int64_t)args.workspace_bytes}, first.options().dtype(at::kByte).requires_grad(false)) : Tensor();
+    args.workspace = args.workspace_bytes ? workspace.data_ptr() : nullptr;
     launch("fdgs_adamw_step", library.adamw, args, device);
     // written in place: a graph that has saved a parameter is to notice, as after torch's own steps
     for (Py_ssize_t i = 0; i < n; ++i) {
@@ -279,6 +284,10 @@ PyObject* moment8_convert(PyObject* a) {
     args.value_type = type == at::kBFloat16 ? FDGS_TYPE_BF16 : FDGS_TYPE_F32;
     args.nearest = ko == Py_None;
     args.tensors = out.data();
+    const c10::DeviceGuard guard(first.device());
+    args.workspace_bytes = library.moment8_ws(args.num_tensors);
+    const Tensor workspace = args.workspace_bytes ? at::empty({(int64_t)args.workspace_bytes}, first.options().dtype(at::kByte)) : Tensor();
+    args.workspace = args.workspace_bytes ? workspace.data_ptr() : nullptr;
     launch(pack ? "fdgs_moment8_pack" : "fdgs_moment8_unpack", pack ? library.pack8 : library.unpack8, args, first.device());
     Py_RETURN_NONE;
 }
@@ -505,12 +514,12 @@ PyObject* rows_layout(PyObject* a) {
     return Py_BuildValue("NLL", PyBool_FromLong(r.is_same(t)), (long long)width, (long long)stride);
 }
 
-// bind(module, addresses of fdgs_embedding_fwd, _bwd_workspace_bytes, _bwd, fdgs_adamw_step, fdgs_moment8_unpack, _pack and
-// fdgs_strerror)
+// bind(module, addresses of fdgs_embedding_fwd, _bwd_workspace_bytes, _bwd, fdgs_adamw_step, fdgs_moment8_unpack, _pack,
+// fdgs_strerror, fdgs_adamw_workspace_bytes, fdgs_moment8_workspace_bytes)
 PyObject* bind(PyObject* a) {
-    unsigned long long fwd, ws, bwd, adamw, unpack, pack, err;
+    unsigned long long fwd, ws, bwd, adamw, unpack, pack, err, adamw_ws, moment8_ws;
     PyObject* module;
-    if (!PyArg_ParseTuple(a, "OKKKKKKK", &module, &fwd, &ws, &bwd, &adamw, &unpack, &pack, &err)) throw Raised();
+    if (!PyArg_ParseTuple(a, "OKKKKKKKKK", &module, &fwd, &ws, &bwd, &adamw, &unpack, &pack, &err, &adamw_ws, &moment8_ws)) throw Raised();
     Py_INCREF(module);
     Py_XDECREF(library.module);
     library.module = module;
@@ -521,6 +530,8 @@ PyObject* bind(PyObject* a) {
     library.unpack8 = (decltype(library.unpack8))(uintptr_t)unpack;
     library.pack8 = (decltype(library.pack8))(uintptr_t)pack;
     library.strerror = (decltype(library.strerror))(uintptr_t)err;
+    library.adamw_ws = (decltype(library.adamw_ws))(uintptr_t)adamw_ws;
+    library.moment8_ws = (decltype(library.moment8_ws))(uintptr_t)moment8_ws;
     Py_RETURN_NONE;
 }
 

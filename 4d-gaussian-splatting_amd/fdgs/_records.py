@@ -17,7 +17,7 @@ class AdamWTensor(C.Structure):
 class AdamWArgs(C.Structure):
     _fields_ = [("num_tensors", C.c_int32), ("param_type", C.c_int32), ("state_bits", C.c_int32),
                 ("reserved", C.c_int32), ("beta1", C.c_double), ("beta2", C.c_double), ("eps", C.c_double),
-                ("tensors", C.c_char_p)]
+                ("tensors", C.c_char_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
 
 
 class Moment8Tensor(C.Structure):
@@ -27,7 +27,7 @@ class Moment8Tensor(C.Structure):
 
 class Moment8Args(C.Structure):
     _fields_ = [("num_tensors", C.c_int32), ("value_type", C.c_int32), ("nearest", C.c_int32), ("reserved", C.c_int32),
-                ("tensors", C.c_char_p)]
+                ("tensors", C.c_char_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
 
 
 EMBEDDING_MAX_TOKENS = 1 << 30          # FDGS_EMBEDDING_MAX_TOKENS

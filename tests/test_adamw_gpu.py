@@ -351,10 +351,12 @@ def test_capture_is_refused_and_leaves_the_state_alone():
     assert (q == 2).all() and (p == 1).all() and (m == 0).all()
 
 
-def test_more_tensors_than_one_launch_takes():
+@pytest.mark.parametrize("count", [40, 41, 80, 81, 171, 400])
+def test_more_tensors_than_one_launch_takes(count):
+    """Lists at the limits of a launch's arguments, and of the table in device memory that longer ones go through."""
     from fdgs import adamw
     rng = np.random.default_rng(0)
-    sizes = [int(n) for n in rng.integers(0, 700, 171)]
+    sizes = [int(n) for n in rng.integers(0, 700, count)]
     data = _inputs(sizes, 5)
     ps, gs, ms, vs = ([torch.from_numpy(d[k]).cuda() for d in data] for k in range(4))
     adamw.adamw_step(ps, gs, ms, vs, steps=3, lr=1e-3, weight_decay=0.0)
@@ -365,3 +367,6 @@ def test_more_tensors_than_one_launch_takes():
         denom = np.sqrt(v64 / (1 - 0.999 ** 3)) + 1e-8
         scale = 1e-3 / (1 - 0.9 ** 3) / denom
         _within(p.cpu().numpy(), w64, 12.2 * U * np.abs(m64) * scale + 1.01 * tol * scale + 4.04 * U * np.abs(d[0]) + 2.0 ** -149, "w")
+    packed = adamw.pack8(ms, True)                               # and their conversions, there and back
+    for m, x in zip(ms, adamw.unpack8(packed)):
+        assert np.array_equal(x.cpu().numpy(), ac.decode(*ac.encode(m.cpu().numpy(), 0x8000, True), True))
