@@ -174,7 +174,7 @@ extern "C" int fdgs_embedding_fwd(const fdgs_embedding_fwd_args* a, void* stream
 
 __global__ void __launch_bounds__(ER_THREADS)
 embedding_rank_kernel(const void* __restrict__ ids, int tokens, int wide, long long padding, uint32_t rows,
-                      uint32_t* __restrict__ keys, uint32_t* __restrict__ perm) {
+                      uint2* __restrict__ sorted) {
     __shared__ __align__(16) uint32_t sk[ER_CHUNK];
     __shared__ uint32_t part[4][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -209,8 +209,7 @@ embedding_rank_kernel(const void* __restrict__ ids, int tokens, int wide, long l
     __syncthreads();
     if (wave == 0 && me < tokens) {
         const uint32_t r = part[0][lane] + part[1][lane] + part[2][lane] + part[3][lane];
-        keys[r] = key;
-        perm[r] = (uint32_t)me;
+        sorted[r] = make_uint2(key, (uint32_t)me);
     }
 }
 
@@ -225,7 +224,7 @@ embedding_rank_kernel(const void* __restrict__ ids, int tokens, int wide, long l
 
 __global__ void __launch_bounds__(EB_THREADS)
 embedding_bucket_kernel(const void* __restrict__ ids, int tokens, int wide, long long padding, uint32_t rows, int shift,
-                        uint32_t* __restrict__ keys, uint32_t* __restrict__ perm, uint32_t* __restrict__ start) {
+                        uint2* __restrict__ out, uint32_t* __restrict__ start) {
     extern __shared__ __align__(16) uint32_t eb_lds[];
     __shared__ uint32_t wsum[EB_THREADS / 64], without;
     uint32_t* lkey = eb_lds;
@@ -285,19 +284,17 @@ embedding_bucket_kernel(const void* __restrict__ ids, int tokens, int wide, long
     }
     __syncthreads();
     for (int i = threadIdx.x; i < tokens; i += EB_THREADS) {
-        keys[i] = lkey[i];
-        perm[i] = ltok[i];
+        out[i] = make_uint2(lkey[i], ltok[i]);
     }
 }
 
 __global__ void __launch_bounds__(ER_THREADS)
-embedding_place_kernel(const uint32_t* __restrict__ keys_in, const uint32_t* __restrict__ perm_in,
-                       const uint32_t* __restrict__ start, int tokens, int shift, uint32_t rows, uint32_t* __restrict__ keys,
-                       uint32_t* __restrict__ perm) {
+embedding_place_kernel(const uint2* __restrict__ in, const uint32_t* __restrict__ start, int tokens, int shift, uint32_t rows,
+                       uint2* __restrict__ sorted) {
     __shared__ uint32_t part[4][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int own = blockIdx.x * 64, me = min(own + lane, tokens - 1);
-    const uint32_t key = keys_in[me], tok = perm_in[me];
+    const uint32_t key = in[me].x, tok = in[me].y;
     // the buckets that the 64 places touch, from the first one's first token to the last one's last
     const uint32_t kf = (uint32_t)__builtin_amdgcn_readfirstlane((int)key), kl = (uint32_t)__builtin_amdgcn_readlane((int)key, 63);
     const int lo = kf == rows ? 0 : (int)start[kf >> shift];
@@ -307,10 +304,10 @@ embedding_place_kernel(const uint32_t* __restrict__ keys_in, const uint32_t* __r
     // a wave's share of them, 64 at a time: a lane loads one, all lanes compare with each
     for (int b = lo + wave * 64; b < hi; b += 256) {
         const int j = b + lane;
-        const uint32_t ok = j < hi ? keys_in[j] : 0xFFFFFFFFu, ot = j < hi ? perm_in[j] : 0xFFFFFFFFu;
+        const uint2 other = j < hi ? in[j] : make_uint2(0xFFFFFFFFu, 0xFFFFFFFFu);
 #pragma unroll 16
         for (int q = 0; q < 64; ++q) {
-            const uint32_t kq = (uint32_t)__builtin_amdgcn_readlane((int)ok, q), tq = (uint32_t)__builtin_amdgcn_readlane((int)ot, q);
+            const uint32_t kq = (uint32_t)__builtin_amdgcn_readlane((int)other.x, q), tq = (uint32_t)__builtin_amdgcn_readlane((int)other.y, q);
             before += (((unsigned long long)kq << 32) | tq) < mine ? 1u : 0u;
         }
     }
@@ -318,8 +315,7 @@ embedding_place_kernel(const uint32_t* __restrict__ keys_in, const uint32_t* __r
     __syncthreads();
     if (wave == 0 && own + lane < tokens) {
         const uint32_t r = key == rows ? (uint32_t)me : (uint32_t)lo + part[0][lane] + part[1][lane] + part[2][lane] + part[3][lane];
-        keys[r] = key;
-        perm[r] = tok;
+        sorted[r] = make_uint2(key, tok);
     }
 }
 
@@ -331,9 +327,9 @@ embedding_place_kernel(const uint32_t* __restrict__ keys_in, const uint32_t* __r
 #define EX_MAX_BLOCKS 1024
 
 struct EmSort {
-    const void* ids;                                 // first pass: the tokens' ids; later passes: keys_in
-    const uint32_t* keys_in; const uint32_t* perm_in;
-    uint32_t* keys_out; uint32_t* perm_out;
+    const void* ids;                                 // first pass: the tokens' ids; later passes: the pairs `in`
+    const uint2* in;
+    uint2* out;
     uint32_t* hist; uint32_t* totals;
     long long padding;
     uint32_t rows, mask;
@@ -342,7 +338,7 @@ struct EmSort {
 
 template <bool FIRST>
 __device__ __forceinline__ uint32_t ex_key(const EmSort& a, int i) {
-    return FIRST ? em_key(a.ids, i, a.wide, a.padding, a.rows) : a.keys_in[i];
+    return FIRST ? em_key(a.ids, i, a.wide, a.padding, a.rows) : a.in[i].x;
 }
 
 template <bool FIRST>
@@ -395,6 +391,7 @@ embedding_scan_kernel(uint32_t* __restrict__ hist, uint32_t* __restrict__ totals
     sums[chunk][d] = s;
     __syncthreads();
     uint32_t run = 0, all = 0;
+#pragma unroll
     for (int c = 0; c < 32; ++c) {
         run += c < chunk ? sums[c][d] : 0u;
         all += sums[c][d];
@@ -414,7 +411,7 @@ embedding_scatter_kernel(EmSort a) {
     __shared__ uint32_t running[EX_BINS];            // next place of each digit for this workgroup
     __shared__ uint32_t cnt[4][EX_BINS];             // a wave's count of each digit, then where its first one lies in the tile
     __shared__ uint32_t shift_to[EX_BINS];           // from a place in the tile to the place in the output
-    __shared__ uint32_t lk[EX_TILE(EX_IPL)], lt[EX_TILE(EX_IPL)];   // the tile in the order of its digits
+    __shared__ uint2 ordered[EX_TILE(EX_IPL)];       // the tile in the order of its digits
     __shared__ uint32_t wsum[4];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int bins = 1 << a.bits;
@@ -440,8 +437,14 @@ embedding_scatter_kernel(EmSort a) {
 #pragma unroll
         for (int k = 0; k < EX_IPL; ++k) {
             const int i = at + 64 * k;
-            key[k] = i < end ? ex_key<FIRST>(a, i) : 0xFFFFFFFFu;
-            tok[k] = FIRST ? (uint32_t)i : (i < end ? a.perm_in[i] : 0u);
+            if (FIRST) {
+                key[k] = i < end ? ex_key<true>(a, i) : 0xFFFFFFFFu;
+                tok[k] = (uint32_t)i;
+            } else {
+                const uint2 e = i < end ? a.in[i] : make_uint2(0xFFFFFFFFu, 0u);
+                key[k] = e.x;
+                tok[k] = e.y;
+            }
         }
 #pragma unroll
         for (int k = 0; k < EX_IPL; ++k) {
@@ -489,16 +492,14 @@ embedding_scatter_kernel(EmSort a) {
         for (int k = 0; k < EX_IPL; ++k) {
             if (at + 64 * k < end) {
                 const uint32_t to = cnt[wave][(key[k] >> a.shift) & a.mask] + rank[k];
-                lk[to] = key[k];
-                lt[to] = tok[k];
+                ordered[to] = make_uint2(key[k], tok[k]);
             }
         }
         __syncthreads();
         const int have = min(end - tile, EX_TILE(EX_IPL));
         for (int j = threadIdx.x; j < have; j += EX_THREADS) {
-            const uint32_t kj = lk[j], to = shift_to[(kj >> a.shift) & a.mask] + (uint32_t)j;
-            a.keys_out[to] = kj;
-            a.perm_out[to] = lt[j];
+            const uint2 e = ordered[j];
+            a.out[shift_to[(e.x >> a.shift) & a.mask] + (uint32_t)j] = e;
         }
         __syncthreads();
     }
@@ -512,7 +513,7 @@ embedding_scatter_kernel(EmSort a) {
 #define EW_SMALL 128                                 // so few tokens are sorted by every workgroup for itself
 
 struct EmBwd {
-    const uint32_t* keys; const uint32_t* perm;      // sorted
+    const uint2* sorted;                             // (key, token)
     const void* ids; const void* dout; void* dtable;
     float* head; float* tail;                        // [shares][dim] partial sums of rows that a share's end cuts
     uint32_t* info;                                  // [shares] EW_HEAD | row: the share ends a row that began earlier
@@ -524,13 +525,13 @@ struct EmBwd {
 #define EW_HEAD 0x80000000u
 
 // First sorted token whose place in the sequence (its index + its key) is not below `d`, by the whole wave.
-__device__ __forceinline__ int ew_search(const uint32_t* __restrict__ keys, int tokens, long long d) {
+__device__ __forceinline__ int ew_search(const uint2* __restrict__ sorted, int tokens, long long d) {
     const int lane = threadIdx.x & 63;
     int lo = 0, hi = d < tokens ? (int)d : tokens;   // places grow by one at least: token d's is not below d
     while (lo < hi) {
         const int step = (hi - lo + 63) / 64;
         const int i = lo + lane * step;
-        const int less = __popcll(__ballot(i < hi && (long long)i + (long long)keys[i] < d));   // a prefix of the lanes
+        const int less = __popcll(__ballot(i < hi && (long long)i + (long long)sorted[i].x < d));   // a prefix of the lanes
         if (less == 0) break;
         hi = min(hi, lo + less * step);
         lo += (less - 1) * step + 1;
@@ -573,7 +574,7 @@ embedding_walk_kernel(EmBwd a) {
         k1 = i1 = a.tokens;
     } else {
         if (wave < 2) {
-            const int i = ew_search(a.keys, a.tokens, wave ? d1 : d0);
+            const int i = ew_search(a.sorted, a.tokens, wave ? d1 : d0);
             if ((threadIdx.x & 63) == 0) bound[wave] = i;
         }
         __syncthreads();
@@ -582,8 +583,9 @@ embedding_walk_kernel(EmBwd a) {
         k0 = max(i0 - 1, 0);
         k1 = i1;                                     // k1 - k0 <= span + 1 <= cap
         for (int j = k0 + (int)threadIdx.x; j < k1; j += EW_THREADS) {
-            sk[j - k0] = a.keys[j];
-            sp[j - k0] = a.perm[j];
+            const uint2 e = a.sorted[j];
+            sk[j - k0] = e.x;
+            sp[j - k0] = e.y;
         }
     }
     __syncthreads();
@@ -755,7 +757,7 @@ embedding_join_kernel(EmBwd a) {
         while (lo < hi) {
             const int step = (hi - lo + 63) / 64;
             const int i = lo + lane * step;
-            const int less = __popcll(__ballot(i < hi && a.keys[i] < row));
+            const int less = __popcll(__ballot(i < hi && a.sorted[i].x < row));
             if (less == 0) break;
             hi = min(hi, lo + less * step);
             lo += (less - 1) * step + 1;
@@ -788,7 +790,7 @@ embedding_join_kernel(EmBwd a) {
 struct EmPlan {
     int vec, nv, tiles, lanes, groups, share;
     long long shares, blocks;
-    size_t keys, perm, keys2, perm2, hist, totals, info, fresh, head, tail, bytes;   // offsets into the workspace
+    size_t sorted, other, hist, totals, info, fresh, head, tail, bytes;   // offsets into the workspace
 };
 
 static int em_full(int type) { return type == FDGS_TYPE_F32 ? EmF32::full : EmBf16::full; }
@@ -814,11 +816,9 @@ static EmPlan em_plan(long long tokens, long long rows, int dim, int type) {
     p.shares = p.blocks * p.groups;
     size_t at = 0;
     auto take = [&at](size_t n) { const size_t o = at; at += (n + 255) / 256 * 256; return o; };
-    p.keys = take(tokens * 4);
-    p.perm = take(tokens * 4);
+    p.sorted = take(tokens * 8);
     const bool radix = tokens > ER_MAX_TOKENS, buckets = tokens > ER_DIRECT && !radix;
-    p.keys2 = take(radix || buckets ? tokens * 4 : 0);
-    p.perm2 = take(radix || buckets ? tokens * 4 : 0);
+    p.other = take(radix || buckets ? tokens * 8 : 0);
     p.hist = take(radix ? (size_t)EX_BINS * EX_MAX_BLOCKS * 4 : buckets ? (EB_BUCKETS + 1) * 4 : 0);
     p.totals = take(radix ? EX_BINS * 4 : 0);
     const bool small = tokens <= EW_SMALL;           // no row is cut
@@ -835,7 +835,7 @@ extern "C" size_t fdgs_embedding_bwd_workspace_bytes(int64_t num_tokens, int32_t
     return em_plan(num_tokens, num_rows, dim, type).bytes;
 }
 
-// Sorted pairs end up in (ws + p.keys, ws + p.perm).
+// The sorted pairs end up at ws + p.sorted.
 static int em_sort(const fdgs_embedding_bwd_args* a, const EmPlan& p, char* ws, hipStream_t s) {
     const int tokens = (int)a->num_tokens;
     const long long padding = a->padding_id >= 0 ? a->padding_id : -1;
@@ -844,7 +844,7 @@ static int em_sort(const fdgs_embedding_bwd_args* a, const EmPlan& p, char* ws, 
     while (key_bits < 31 && (1ll << key_bits) <= (long long)a->num_rows) ++key_bits;   // keys 0 .. num_rows
     if (tokens <= ER_DIRECT) {
         hipLaunchKernelGGL(embedding_rank_kernel, dim3((tokens + 63) / 64), dim3(ER_THREADS), 0, s, a->ids, tokens, wide, padding,
-                           (uint32_t)a->num_rows, (uint32_t*)(ws + p.keys), (uint32_t*)(ws + p.perm));
+                           (uint32_t)a->num_rows, (uint2*)(ws + p.sorted));
         FDGS_CHECK_LAUNCH();
         return FDGS_OK;
     }
@@ -853,12 +853,13 @@ static int em_sort(const fdgs_embedding_bwd_args* a, const EmPlan& p, char* ws, 
         static_assert(EB_BUCKETS == 1 << 11, "buckets of the upper 11 bits");
         if (hipFuncSetAttribute((const void*)embedding_bucket_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, EB_LDS) != hipSuccess)
             return FDGS_ELAUNCH;
-        uint32_t *keys2 = (uint32_t*)(ws + p.keys2), *perm2 = (uint32_t*)(ws + p.perm2), *start = (uint32_t*)(ws + p.hist);
+        uint2* other = (uint2*)(ws + p.other);
+        uint32_t* start = (uint32_t*)(ws + p.hist);
         hipLaunchKernelGGL(embedding_bucket_kernel, dim3(1), dim3(EB_THREADS), EB_LDS, s, a->ids, tokens, wide, padding,
-                           (uint32_t)a->num_rows, shift, keys2, perm2, start);
+                           (uint32_t)a->num_rows, shift, other, start);
         FDGS_CHECK_LAUNCH();
-        hipLaunchKernelGGL(embedding_place_kernel, dim3((tokens + 63) / 64), dim3(ER_THREADS), 0, s, keys2, perm2, start, tokens, shift,
-                           (uint32_t)a->num_rows, (uint32_t*)(ws + p.keys), (uint32_t*)(ws + p.perm));
+        hipLaunchKernelGGL(embedding_place_kernel, dim3((tokens + 63) / 64), dim3(ER_THREADS), 0, s, other, start, tokens, shift,
+                           (uint32_t)a->num_rows, (uint2*)(ws + p.sorted));
         FDGS_CHECK_LAUNCH();
         return FDGS_OK;
     }
@@ -875,11 +876,9 @@ static int em_sort(const fdgs_embedding_bwd_args* a, const EmPlan& p, char* ws, 
     for (int pass = 0; pass < passes; ++pass) {
         k.bits = (key_bits - k.shift + passes - pass - 1) / (passes - pass);           // the remaining bits, evenly
         k.mask = (1u << k.bits) - 1u;
-        const bool to_first = ((passes - 1 - pass) & 1) == 0;                          // the last pass ends in keys / perm
-        k.keys_out = (uint32_t*)(ws + (to_first ? p.keys : p.keys2));
-        k.perm_out = (uint32_t*)(ws + (to_first ? p.perm : p.perm2));
-        k.keys_in = (const uint32_t*)(ws + (to_first ? p.keys2 : p.keys));
-        k.perm_in = (const uint32_t*)(ws + (to_first ? p.perm2 : p.perm));
+        const bool to_first = ((passes - 1 - pass) & 1) == 0;                          // the last pass ends in `sorted`
+        k.out = (uint2*)(ws + (to_first ? p.sorted : p.other));
+        k.in = (const uint2*)(ws + (to_first ? p.other : p.sorted));
         const dim3 grid((unsigned)blocks), threads(EX_THREADS);
         if (pass == 0) hipLaunchKernelGGL(embedding_hist_kernel<true>, grid, threads, 0, s, k);
         else hipLaunchKernelGGL(embedding_hist_kernel<false>, grid, threads, 0, s, k);
@@ -937,7 +936,7 @@ extern "C" int fdgs_embedding_bwd(const fdgs_embedding_bwd_args* a, void* stream
         if (rc != FDGS_OK) return rc;
     }
     EmBwd k = {};
-    k.keys = (const uint32_t*)(ws + p.keys); k.perm = (const uint32_t*)(ws + p.perm);
+    k.sorted = (const uint2*)(ws + p.sorted);
     k.dout = a->grad_out; k.dtable = a->grad_table;
     k.head = (float*)(ws + p.head); k.tail = (float*)(ws + p.tail); k.fresh = (uint8_t*)(ws + p.fresh);
     k.info = (uint32_t*)(ws + p.info); k.shares = (int)p.shares;
