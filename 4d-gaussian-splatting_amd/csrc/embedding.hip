@@ -11,9 +11,8 @@
 // then the row's write - cut into shares of equal length.  A token's place in that sequence is i + id(i), so a share finds
 // its first token by one search and needs no table of row starts; a share costs the same whether it holds the tokens
 // of one frequent row or the zeros of many rows that nobody asked for.  A row that is cut by a share's end leaves
-// partial sums in the workspace, which a last launch adds up in the shares' order.  No atomics.
+// partial sums in the workspace, which a last launch adds up in the shares' order.  No atomic touches a sum.
 #include "fdgs_common.h"
-#include <hip/hip_bf16.h>
 
 // ---- element types: 16 bytes to a vector where the row is that long, else one element ----
 typedef uint32_t em_u4 __attribute__((ext_vector_type(4)));
@@ -90,6 +89,8 @@ struct EmFwd {
 
 // A workgroup has whole tokens, as many as make up to 1024 vectors (or, of a longer row, 1024 vectors of one token): a
 // thread has up to four vectors, all of whose ids and then all of whose rows are asked for before the first is used.
+// Bound by the output's lines and, where the table does not fit an XCD's 4 MB of L2, by the rows that come from behind it:
+// 300,000 x 48 floats 14 us (4.4 TB/s), 2,000,000 x 48 from 65,536 rows 120 us, from 8,192 rows 66 us (5.8 TB/s).
 template <class T, int VEC>
 __global__ void __launch_bounds__(EF_THREADS)
 embedding_fwd_kernel(EmFwd a) {
@@ -144,7 +145,6 @@ static int em_fwd_launch(const EmFwd& k0, hipStream_t s) {
 }
 
 static bool em_type_ok(int t) { return t == FDGS_TYPE_F32 || t == FDGS_TYPE_BF16 || t == FDGS_TYPE_F16; }
-#define EM_MAX_DIM (1 << 24)                         // column tiles stay within a grid's second dimension
 
 extern "C" int fdgs_embedding_fwd(const fdgs_embedding_fwd_args* a, void* stream) {
     if (!a || a->num_tokens < 0 || a->num_rows < 0 || a->dim < 0 || !em_type_ok(a->type)) return FDGS_EINVAL;
@@ -152,7 +152,7 @@ extern "C" int fdgs_embedding_fwd(const fdgs_embedding_fwd_args* a, void* stream
     if (a->num_tokens == 0 || a->dim == 0) return FDGS_OK;
     if (!a->ids || !a->out || (a->num_rows > 0 && !a->table)) return FDGS_EINVAL;
     if (a->num_rows > 0 && a->table_row_stride < 0) return FDGS_EINVAL;
-    if (a->dim > EM_MAX_DIM || a->num_tokens > 0x7fffffffLL) return FDGS_ETOOLARGE;
+    if (a->dim > FDGS_EMBEDDING_MAX_DIM || a->num_tokens > 0x7fffffffLL) return FDGS_ETOOLARGE;
     EmFwd k = {};
     k.ids = a->ids; k.table = a->table; k.out = a->out;
     k.tokens = (int)a->num_tokens; k.table_stride = a->table_row_stride;
@@ -170,7 +170,7 @@ extern "C" int fdgs_embedding_fwd(const fdgs_embedding_fwd_args* a, void* stream
 #define ER_THREADS 256
 #define ER_CHUNK 4096                                // keys staged in LDS at a time
 #define ER_DIRECT 4096                               // up to here in one launch; beyond, by buckets:
-#define ER_MAX_TOKENS 16384                          // what a workgroup's LDS sorts into buckets
+#define ER_MAX_TOKENS 16384                          // beyond, T^2 comparisons of equal ids would take long
 
 __global__ void __launch_bounds__(ER_THREADS)
 embedding_rank_kernel(const void* __restrict__ ids, int tokens, int wide, long long padding, uint32_t rows,
@@ -213,31 +213,32 @@ embedding_rank_kernel(const void* __restrict__ ids, int tokens, int wide, long l
     }
 }
 
-// More: one workgroup puts the tokens into up to 2048 buckets by the upper bits of their keys, in LDS and in no
-// particular order, then a token's place is counted among the tokens of its bucket alone (and of those that the same 64
-// places touch), by key and then by token.  T^2 comparisons remain only where most tokens have one id.  At 16,384 tokens
-// of 65,536 rows, a frequent one among them and a fifth of the tokens without a row, 22 us; against all tokens it was 68.
+// More: every workgroup puts 4096 tokens into 2048 buckets by the upper bits of their keys, in LDS and in no particular
+// order, which makes a list of each 4096; then a token's place is counted among the tokens of its bucket alone (and of those
+// that the same 64 places touch) in every list, by key and then by token, a wave for a list.  T^2 comparisons remain only
+// where most tokens have one id.  At 16,384 tokens of 65,536 rows, a frequent one among them and a fifth of the tokens without a
+// row, 16 us; with one list of all tokens 22, against all tokens without buckets 68.
 #define EB_THREADS 1024
-#define EB_PER (ER_MAX_TOKENS / EB_THREADS)
+#define EB_LIST 4096
+#define EB_PER (EB_LIST / EB_THREADS)
 #define EB_BUCKETS 2048
-#define EB_LDS (ER_MAX_TOKENS * 6 + EB_BUCKETS * 4)  // keys, tokens (16 bits), counts: 104 KB
+#define EB_STARTS (EB_BUCKETS + 1)                   // where a list's buckets start, and where its last one ends
 
 __global__ void __launch_bounds__(EB_THREADS)
 embedding_bucket_kernel(const void* __restrict__ ids, int tokens, int wide, long long padding, uint32_t rows, int shift,
-                        uint2* __restrict__ out, uint32_t* __restrict__ start) {
-    extern __shared__ __align__(16) uint32_t eb_lds[];
-    __shared__ uint32_t wsum[EB_THREADS / 64], without;
-    uint32_t* lkey = eb_lds;
-    uint32_t* count = eb_lds + ER_MAX_TOKENS;
-    uint16_t* ltok = (uint16_t*)(count + EB_BUCKETS);
+                        uint2* __restrict__ lists, uint32_t* __restrict__ starts) {
+    __shared__ uint2 ordered[EB_LIST];
+    __shared__ uint32_t count[EB_BUCKETS], wsum[EB_THREADS / 64], without;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int from = blockIdx.x * EB_LIST, have = min(tokens - from, EB_LIST);
+    uint32_t* start = starts + blockIdx.x * EB_STARTS;
     count[threadIdx.x] = 0;
     count[threadIdx.x + EB_THREADS] = 0;
     uint32_t key[EB_PER], slot[EB_PER];
 #pragma unroll
     for (int k = 0; k < EB_PER; ++k) {
         const int i = threadIdx.x + k * EB_THREADS;
-        key[k] = i < tokens ? em_key(ids, i, wide, padding, rows) : 0xFFFFFFFFu;
+        key[k] = i < have ? em_key(ids, from + i, wide, padding, rows) : 0xFFFFFFFFu;
     }
     if (threadIdx.x == 0) without = 0;
     __syncthreads();
@@ -266,60 +267,71 @@ embedding_bucket_kernel(const void* __restrict__ ids, int tokens, int wide, long
 #pragma unroll
     for (int w = 0; w < EB_THREADS / 64; ++w)
         if (w < wave) base += wsum[w];
-    const uint32_t first = base + incl - c0 - c1;
+    const uint32_t first = base + incl - c0 - c1, valid = (uint32_t)have - without;
     count[2 * threadIdx.x] = first;
     count[2 * threadIdx.x + 1] = first + c0;
     start[2 * threadIdx.x] = first;
     start[2 * threadIdx.x + 1] = first + c0;
-    if (threadIdx.x == 0) start[EB_BUCKETS] = (uint32_t)tokens - without;
+    if (threadIdx.x == 0) start[EB_BUCKETS] = valid;
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < EB_PER; ++k) {
         const int i = threadIdx.x + k * EB_THREADS;
-        if (i < tokens) {
-            const uint32_t to = slot[k] + (key[k] == rows ? (uint32_t)tokens - without : count[key[k] >> shift]);
-            lkey[to] = key[k];
-            ltok[to] = (uint16_t)i;
-        }
+        if (i < have) ordered[slot[k] + (key[k] == rows ? valid : count[key[k] >> shift])] = make_uint2(key[k], (uint32_t)(from + i));
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < tokens; i += EB_THREADS) {
-        out[i] = make_uint2(lkey[i], ltok[i]);
-    }
+    for (int i = threadIdx.x; i < have; i += EB_THREADS) lists[from + i] = ordered[i];
 }
 
 __global__ void __launch_bounds__(ER_THREADS)
-embedding_place_kernel(const uint2* __restrict__ in, const uint32_t* __restrict__ start, int tokens, int shift, uint32_t rows,
-                       uint2* __restrict__ sorted) {
+embedding_place_kernel(const uint2* __restrict__ lists, const uint32_t* __restrict__ starts, int tokens, int nlists, int shift,
+                       uint32_t rows, uint2* __restrict__ sorted) {
     __shared__ uint32_t part[4][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int own = blockIdx.x * 64, me = min(own + lane, tokens - 1);
-    const uint32_t key = in[me].x, tok = in[me].y;
-    // the buckets that the 64 places touch, from the first one's first token to the last one's last
+    const int own = blockIdx.x * 64, me = min(own + lane, tokens - 1);   // 64 places of one list
+    const uint2 mine2 = lists[me];
+    const uint32_t key = mine2.x;
+    const unsigned long long mine = ((unsigned long long)key << 32) | mine2.y;
+    // the buckets that the 64 places touch, the first one's and the last one's
     const uint32_t kf = (uint32_t)__builtin_amdgcn_readfirstlane((int)key), kl = (uint32_t)__builtin_amdgcn_readlane((int)key, 63);
-    const int lo = kf == rows ? 0 : (int)start[kf >> shift];
-    const int hi = kf == rows ? 0 : (int)start[kl == rows ? EB_BUCKETS : (kl >> shift) + 1];
-    const unsigned long long mine = ((unsigned long long)key << 32) | tok;
+    const int bf = kf == rows ? EB_BUCKETS : (int)(kf >> shift), bl = kl == rows ? EB_BUCKETS : (int)(kl >> shift) + 1;
     uint32_t before = 0;
-    // a wave's share of them, 64 at a time: a lane loads one, all lanes compare with each
-    for (int b = lo + wave * 64; b < hi; b += 256) {
-        const int j = b + lane;
-        const uint2 other = j < hi ? in[j] : make_uint2(0xFFFFFFFFu, 0xFFFFFFFFu);
+    if (kf != rows) {
+        for (int l = wave; l < nlists; l += 4) {
+            const uint2* __restrict__ list = lists + (size_t)l * EB_LIST;
+            const int lo = (int)starts[l * EB_STARTS + bf], hi = (int)starts[l * EB_STARTS + bl];
+            before += (uint32_t)lo;                  // all of the list's smaller buckets
+            // the buckets themselves, 64 tokens at a time: a lane loads one, all lanes compare with each
+            for (int b = lo; b < hi; b += 64) {
+                const uint2 other = b + lane < hi ? list[b + lane] : make_uint2(0xFFFFFFFFu, 0xFFFFFFFFu);
 #pragma unroll 16
-        for (int q = 0; q < 64; ++q) {
-            const uint32_t kq = (uint32_t)__builtin_amdgcn_readlane((int)other.x, q), tq = (uint32_t)__builtin_amdgcn_readlane((int)other.y, q);
-            before += (((unsigned long long)kq << 32) | tq) < mine ? 1u : 0u;
+                for (int q = 0; q < 64; ++q) {
+                    const uint32_t kq = (uint32_t)__builtin_amdgcn_readlane((int)other.x, q), tq = (uint32_t)__builtin_amdgcn_readlane((int)other.y, q);
+                    before += (((unsigned long long)kq << 32) | tq) < mine ? 1u : 0u;
+                }
+            }
         }
     }
     part[wave][lane] = before;
     __syncthreads();
     if (wave == 0 && own + lane < tokens) {
-        const uint32_t r = key == rows ? (uint32_t)me : (uint32_t)lo + part[0][lane] + part[1][lane] + part[2][lane] + part[3][lane];
-        sorted[r] = make_uint2(key, tok);
+        uint32_t r = part[0][lane] + part[1][lane] + part[2][lane] + part[3][lane];
+        if (key == rows) {                           // behind all that have a row: list by list, as they lie
+            const int at = own / EB_LIST;
+            r = 0;
+            for (int l = 0; l < nlists; ++l) {
+                const uint32_t valid = starts[l * EB_STARTS + EB_BUCKETS];
+                r += valid;
+                if (l < at) r += (uint32_t)EB_LIST - valid;
+                if (l == at) r += (uint32_t)(me - at * EB_LIST) - valid;
+            }
+        }
+        sorted[r] = mine2;
     }
 }
 
-// Many tokens: a radix sort by digits of at most 9 bits (two passes for tables of up to 262,143 rows), three launches a pass (counts of each workgroup, their scan, scatter).
+// Many tokens: a radix sort by digits of at most 9 bits (two passes for tables of up to 262,143 rows), three launches a
+// pass: counts of each workgroup, their scan, scatter.  2,000,000 tokens of 65,536 rows 57 us, 300,000 of 8,192 29 us.
 #define EX_THREADS 256
 #define EX_TILE(ipl) (EX_THREADS * (ipl))             // tokens that a workgroup takes at a time, ipl to a lane
 #define EX_BITS 9
@@ -686,7 +698,7 @@ embedding_walk_kernel(EmBwd a) {
 }
 
 // ---- rows that were cut: the partial sums of the shares from the row's first token on, in order ----
-#define EC_SCAN 16                                   // shares that a workgroup looks at, at least
+#define EC_SCAN 4                                   // shares that a workgroup looks at, at least
 #define EC_LONG (-2)                                 // more partial sums than two looks at the flags reach: 16
 
 template <class T, int VEC>
@@ -743,9 +755,9 @@ embedding_join_kernel(EmBwd a) {
             float acc[VEC];
 #pragma unroll
             for (int j = 0; j < VEC; ++j) acc[j] = 0.0f;
+            ec_add<VEC>(a.head + (long long)end_of[e] * a.dim + col, acc);
 #pragma unroll 4
             for (int q = first_of[e]; q < end_of[e]; ++q) ec_add<VEC>(a.tail + (long long)q * a.dim + col, acc);
-            ec_add<VEC>(a.head + (long long)end_of[e] * a.dim + col, acc);
             ec_write<T, VEC>(a, row_of[e], col, acc);
         }
     }
@@ -819,7 +831,7 @@ static EmPlan em_plan(long long tokens, long long rows, int dim, int type) {
     p.sorted = take(tokens * 8);
     const bool radix = tokens > ER_MAX_TOKENS, buckets = tokens > ER_DIRECT && !radix;
     p.other = take(radix || buckets ? tokens * 8 : 0);
-    p.hist = take(radix ? (size_t)EX_BINS * EX_MAX_BLOCKS * 4 : buckets ? (EB_BUCKETS + 1) * 4 : 0);
+    p.hist = take(radix ? (size_t)EX_BINS * EX_MAX_BLOCKS * 4 : buckets ? (size_t)EB_STARTS * (ER_MAX_TOKENS / EB_LIST) * 4 : 0);
     p.totals = take(radix ? EX_BINS * 4 : 0);
     const bool small = tokens <= EW_SMALL;           // no row is cut
     p.info = take(small ? 0 : p.shares * 4);
@@ -849,17 +861,15 @@ static int em_sort(const fdgs_embedding_bwd_args* a, const EmPlan& p, char* ws, 
         return FDGS_OK;
     }
     if (tokens <= ER_MAX_TOKENS) {
-        const int shift = key_bits > 11 ? key_bits - 11 : 0;                           // 2048 buckets
-        static_assert(EB_BUCKETS == 1 << 11, "buckets of the upper 11 bits");
-        if (hipFuncSetAttribute((const void*)embedding_bucket_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, EB_LDS) != hipSuccess)
-            return FDGS_ELAUNCH;
-        uint2* other = (uint2*)(ws + p.other);
-        uint32_t* start = (uint32_t*)(ws + p.hist);
-        hipLaunchKernelGGL(embedding_bucket_kernel, dim3(1), dim3(EB_THREADS), EB_LDS, s, a->ids, tokens, wide, padding,
-                           (uint32_t)a->num_rows, shift, other, start);
+        const int shift = key_bits > 11 ? key_bits - 11 : 0, nlists = (tokens + EB_LIST - 1) / EB_LIST;
+        static_assert(EB_BUCKETS == 1 << 11 && EB_BUCKETS == 2 * EB_THREADS, "buckets of the upper 11 bits, two to a thread");
+        uint2* lists = (uint2*)(ws + p.other);
+        uint32_t* starts = (uint32_t*)(ws + p.hist);
+        hipLaunchKernelGGL(embedding_bucket_kernel, dim3(nlists), dim3(EB_THREADS), 0, s, a->ids, tokens, wide, padding,
+                           (uint32_t)a->num_rows, shift, lists, starts);
         FDGS_CHECK_LAUNCH();
-        hipLaunchKernelGGL(embedding_place_kernel, dim3((tokens + 63) / 64), dim3(ER_THREADS), 0, s, other, start, tokens, shift,
-                           (uint32_t)a->num_rows, (uint2*)(ws + p.sorted));
+        hipLaunchKernelGGL(embedding_place_kernel, dim3((tokens + 63) / 64), dim3(ER_THREADS), 0, s, lists, starts, tokens, nlists,
+                           shift, (uint32_t)a->num_rows, (uint2*)(ws + p.sorted));
         FDGS_CHECK_LAUNCH();
         return FDGS_OK;
     }
@@ -912,10 +922,15 @@ static int em_bwd_launch(const EmBwd& k, const EmPlan& p, hipStream_t s) {
     if (p.vec > 1) hipLaunchKernelGGL((embedding_walk_kernel<T, T::full, false>), grid, threads, 0, s, k);
     else hipLaunchKernelGGL((embedding_walk_kernel<T, 1, false>), grid, threads, 0, s, k);
     FDGS_CHECK_LAUNCH();
-    const int scan = p.groups > EC_SCAN ? p.groups : EC_SCAN;
-    const dim3 joins((unsigned)((p.shares + scan - 1) / scan), (unsigned)p.tiles);
-    if (p.vec > 1) hipLaunchKernelGGL((embedding_join_kernel<T, T::full>), joins, threads, 0, s, k);
-    else hipLaunchKernelGGL((embedding_join_kernel<T, 1>), joins, threads, 0, s, k);
+    // at most 64 lanes to a row here, so that there are groups to divide the partial sums of a long one
+    EmBwd j = k;
+    const int tiles = (p.nv + 63) / 64;
+    j.lanes = (p.nv + tiles - 1) / tiles;
+    j.groups = EW_THREADS / j.lanes;
+    const int scan = j.groups > EC_SCAN ? j.groups : EC_SCAN;
+    const dim3 joins((unsigned)((p.shares + scan - 1) / scan), (unsigned)tiles);
+    if (p.vec > 1) hipLaunchKernelGGL((embedding_join_kernel<T, T::full>), joins, threads, 0, s, j);
+    else hipLaunchKernelGGL((embedding_join_kernel<T, 1>), joins, threads, 0, s, j);
     FDGS_CHECK_LAUNCH();
     return FDGS_OK;
 }
@@ -925,9 +940,10 @@ extern "C" int fdgs_embedding_bwd(const fdgs_embedding_bwd_args* a, void* stream
     if (a->id_bytes != 4 && a->id_bytes != 8) return FDGS_EINVAL;
     if (a->num_rows == 0 || a->dim == 0) return FDGS_OK;
     if (!a->grad_table || (a->num_tokens > 0 && (!a->ids || !a->grad_out)) || a->grad_out_row_stride < 0) return FDGS_EINVAL;
-    if (a->dim > EM_MAX_DIM || a->num_tokens > FDGS_EMBEDDING_MAX_TOKENS) return FDGS_ETOOLARGE;
+    if (a->dim > FDGS_EMBEDDING_MAX_DIM || a->num_tokens > FDGS_EMBEDDING_MAX_TOKENS) return FDGS_ETOOLARGE;
     const EmPlan p = em_plan(a->num_tokens, a->num_rows, a->dim, a->type);
-    if (p.shares > 0x7fffffffLL || p.tiles > 65535) return FDGS_ETOOLARGE;
+    static_assert(FDGS_EMBEDDING_MAX_DIM / EmF32::full / 64 <= 65535, "column tiles in a grid's second dimension");
+    if (p.shares > 0x7fffffffLL) return FDGS_ETOOLARGE;
     if (!a->workspace || a->workspace_bytes < p.bytes) return FDGS_EWORKSPACE;
     hipStream_t s = (hipStream_t)stream;
     char* ws = (char*)a->workspace;

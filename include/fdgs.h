@@ -555,6 +555,7 @@ int fdgs_moment8_pack(const fdgs_moment8_args* a, void* stream);
  * A token has no row - zeros in out, nothing in the gradient - when its id is negative or padding_id; an id of num_rows
  * or more gives a row of NaN, and nothing in the gradient.                                            */
 #define FDGS_EMBEDDING_MAX_TOKENS (1 << 30)          /* of the gradient; the lookup takes 2^31 - 1 */
+#define FDGS_EMBEDDING_MAX_DIM (1 << 22)
 typedef struct {
     int64_t num_tokens;
     int32_t num_rows, dim;
