@@ -58,6 +58,9 @@ def prepare(viewpoint_camera, pc, deforms, bg_color: torch.Tensor, scaling_modif
     opacity = pc._opacity
     codebook = getattr(pc, "feature_codebook", None)
     codebook = codebook if isinstance(codebook, FeatureCodebook) else None
+    if codebook is not None and (codebook.ids.shape[0] != means3D.shape[0] or tuple(codebook.table.shape[1:]) != (16, 3)):
+        raise ValueError(f"the codebook has {codebook.ids.shape[0]} ids and rows of {tuple(codebook.table.shape[1:])}; "
+                         f"{means3D.shape[0]} Gaussians need an id each and rows of (16, 3)")
     # Without gradients, with this package's deformation field and a model that keeps the SH coefficients as the
     # reference's GaussianModel does, the two tensors go to the deformation kernel as they are: get_features is a
     # concatenation into a fresh [N,16,3] tensor on every call (gaussian_model.py:86-89)

@@ -70,3 +70,19 @@ def test_rows_of_strided_gradients():
                                    (base[:1, :1].expand(6, 5, 8), 2, 8, 0), (base[:, ::2, :4], 2, 4, None), (base[::2], 1, 40, 80),
                                    (base[:, 0], 1, 8, 40), (base.transpose(0, 1), 2, 8, None), (torch.zeros(()).expand(6, 5, 8), 2, 8, None)):
         assert rows_layout(t, lead) == (stride is not None, width, width if stride is None else stride), (t.shape, t.stride())
+
+
+@pytest.mark.parametrize("ids, row", [(3, (16, 3)), (5, (16, 3)), (4, (48,)), (4, (15, 3))])
+def test_render_refuses_a_codebook_that_does_not_fit(ids, row):
+    """An id for each Gaussian and rows of 16 x 3, or the kernels behind would read past the looked-up rows."""
+    from types import SimpleNamespace
+    from fdgs.embedding import FeatureCodebook
+    from fdgs.renderer import render
+    eye = torch.eye(4)
+    cam = SimpleNamespace(FoVx=1.0, FoVy=1.0, image_height=8, image_width=8, world_view_transform=eye, full_proj_transform=eye,
+                          camera_center=torch.zeros(3), time=0.0)
+    xyz = torch.zeros(4, 3)
+    pc = SimpleNamespace(get_xyz=xyz, _xyz=xyz, _opacity=torch.zeros(4, 1), active_sh_degree=3, max_sh_degree=3,
+                         feature_codebook=FeatureCodebook(torch.zeros(7, *row), torch.zeros(ids, dtype=torch.int32)))
+    with pytest.raises(ValueError, match="an id each"):
+        render(cam, pc, None, torch.zeros(3), stage="coarse")
