@@ -18,7 +18,13 @@
 
 namespace {
 
-struct Refused { PyObject* type; std::string what; };
+// (A standard exception, so that one that leaves a backward pass is autograd's to report.)
+struct Refused : std::exception {
+    PyObject* type;
+    std::string text;
+    Refused(PyObject* t, std::string s) : type(t), text(std::move(s)) {}
+    const char* what() const noexcept override { return text.c_str(); }
+};
 [[noreturn]] void value_error(const std::string& s) { throw Refused{PyExc_ValueError, s}; }
 struct Raised {};                                    // a Python exception is set
 
@@ -68,6 +74,17 @@ struct Each {
         const unsigned long v = PyLong_AsUnsignedLongMask(n.p);
         if (v == (unsigned long)-1 && PyErr_Occurred()) throw Raised();
         return (uint32_t)v;
+    }
+};
+
+// The memory that a call writes: two pieces that overlap would be written by workgroups that do not wait for each other.
+struct Written {
+    std::vector<std::pair<uintptr_t, size_t>> pieces;
+    void add(const void* p, size_t bytes) { if (bytes) pieces.emplace_back((uintptr_t)p, bytes); }
+    void check() {
+        std::sort(pieces.begin(), pieces.end());
+        for (size_t i = 1; i < pieces.size(); ++i)
+            if (pieces[i - 1].first + pieces[i - 1].second > pieces[i].first) value_error("a tensor is in the lists twice, or two of them overlap");
     }
 };
 
@@ -159,8 +176,8 @@ PyObject* adamw_step(PyObject* a) {
         value_error("8-bit moments need keys: a number for each tensor, others at every step");
     std::vector<Tensor> hold;                        // copies of gradients, kept until the kernels are on the stream
     std::vector<fdgs_adamw_tensor> out(n);
-    std::vector<uintptr_t> written;
-    written.reserve(3 * n);
+    Written written;
+    written.pieces.reserve((eight ? 5 : 3) * n + (bf16 ? n : 0));
     for (Py_ssize_t i = 0; i < n; ++i) {
         const at::Tensor &pt = tensor(p.at(i), "params"), &gt = tensor(g.at(i), "grads");
         const int64_t numel = pt.numel();
@@ -219,15 +236,18 @@ PyObject* adamw_step(PyObject* a) {
         r.step = (int32_t)step;
         r.lr = lr.number(i);
         r.weight_decay = wd.number(i);
-        if (numel) {
-            written.push_back((uintptr_t)r.param);
-            written.push_back((uintptr_t)r.exp_avg);
-            written.push_back((uintptr_t)r.exp_avg_sq);
+        written.add(r.param, numel * (bf16 ? 2 : 4));
+        written.add(r.exp_avg, numel * (eight ? 1 : 4));
+        written.add(r.exp_avg_sq, numel * (eight ? 1 : 4));
+        if (bf16) written.add(r.residual, numel * 2);
+        if (eight) {
+            const int64_t blocks = (numel + FDGS_MOMENT8_BLOCK - 1) / FDGS_MOMENT8_BLOCK;
+            written.add(r.exp_avg_exponents, blocks);
+            written.add(r.exp_avg_sq_exponents, blocks);
         }
         out[i] = r;
     }
-    std::sort(written.begin(), written.end());
-    if (std::adjacent_find(written.begin(), written.end()) != written.end()) value_error("a tensor is in the lists twice");
+    written.check();
     fdgs_adamw_args args;
     memset(&args, 0, sizeof(args));
     args.num_tensors = (int32_t)n;
@@ -263,6 +283,8 @@ PyObject* moment8_convert(PyObject* a) {
     if (type != at::kFloat && type != at::kBFloat16) value_error("the values of 8-bit moments are float32 or bfloat16");
     on_gpu(first);
     std::vector<fdgs_moment8_tensor> out(n);
+    Written written;
+    written.pieces.reserve((pack ? 2 : 1) * n);
     for (Py_ssize_t i = 0; i < n; ++i) {
         const at::Tensor& t = tensor(v.at(i), "values");
         if (t.scalar_type() != type || t.device() != first.device() || !t.is_contiguous())
@@ -276,8 +298,15 @@ PyObject* moment8_convert(PyObject* a) {
         r.numel = t.numel();
         r.is_signed = x.is_signed;
         r.round_key = ko == Py_None ? 0u : keys.low32(i);
+        if (pack) {
+            written.add(r.codes, r.numel);
+            written.add(r.exponents, (r.numel + FDGS_MOMENT8_BLOCK - 1) / FDGS_MOMENT8_BLOCK);
+        } else {
+            written.add(r.value, r.numel * t.element_size());
+        }
         out[i] = r;
     }
+    written.check();
     fdgs_moment8_args args;
     memset(&args, 0, sizeof(args));
     args.num_tensors = (int32_t)n;
@@ -541,7 +570,7 @@ PyObject* guarded(PyObject*, PyObject* args) {
         return F(args);
     } catch (const Raised&) {
     } catch (const Refused& r) {
-        PyErr_SetString(r.type, r.what.c_str());
+        PyErr_SetString(r.type, r.what());
     } catch (const std::bad_alloc&) {
         PyErr_NoMemory();
     } catch (const c10::Error& e) {

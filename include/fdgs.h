@@ -551,7 +551,7 @@ int fdgs_moment8_pack(const fdgs_moment8_args* a, void* stream);
  *   out[i, :] = scale * table[ids[i], :]            for the tokens i
  *   grad_table[r, :] = scale * sum_{i : ids[i] = r} grad_out[i, :]   for every row r; rows no token asks for get zeros
  * in float32, rounded once to `type` (FDGS_TYPE_F32 / BF16 / F16: table, out and both gradients).  The sums are taken
- * in an order that the ids alone decide (no atomics): equal inputs give equal bits.
+ * in an order that the ids alone decide: equal inputs give equal bits.
  * A token has no row - zeros in out, nothing in the gradient - when its id is negative or padding_id; an id of num_rows
  * or more gives a row of NaN, and nothing in the gradient.                                            */
 #define FDGS_EMBEDDING_MAX_TOKENS (1 << 30)          /* of the gradient; the lookup takes 2^31 - 1 */

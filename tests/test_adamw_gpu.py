@@ -370,3 +370,81 @@ def test_more_tensors_than_one_launch_takes(count):
     packed = adamw.pack8(ms, True)                               # and their conversions, there and back
     for m, x in zip(ms, adamw.unpack8(packed)):
         assert np.array_equal(x.cpu().numpy(), ac.decode(*ac.encode(m.cpu().numpy(), 0x8000, True), True))
+
+
+def _small(bits, bf16, n=3):
+    """Arguments of a step over n tensors that holds good."""
+    from fdgs.adamw import Moment8
+    kind = torch.bfloat16 if bf16 else torch.float32
+    p, g = ([torch.ones(300 + i, dtype=kind, device="cuda") for i in range(n)] for _ in range(2))
+    m, v = ([Moment8.zeros_like(x, signed) if bits == 8 else torch.zeros(x.shape, device="cuda") for x in p] for signed in (True, False))
+    low = [torch.zeros(x.shape, dtype=torch.int16, device="cuda") for x in p]
+    return dict(params=p, grads=g, exp_avgs=m, exp_avg_sqs=v, steps=1, lr=0.1, residuals=low if bf16 else None,
+                keys=list(range(n)) if bits == 8 else None)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("bf16", [False, True])
+def test_step_refuses_and_changes_nothing(bits, bf16):
+    from fdgs.adamw import Moment8, adamw_step
+    dev, other = "cuda", torch.float32 if bf16 else torch.bfloat16
+    kind = torch.bfloat16 if bf16 else torch.float32
+    z = lambda n, t=kind: torch.zeros(n, dtype=t, device=dev)  # noqa: E731
+    both = z(2 * 302 - 1)                                # two tensors that share an element
+    cases = [("same length", dict(grads=lambda a: a[:2])), ("same length", dict(exp_avgs=lambda a: a + a[:1])),
+             ("one type", dict(params=lambda a: [*a[:2], z(302, other)])), ("one type", dict(grads=lambda a: [*a[:2], z(302, other)])),
+             ("contiguous", dict(params=lambda a: [*a[:2], z((302, 2))[:, 0]])), ("its size", dict(grads=lambda a: [*a[:2], z(301)])),
+             ("one device", dict(grads=lambda a: [*a[:2], torch.zeros(302, dtype=kind)])),
+             ("count from 1", dict(steps=lambda a: 0)), ("count from 1", dict(steps=lambda a: [1, 1, -3])),
+             ("one value", dict(lr=lambda a: [0.1, 0.1])), ("one value", dict(steps=lambda a: [1])),
+             ("twice", dict(params=lambda a: [a[0], a[1], a[0][:300]], grads=lambda a: [a[0], a[1], a[0]],
+                            exp_avgs=lambda a: [a[0], a[1], a[0]], exp_avg_sqs=lambda a: [a[0], a[1], a[0]],
+                            **({"residuals": lambda a: [a[0], a[1], a[0]]} if bf16 else {}))),
+             ("overlap", dict(params=lambda a: [a[0], both[:301], both[300:602]]))]
+    if bf16:
+        cases += [("residual", dict(residuals=lambda a: None)), ("residual", dict(residuals=lambda a: a[:2])),
+                  ("residual", dict(residuals=lambda a: [*a[:2], z(302, torch.int32)])),
+                  ("overlap", dict(residuals=lambda a: [a[0], a[2][:301], a[2]]))]
+    if bits == 8:
+        cases += [("keys", dict(keys=lambda a: None)), ("keys", dict(keys=lambda a: a[:2])), ("do not mix", dict(exp_avgs=lambda a: [*a[:2], z(302, torch.float32)])),
+                  ("the second is not", dict(exp_avgs=lambda a: [x._replace(signed=False) for x in a])),
+                  ("one exponent per", dict(exp_avg_sqs=lambda a: [*a[:2], a[2]._replace(exponents=z(1, torch.uint8))])),
+                  ("uint8", dict(exp_avg_sqs=lambda a: [*a[:2], a[2]._replace(codes=z(302, torch.int8))])),
+                  ("overlap", dict(exp_avgs=lambda a: [x._replace(exponents=a[0].exponents) for x in a]))]
+    else:
+        cases += [("float32 tensors", dict(exp_avgs=lambda a: [*a[:2], z(302, torch.float16)])),
+                  ("Moment8", dict(exp_avgs=lambda a: [*a[:2], Moment8.zeros_like(a[2], True)])),
+                  ("overlap", dict(exp_avg_sqs=lambda a: [a[0], a[2][:301], a[2]]))]
+    for match, change in cases:
+        args = _small(bits, bf16)
+        args.update({k: f(args[k]) for k, f in change.items()})
+        before = [x.clone() for x in args["params"]]
+        with pytest.raises((ValueError, TypeError), match=match):
+            adamw_step(**args)
+        assert all(torch.equal(x, y) for x, y in zip(before, args["params"])), match
+    with pytest.raises(ValueError, match="not torch"):
+        adamw_step([z(4, torch.float64)], [z(4, torch.float64)], [z(4)], [z(4)], steps=1, lr=0.1)
+    args = _small(bits, bf16)
+    adamw_step(**args)                                   # as they stand they are a step
+    assert all((x != 1).all() for x in args["params"])
+
+
+def test_conversions_refuse_overlapping_results():
+    from fdgs.adamw import Moment8, pack8, unpack8
+    ms = pack8([torch.ones(300, device="cuda"), torch.ones(300, device="cuda")], False)
+    out = torch.zeros(599, device="cuda")
+    with pytest.raises(ValueError, match="overlap"):
+        unpack8(ms, out=[out[:300], out[299:]])
+    with pytest.raises(ValueError, match="one type"):
+        unpack8(ms, out=[out[:300], torch.zeros(300, dtype=torch.bfloat16, device="cuda")])
+    with pytest.raises(ValueError, match="for each"):
+        unpack8(ms, out=[out[:300]])
+    with pytest.raises(ValueError, match="one code per"):
+        unpack8(ms, out=[out[:300], out[300:]])
+    assert (out == 0).all()
+    assert unpack8([]) == [] and pack8([], True) == []
+    with pytest.raises(ValueError, match="float32"):
+        pack8([torch.ones(4, device="cuda", dtype=torch.bfloat16)], True)
+    with pytest.raises(ValueError, match="one value"):
+        pack8([torch.ones(4, device="cuda")], True, keys=[1, 2])
+    assert isinstance(ms[0], Moment8)
