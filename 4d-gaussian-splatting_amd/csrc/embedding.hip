@@ -92,19 +92,18 @@ struct EmFwd {
 // Bound by the output's lines and, where the table does not fit an XCD's 4 MB of L2, by the rows that come from behind it:
 // 300,000 x 48 floats 14 us (4.4 TB/s), 2,000,000 x 48 from 65,536 rows 120 us, from 8,192 rows 66 us (5.8 TB/s).
 template <class T, int VEC>
-__global__ void __launch_bounds__(EF_THREADS)
-embedding_fwd_kernel(EmFwd a) {
+__device__ __forceinline__ void ef_group(const EmFwd& a, int group, int tile, uint32_t thread) {
     typedef EmVec<T, VEC> Vec;
     typedef typename T::raw raw;
-    const int tok0 = blockIdx.x * a.per_group, have = min(a.per_group, a.tokens - tok0);
-    const int c0 = blockIdx.y * EF_VECTORS, cols = min(a.nv - c0, EF_VECTORS);   // all of them, or a part of one row
+    const int tok0 = group * a.per_group, have = min(a.per_group, a.tokens - tok0);
+    const int c0 = tile * EF_VECTORS, cols = min(a.nv - c0, EF_VECTORS);   // all of them, or a part of one row
     const uint32_t end = (uint32_t)have * (uint32_t)cols;
     Vec v[EF_UNROLL];
     int tok[EF_UNROLL], col[EF_UNROLL];
     long long id[EF_UNROLL];
 #pragma unroll
     for (int u = 0; u < EF_UNROLL; ++u) {
-        const uint32_t e = u * EF_THREADS + threadIdx.x;
+        const uint32_t e = u * EF_THREADS + thread;
         const uint32_t t = a.per_group > 1 ? em_div(e, a.by_nv) : 0u;
         tok[u] = e < end ? tok0 + (int)t : -1;
         col[u] = em_col<VEC>(c0 + (int)(e - t * (uint32_t)a.nv), a.nv, a.dim);
@@ -129,73 +128,92 @@ embedding_fwd_kernel(EmFwd a) {
     }
 }
 
+template <class T, int VEC>
+__global__ void __launch_bounds__(EF_THREADS)
+embedding_fwd_kernel(EmFwd a) { ef_group<T, VEC>(a, blockIdx.x, blockIdx.y, threadIdx.x); }
+
 template <class T>
-static int em_fwd_launch(const EmFwd& k0, hipStream_t s) {
-    EmFwd k = k0;
-    const int vec = k.dim >= T::full ? T::full : 1;
-    k.nv = (k.dim + vec - 1) / vec;
-    k.by_nv = em_div_of((uint32_t)k.nv);
-    k.per_group = k.nv < EF_VECTORS ? EF_VECTORS / k.nv : 1;
-    const int tiles = (k.nv + EF_VECTORS - 1) / EF_VECTORS;
-    const dim3 grid((unsigned)(((long long)k.tokens + k.per_group - 1) / k.per_group), (unsigned)tiles), threads(EF_THREADS);
-    if (vec > 1) hipLaunchKernelGGL((embedding_fwd_kernel<T, T::full>), grid, threads, 0, s, k);
-    else hipLaunchKernelGGL((embedding_fwd_kernel<T, 1>), grid, threads, 0, s, k);
+static int em_fwd_launch(const EmFwd& k, int vec, dim3 grid, hipStream_t s) {
+    if (vec > 1) hipLaunchKernelGGL((embedding_fwd_kernel<T, T::full>), grid, dim3(EF_THREADS), 0, s, k);
+    else hipLaunchKernelGGL((embedding_fwd_kernel<T, 1>), grid, dim3(EF_THREADS), 0, s, k);
     FDGS_CHECK_LAUNCH();
     return FDGS_OK;
 }
 
+static int em_full(int type) { return type == FDGS_TYPE_F32 ? EmF32::full : EmBf16::full; }
 static bool em_type_ok(int t) { return t == FDGS_TYPE_F32 || t == FDGS_TYPE_BF16 || t == FDGS_TYPE_F16; }
 
-extern "C" int fdgs_embedding_fwd(const fdgs_embedding_fwd_args* a, void* stream) {
-    if (!a || a->num_tokens < 0 || a->num_rows < 0 || a->dim < 0 || !em_type_ok(a->type)) return FDGS_EINVAL;
-    if (a->id_bytes != 4 && a->id_bytes != 8) return FDGS_EINVAL;
-    if (a->num_tokens == 0 || a->dim == 0) return FDGS_OK;
-    if (!a->ids || !a->out || (a->num_rows > 0 && !a->table)) return FDGS_EINVAL;
-    if (a->num_rows > 0 && a->table_row_stride < 0) return FDGS_EINVAL;
-    if (a->dim > FDGS_EMBEDDING_MAX_DIM || a->num_tokens > 0x7fffffffLL) return FDGS_ETOOLARGE;
-    EmFwd k = {};
-    k.ids = a->ids; k.table = a->table; k.out = a->out;
-    k.tokens = (int)a->num_tokens; k.table_stride = a->table_row_stride;
-    k.padding = a->padding_id >= 0 ? a->padding_id : -1;
-    k.rows = a->num_rows; k.dim = a->dim; k.wide = a->id_bytes == 8; k.scale = a->scale;
-    hipStream_t s = (hipStream_t)stream;
-    if (a->type == FDGS_TYPE_F32) return em_fwd_launch<EmF32>(k, s);
-    if (a->type == FDGS_TYPE_BF16) return em_fwd_launch<EmBf16>(k, s);
-    return em_fwd_launch<EmF16>(k, s);
+// ---- the tokens by row: (key, token) pairs, stable ----
+// The sort's launches wait more than they work: their workgroups leave most of the chip idle.  Where a lookup sorts its
+// tokens for the gradient that will follow, the launches have parts of the lookup's work beside their own (16,384 tokens of 2048
+// bfloat16 numbers: 30 us, 40 one after the other).
+struct EmPart {
+    EmFwd a;
+    int first, last, type, vec;                      // workgroups' work (tokens and column tile) [first, last)
+    EmDiv by_tiles;
+};
+__device__ __forceinline__ void ep_group(const EmPart& f, int block, int threads) {
+    const int each = threads / EF_THREADS;
+    const int g = f.first + block * each + (each > 1 ? (int)(threadIdx.x / EF_THREADS) : 0);
+    if (g >= f.last) return;
+    const int group = (int)em_div((uint32_t)g, f.by_tiles), tile = g - group * (int)f.by_tiles.d;
+    const uint32_t thread = threadIdx.x % EF_THREADS;
+    if (f.type == FDGS_TYPE_F32) {
+        if (f.vec > 1) ef_group<EmF32, EmF32::full>(f.a, group, tile, thread);
+        else ef_group<EmF32, 1>(f.a, group, tile, thread);
+    } else if (f.type == FDGS_TYPE_BF16) {
+        if (f.vec > 1) ef_group<EmBf16, EmBf16::full>(f.a, group, tile, thread);
+        else ef_group<EmBf16, 1>(f.a, group, tile, thread);
+    } else {
+        if (f.vec > 1) ef_group<EmF16, EmF16::full>(f.a, group, tile, thread);
+        else ef_group<EmF16, 1>(f.a, group, tile, thread);
+    }
+}
+// One step of a sort in `blocks` workgroups, every `period`-th from the first on (an odd number: the workgroups go to the 8
+// XCDs in turn), and a part of a lookup in the others.
+template <class Step>
+__global__ void __launch_bounds__(Step::threads)
+embedding_step_kernel(Step step, int blocks, int period, EmPart part) {
+    const int b = (int)blockIdx.x, round = b / period;
+    if (round < blocks && round * period == b) step.run(round);
+    else ep_group(part, round < blocks ? b - round - 1 : b - blocks, Step::threads);
 }
 
-// ---- the tokens by row: (key, token) pairs, stable ----
-// Few tokens: a token's place is the number of tokens that come before it, counted against all of them; the workgroup has
-// 64 tokens, its waves divide the others.  T^2 / 64 comparisons of a wave spread over the chip, one launch.
 #define ER_THREADS 256
-#define ER_CHUNK 4096                                // keys staged in LDS at a time
 #define ER_DIRECT 4096                               // up to here in one launch; beyond, by buckets:
 #define ER_MAX_TOKENS 16384                          // beyond, T^2 comparisons of equal ids would take long
 
-__global__ void __launch_bounds__(ER_THREADS)
-embedding_rank_kernel(const void* __restrict__ ids, int tokens, int wide, long long padding, uint32_t rows,
-                      uint2* __restrict__ sorted) {
-    __shared__ __align__(16) uint32_t sk[ER_CHUNK];
-    __shared__ uint32_t part[4][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int own = blockIdx.x * 64;                 // first token of the workgroup
-    const int me = own + lane;
-    const uint32_t key = me < tokens ? em_key(ids, me, wide, padding, rows) : 0xFFFFFFFFu;
-    uint32_t before = 0;
-    for (int c0 = 0; c0 < tokens; c0 += ER_CHUNK) {
-        __syncthreads();
-        for (int j = threadIdx.x; j < ER_CHUNK; j += ER_THREADS)
-            sk[j] = c0 + j < tokens ? em_key(ids, c0 + j, wide, padding, rows) : 0xFFFFFFFFu;   // after every key
+struct EmIds {
+    const void* ids;
+    long long padding;
+    uint32_t rows;
+    int tokens, wide;
+    __device__ __forceinline__ uint32_t key(int i) const { return em_key(ids, i, wide, padding, rows); }
+};
+
+struct EmRank {
+    static const int threads = ER_THREADS;
+    EmIds in;
+    uint2* sorted;
+    __device__ __forceinline__ void run(int block) const {
+        __shared__ __align__(16) uint32_t sk[ER_DIRECT];
+        __shared__ uint32_t part[4][64];
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, tokens = in.tokens;
+        const int own = block * 64;             // first token of the workgroup
+        const int me = own + lane;
+        const uint32_t key = me < tokens ? in.key(me) : 0xFFFFFFFFu;
+        uint32_t before = 0;
+        for (int j = threadIdx.x; j < (tokens + 63) / 64 * 64; j += ER_THREADS) sk[j] = j < tokens ? in.key(j) : 0xFFFFFFFFu;   // after every key
         __syncthreads();
         // blocks of 64 keys, one wave each: those before the own tokens win ties, those behind lose them
-        for (int b = wave * 64; b < ER_CHUNK && c0 + b < tokens; b += 256) {
-            if (c0 + b == own) {
+        for (int b = wave * 64; b < tokens; b += 256) {
+            if (b == own) {
                 for (int j = 0; j < 64; ++j) {
                     const uint32_t o = sk[b + j];
                     before += (o < key || (o == key && j < lane)) ? 1u : 0u;
                 }
             } else {
-                const uint32_t limit = key + (c0 + b < own ? 1u : 0u);       // o <= key, or o < key
+                const uint32_t limit = key + (b < own ? 1u : 0u);            // o <= key, or o < key
                 const uint4* q = (const uint4*)(sk + b);
 #pragma unroll
                 for (int j = 0; j < 16; ++j) {
@@ -204,14 +222,14 @@ embedding_rank_kernel(const void* __restrict__ ids, int tokens, int wide, long l
                 }
             }
         }
+        part[wave][lane] = before;
+        __syncthreads();
+        if (wave == 0 && me < tokens) {
+            const uint32_t r = part[0][lane] + part[1][lane] + part[2][lane] + part[3][lane];
+            sorted[r] = make_uint2(key, (uint32_t)me);
+        }
     }
-    part[wave][lane] = before;
-    __syncthreads();
-    if (wave == 0 && me < tokens) {
-        const uint32_t r = part[0][lane] + part[1][lane] + part[2][lane] + part[3][lane];
-        sorted[r] = make_uint2(key, (uint32_t)me);
-    }
-}
+};
 
 // More: every workgroup puts 4096 tokens into 2048 buckets by the upper bits of their keys, in LDS and in no particular
 // order, which makes a list of each 4096; then a token's place is counted among the tokens of its bucket alone (and of those
@@ -224,111 +242,123 @@ embedding_rank_kernel(const void* __restrict__ ids, int tokens, int wide, long l
 #define EB_BUCKETS 2048
 #define EB_STARTS (EB_BUCKETS + 1)                   // where a list's buckets start, and where its last one ends
 
-__global__ void __launch_bounds__(EB_THREADS)
-embedding_bucket_kernel(const void* __restrict__ ids, int tokens, int wide, long long padding, uint32_t rows, int shift,
-                        uint2* __restrict__ lists, uint32_t* __restrict__ starts) {
-    __shared__ uint2 ordered[EB_LIST];
-    __shared__ uint32_t count[EB_BUCKETS], wsum[EB_THREADS / 64], without;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int from = blockIdx.x * EB_LIST, have = min(tokens - from, EB_LIST);
-    uint32_t* start = starts + blockIdx.x * EB_STARTS;
-    count[threadIdx.x] = 0;
-    count[threadIdx.x + EB_THREADS] = 0;
-    uint32_t key[EB_PER], slot[EB_PER];
+struct EmBucket {
+    static const int threads = EB_THREADS;
+    EmIds in;
+    int shift;
+    uint2* __restrict__ lists;
+    uint32_t* __restrict__ starts;
+    __device__ __forceinline__ void run(int block) const {
+        __shared__ uint2 ordered[EB_LIST];
+        __shared__ uint32_t count[EB_BUCKETS], wsum[EB_THREADS / 64], without;
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        const int from = block * EB_LIST, have = min(in.tokens - from, EB_LIST);
+        const uint32_t rows = in.rows;
+        uint32_t* start = starts + block * EB_STARTS;
+        count[threadIdx.x] = 0;
+        count[threadIdx.x + EB_THREADS] = 0;
+        uint32_t key[EB_PER], slot[EB_PER];
 #pragma unroll
-    for (int k = 0; k < EB_PER; ++k) {
-        const int i = threadIdx.x + k * EB_THREADS;
-        key[k] = i < have ? em_key(ids, from + i, wide, padding, rows) : 0xFFFFFFFFu;
+        for (int k = 0; k < EB_PER; ++k) {
+            const int i = threadIdx.x + k * EB_THREADS;
+            key[k] = i < have ? in.key(from + i) : 0xFFFFFFFFu;
+        }
+        if (threadIdx.x == 0) without = 0;
+        __syncthreads();
+        // tokens without a row are not put in order: they go to the end, a wave's together (one count of all of them would
+        // take an LDS atomic each to the same word)
+#pragma unroll
+        for (int k = 0; k < EB_PER; ++k) {
+            const unsigned long long none = __ballot(key[k] == rows);
+            uint32_t b = 0;
+            if (none && lane == 0) b = atomicAdd(&without, (uint32_t)__popcll(none));
+            b = (uint32_t)__builtin_amdgcn_readfirstlane((int)b);
+            slot[k] = key[k] == rows ? b + (uint32_t)__popcll(none & ((1ull << lane) - 1ull))
+                      : key[k] < rows ? atomicAdd(&count[key[k] >> shift], 1u) : 0u;
+        }
+        __syncthreads();
+        const uint32_t c0 = count[2 * threadIdx.x], c1 = count[2 * threadIdx.x + 1];
+        uint32_t incl = c0 + c1;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const uint32_t o = __shfl_up(incl, d);
+            if (lane >= d) incl += o;
+        }
+        if (lane == 63) wsum[wave] = incl;
+        __syncthreads();
+        uint32_t base = 0;
+#pragma unroll
+        for (int w = 0; w < EB_THREADS / 64; ++w)
+            if (w < wave) base += wsum[w];
+        const uint32_t first = base + incl - c0 - c1, valid = (uint32_t)have - without;
+        count[2 * threadIdx.x] = first;
+        count[2 * threadIdx.x + 1] = first + c0;
+        start[2 * threadIdx.x] = first;
+        start[2 * threadIdx.x + 1] = first + c0;
+        if (threadIdx.x == 0) start[EB_BUCKETS] = valid;
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < EB_PER; ++k) {
+            const int i = threadIdx.x + k * EB_THREADS;
+            if (i < have) ordered[slot[k] + (key[k] == rows ? valid : count[key[k] >> shift])] = make_uint2(key[k], (uint32_t)(from + i));
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < have; i += EB_THREADS) lists[from + i] = ordered[i];
     }
-    if (threadIdx.x == 0) without = 0;
-    __syncthreads();
-    // tokens without a row are not put in order: they go to the end, a wave's together (one count of all of them would
-    // take an LDS atomic each to the same word)
-#pragma unroll
-    for (int k = 0; k < EB_PER; ++k) {
-        const unsigned long long none = __ballot(key[k] == rows);
-        uint32_t b = 0;
-        if (none && lane == 0) b = atomicAdd(&without, (uint32_t)__popcll(none));
-        b = (uint32_t)__builtin_amdgcn_readfirstlane((int)b);
-        slot[k] = key[k] == rows ? b + (uint32_t)__popcll(none & ((1ull << lane) - 1ull))
-                  : key[k] < rows ? atomicAdd(&count[key[k] >> shift], 1u) : 0u;
-    }
-    __syncthreads();
-    const uint32_t c0 = count[2 * threadIdx.x], c1 = count[2 * threadIdx.x + 1];
-    uint32_t incl = c0 + c1;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint32_t o = __shfl_up(incl, d);
-        if (lane >= d) incl += o;
-    }
-    if (lane == 63) wsum[wave] = incl;
-    __syncthreads();
-    uint32_t base = 0;
-#pragma unroll
-    for (int w = 0; w < EB_THREADS / 64; ++w)
-        if (w < wave) base += wsum[w];
-    const uint32_t first = base + incl - c0 - c1, valid = (uint32_t)have - without;
-    count[2 * threadIdx.x] = first;
-    count[2 * threadIdx.x + 1] = first + c0;
-    start[2 * threadIdx.x] = first;
-    start[2 * threadIdx.x + 1] = first + c0;
-    if (threadIdx.x == 0) start[EB_BUCKETS] = valid;
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < EB_PER; ++k) {
-        const int i = threadIdx.x + k * EB_THREADS;
-        if (i < have) ordered[slot[k] + (key[k] == rows ? valid : count[key[k] >> shift])] = make_uint2(key[k], (uint32_t)(from + i));
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < have; i += EB_THREADS) lists[from + i] = ordered[i];
-}
+};
 
-__global__ void __launch_bounds__(ER_THREADS)
-embedding_place_kernel(const uint2* __restrict__ lists, const uint32_t* __restrict__ starts, int tokens, int nlists, int shift,
-                       uint32_t rows, uint2* __restrict__ sorted) {
-    __shared__ uint32_t part[4][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int own = blockIdx.x * 64, me = min(own + lane, tokens - 1);   // 64 places of one list
-    const uint2 mine2 = lists[me];
-    const uint32_t key = mine2.x;
-    const unsigned long long mine = ((unsigned long long)key << 32) | mine2.y;
-    // the buckets that the 64 places touch, the first one's and the last one's
-    const uint32_t kf = (uint32_t)__builtin_amdgcn_readfirstlane((int)key), kl = (uint32_t)__builtin_amdgcn_readlane((int)key, 63);
-    const int bf = kf == rows ? EB_BUCKETS : (int)(kf >> shift), bl = kl == rows ? EB_BUCKETS : (int)(kl >> shift) + 1;
-    uint32_t before = 0;
-    if (kf != rows) {
-        for (int l = wave; l < nlists; l += 4) {
-            const uint2* __restrict__ list = lists + (size_t)l * EB_LIST;
-            const int lo = (int)starts[l * EB_STARTS + bf], hi = (int)starts[l * EB_STARTS + bl];
-            before += (uint32_t)lo;                  // all of the list's smaller buckets
-            // the buckets themselves, 64 tokens at a time: a lane loads one, all lanes compare with each
-            for (int b = lo; b < hi; b += 64) {
-                const uint2 other = b + lane < hi ? list[b + lane] : make_uint2(0xFFFFFFFFu, 0xFFFFFFFFu);
+struct EmPlace {
+    static const int threads = ER_THREADS;
+    const uint2* __restrict__ lists;
+    const uint32_t* __restrict__ starts;
+    int tokens, nlists, shift;
+    uint32_t rows;
+    uint2* __restrict__ sorted;
+    __device__ __forceinline__ void run(int block) const {
+        __shared__ uint32_t part[4][64];
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        const int own = block * 64, me = min(own + lane, tokens - 1);   // 64 places of one list
+        const uint2 mine2 = lists[me];
+        const uint32_t key = mine2.x;
+        const unsigned long long mine = ((unsigned long long)key << 32) | mine2.y;
+        // the buckets that the 64 places touch, the first one's and the last one's
+        const uint32_t kf = (uint32_t)__builtin_amdgcn_readfirstlane((int)key), kl = (uint32_t)__builtin_amdgcn_readlane((int)key, 63);
+        const int bf = kf == rows ? EB_BUCKETS : (int)(kf >> shift), bl = kl == rows ? EB_BUCKETS : (int)(kl >> shift) + 1;
+        uint32_t before = 0;
+        if (kf != rows) {
+            for (int l = wave; l < nlists; l += 4) {
+                const uint2* __restrict__ list = lists + (size_t)l * EB_LIST;
+                const int lo = (int)starts[l * EB_STARTS + bf], hi = (int)starts[l * EB_STARTS + bl];
+                before += (uint32_t)lo;                  // all of the list's smaller buckets
+                // the buckets themselves, 64 tokens at a time: a lane loads one, all lanes compare with each
+                for (int b = lo; b < hi; b += 64) {
+                    const uint2 other = b + lane < hi ? list[b + lane] : make_uint2(0xFFFFFFFFu, 0xFFFFFFFFu);
 #pragma unroll 16
-                for (int q = 0; q < 64; ++q) {
-                    const uint32_t kq = (uint32_t)__builtin_amdgcn_readlane((int)other.x, q), tq = (uint32_t)__builtin_amdgcn_readlane((int)other.y, q);
-                    before += (((unsigned long long)kq << 32) | tq) < mine ? 1u : 0u;
+                    for (int q = 0; q < 64; ++q) {
+                        const uint32_t kq = (uint32_t)__builtin_amdgcn_readlane((int)other.x, q), tq = (uint32_t)__builtin_amdgcn_readlane((int)other.y, q);
+                        before += (((unsigned long long)kq << 32) | tq) < mine ? 1u : 0u;
+                    }
                 }
             }
         }
-    }
-    part[wave][lane] = before;
-    __syncthreads();
-    if (wave == 0 && own + lane < tokens) {
-        uint32_t r = part[0][lane] + part[1][lane] + part[2][lane] + part[3][lane];
-        if (key == rows) {                           // behind all that have a row: list by list, as they lie
-            const int at = own / EB_LIST;
-            r = 0;
-            for (int l = 0; l < nlists; ++l) {
-                const uint32_t valid = starts[l * EB_STARTS + EB_BUCKETS];
-                r += valid;
-                if (l < at) r += (uint32_t)EB_LIST - valid;
-                if (l == at) r += (uint32_t)(me - at * EB_LIST) - valid;
+        part[wave][lane] = before;
+        __syncthreads();
+        if (wave == 0 && own + lane < tokens) {
+            uint32_t r = part[0][lane] + part[1][lane] + part[2][lane] + part[3][lane];
+            if (key == rows) {                           // behind all that have a row: list by list, as they lie
+                const int at = own / EB_LIST;
+                r = 0;
+                for (int l = 0; l < nlists; ++l) {
+                    const uint32_t valid = starts[l * EB_STARTS + EB_BUCKETS];
+                    r += valid;
+                    if (l < at) r += (uint32_t)EB_LIST - valid;
+                    if (l == at) r += (uint32_t)(me - at * EB_LIST) - valid;
+                }
             }
+            sorted[r] = mine2;
         }
-        sorted[r] = mine2;
     }
-}
+};
 
 // Many tokens: a radix sort by digits of at most 9 bits (two passes for tables of up to 262,143 rows), three launches a
 // pass: counts of each workgroup, their scan, scatter.  2,000,000 tokens of 65,536 rows 57 us, 300,000 of 8,192 29 us.
@@ -339,32 +369,32 @@ embedding_place_kernel(const uint2* __restrict__ lists, const uint32_t* __restri
 #define EX_MAX_BLOCKS 1024
 
 struct EmSort {
-    const void* ids;                                 // first pass: the tokens' ids; later passes: the pairs `in`
+    EmIds ids;                                       // first pass: the tokens' ids; later passes: the pairs `in`
     const uint2* in;
     uint2* out;
     uint32_t* hist; uint32_t* totals;
-    long long padding;
-    uint32_t rows, mask;
-    int tokens, per_block, nblocks, shift, bits, wide;
+    uint32_t mask;
+    int tokens, per_block, nblocks, shift, bits;
 };
 
 template <bool FIRST>
-__device__ __forceinline__ uint32_t ex_key(const EmSort& a, int i) {
-    return FIRST ? em_key(a.ids, i, a.wide, a.padding, a.rows) : a.in[i].x;
-}
+__device__ __forceinline__ uint32_t ex_key(const EmSort& a, int i) { return FIRST ? a.ids.key(i) : a.in[i].x; }
 
 template <bool FIRST>
-__global__ void __launch_bounds__(EX_THREADS)
-embedding_hist_kernel(EmSort a) {
-    __shared__ uint32_t h[EX_BINS];
-    const int bins = 1 << a.bits;
-    for (int d = threadIdx.x; d < bins; d += EX_THREADS) h[d] = 0;
-    __syncthreads();
-    const int begin = blockIdx.x * a.per_block, end = min(begin + a.per_block, a.tokens);
-    for (int i = begin + threadIdx.x; i < end; i += EX_THREADS) atomicAdd(&h[(ex_key<FIRST>(a, i) >> a.shift) & a.mask], 1u);
-    __syncthreads();
-    for (int d = threadIdx.x; d < bins; d += EX_THREADS) a.hist[(size_t)blockIdx.x * bins + d] = h[d];
-}
+struct EmHist {
+    static const int threads = EX_THREADS;
+    EmSort a;
+    __device__ __forceinline__ void run(int block) const {
+        __shared__ uint32_t h[EX_BINS];
+        const int bins = 1 << a.bits;
+        for (int d = threadIdx.x; d < bins; d += EX_THREADS) h[d] = 0;
+        __syncthreads();
+        const int begin = block * a.per_block, end = min(begin + a.per_block, a.tokens);
+        for (int i = begin + threadIdx.x; i < end; i += EX_THREADS) atomicAdd(&h[(ex_key<FIRST>(a, i) >> a.shift) & a.mask], 1u);
+        __syncthreads();
+        for (int d = threadIdx.x; d < bins; d += EX_THREADS) a.hist[(size_t)block * bins + d] = h[d];
+    }
+};
 
 __device__ __forceinline__ uint32_t ex_scan(uint32_t v, uint32_t* wsum, uint32_t& total) {   // exclusive, 256 threads
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -390,139 +420,147 @@ __device__ __forceinline__ uint32_t ex_scan(uint32_t v, uint32_t* wsum, uint32_t
 // A workgroup has 32 digits (a line of each block's counts); 32 chunks of up to 32 blocks are scanned side by side.
 #define EX_SCAN_THREADS 1024
 static_assert(EX_MAX_BLOCKS <= 32 * 32, "blocks of one scan");
-__global__ void __launch_bounds__(EX_SCAN_THREADS)
-embedding_scan_kernel(uint32_t* __restrict__ hist, uint32_t* __restrict__ totals, int nblocks, int bins) {
-    __shared__ uint32_t sums[32][33];
-    const int d = threadIdx.x & 31, chunk = threadIdx.x >> 5, digit = blockIdx.x * 32 + d;
-    const int each = (nblocks + 31) / 32, b0 = chunk * each;
-    uint32_t v[32], s = 0;
+struct EmScan {
+    static const int threads = EX_SCAN_THREADS;
+    uint32_t* __restrict__ hist;
+    uint32_t* __restrict__ totals;
+    int nblocks, bins;
+    __device__ __forceinline__ void run(int block) const {
+        __shared__ uint32_t sums[32][33];
+        const int d = threadIdx.x & 31, chunk = threadIdx.x >> 5, digit = block * 32 + d;
+        const int each = (nblocks + 31) / 32, b0 = chunk * each;
+        uint32_t v[32], s = 0;
 #pragma unroll
-    for (int k = 0; k < 32; ++k) v[k] = k < each && b0 + k < nblocks && digit < bins ? hist[(size_t)(b0 + k) * bins + digit] : 0u;
+        for (int k = 0; k < 32; ++k) v[k] = k < each && b0 + k < nblocks && digit < bins ? hist[(size_t)(b0 + k) * bins + digit] : 0u;
 #pragma unroll
-    for (int k = 0; k < 32; ++k) s += v[k];
-    sums[chunk][d] = s;
-    __syncthreads();
-    uint32_t run = 0, all = 0;
+        for (int k = 0; k < 32; ++k) s += v[k];
+        sums[chunk][d] = s;
+        __syncthreads();
+        uint32_t run = 0, all = 0;
 #pragma unroll
-    for (int c = 0; c < 32; ++c) {
-        run += c < chunk ? sums[c][d] : 0u;
-        all += sums[c][d];
+        for (int c = 0; c < 32; ++c) {
+            run += c < chunk ? sums[c][d] : 0u;
+            all += sums[c][d];
+        }
+#pragma unroll
+        for (int k = 0; k < 32; ++k) {
+            if (k < each && b0 + k < nblocks && digit < bins) hist[(size_t)(b0 + k) * bins + digit] = run;
+            run += v[k];
+        }
+        if (chunk == 0 && digit < bins) totals[digit] = all;
     }
-#pragma unroll
-    for (int k = 0; k < 32; ++k) {
-        if (k < each && b0 + k < nblocks && digit < bins) hist[(size_t)(b0 + k) * bins + digit] = run;
-        run += v[k];
-    }
-    if (chunk == 0 && digit < bins) totals[digit] = all;
-}
+};
 
 template <bool FIRST, int EX_IPL>
-__global__ void __launch_bounds__(EX_THREADS)
-embedding_scatter_kernel(EmSort a) {
-    static_assert(EX_BINS == 2 * EX_THREADS, "a thread has two neighbouring digits");
-    __shared__ uint32_t running[EX_BINS];            // next place of each digit for this workgroup
-    __shared__ uint32_t cnt[4][EX_BINS];             // a wave's count of each digit, then where its first one lies in the tile
-    __shared__ uint32_t shift_to[EX_BINS];           // from a place in the tile to the place in the output
-    __shared__ uint2 ordered[EX_TILE(EX_IPL)];       // the tile in the order of its digits
-    __shared__ uint32_t wsum[4];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int bins = 1 << a.bits;
-    {
-        uint32_t total;
-        const int d = 2 * threadIdx.x;
-        const bool in0 = d < bins, in1 = d + 1 < bins;
-        const uint32_t t0 = in0 ? a.totals[d] : 0u, t1 = in1 ? a.totals[d + 1] : 0u;
-        const uint32_t h0 = in0 ? a.hist[(size_t)blockIdx.x * bins + d] : 0u;
-        const uint32_t h1 = in1 ? a.hist[(size_t)blockIdx.x * bins + d + 1] : 0u;
-        const uint32_t base = ex_scan(t0 + t1, wsum, total);
-        running[d] = base + h0;
-        running[d + 1] = base + t0 + h1;
-    }
-    const int begin = blockIdx.x * a.per_block, end = min(begin + a.per_block, a.tokens);
-    const unsigned long long below = lane == 0 ? 0ull : (~0ull >> (64 - lane));
-    for (int tile = begin; tile < end; tile += EX_TILE(EX_IPL)) {
-#pragma unroll
-        for (int w = 0; w < 4; ++w) cnt[w][threadIdx.x] = cnt[w][threadIdx.x + EX_THREADS] = 0;
-        __syncthreads();
-        uint32_t key[EX_IPL], tok[EX_IPL], rank[EX_IPL];
-        const int at = tile + wave * (64 * EX_IPL) + lane;
-#pragma unroll
-        for (int k = 0; k < EX_IPL; ++k) {
-            const int i = at + 64 * k;
-            if (FIRST) {
-                key[k] = i < end ? ex_key<true>(a, i) : 0xFFFFFFFFu;
-                tok[k] = (uint32_t)i;
-            } else {
-                const uint2 e = i < end ? a.in[i] : make_uint2(0xFFFFFFFFu, 0u);
-                key[k] = e.x;
-                tok[k] = e.y;
-            }
+struct EmScatter {
+    static const int threads = EX_THREADS;
+    EmSort a;
+    __device__ __forceinline__ void run(int block) const {
+        static_assert(EX_BINS == 2 * EX_THREADS, "a thread has two neighbouring digits");
+        __shared__ uint32_t running[EX_BINS];            // next place of each digit for this workgroup
+        __shared__ uint32_t cnt[4][EX_BINS];             // a wave's count of each digit, then where its first one lies in the tile
+        __shared__ uint32_t shift_to[EX_BINS];           // from a place in the tile to the place in the output
+        __shared__ uint2 ordered[EX_TILE(EX_IPL)];       // the tile in the order of its digits
+        __shared__ uint32_t wsum[4];
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        const int bins = 1 << a.bits;
+        {
+            uint32_t total;
+            const int d = 2 * threadIdx.x;
+            const bool in0 = d < bins, in1 = d + 1 < bins;
+            const uint32_t t0 = in0 ? a.totals[d] : 0u, t1 = in1 ? a.totals[d + 1] : 0u;
+            const uint32_t h0 = in0 ? a.hist[(size_t)block * bins + d] : 0u;
+            const uint32_t h1 = in1 ? a.hist[(size_t)block * bins + d + 1] : 0u;
+            const uint32_t base = ex_scan(t0 + t1, wsum, total);
+            running[d] = base + h0;
+            running[d + 1] = base + t0 + h1;
         }
+        const int begin = block * a.per_block, end = min(begin + a.per_block, a.tokens);
+        const unsigned long long below = lane == 0 ? 0ull : (~0ull >> (64 - lane));
+        for (int tile = begin; tile < end; tile += EX_TILE(EX_IPL)) {
 #pragma unroll
-        for (int k = 0; k < EX_IPL; ++k) {
-            const bool ok = at + 64 * k < end;
-            const uint32_t d = (key[k] >> a.shift) & a.mask;
-            unsigned long long peers = __ballot(ok);  // lanes with the same digit
+            for (int w = 0; w < 4; ++w) cnt[w][threadIdx.x] = cnt[w][threadIdx.x + EX_THREADS] = 0;
+            __syncthreads();
+            uint32_t key[EX_IPL], tok[EX_IPL], rank[EX_IPL];
+            const int at = tile + wave * (64 * EX_IPL) + lane;
 #pragma unroll
-            for (int b = 0; b < EX_BITS; ++b) {
-                if (b < a.bits) {
-                    const unsigned long long bal = __ballot((d >> b) & 1u);
-                    peers &= ((d >> b) & 1u) ? bal : ~bal;
+            for (int k = 0; k < EX_IPL; ++k) {
+                const int i = at + 64 * k;
+                if (FIRST) {
+                    key[k] = i < end ? ex_key<true>(a, i) : 0xFFFFFFFFu;
+                    tok[k] = (uint32_t)i;
+                } else {
+                    const uint2 e = i < end ? a.in[i] : make_uint2(0xFFFFFFFFu, 0u);
+                    key[k] = e.x;
+                    tok[k] = e.y;
                 }
             }
-            const uint32_t first = (uint32_t)__popcll(peers & below);
-            const uint32_t prev = ok ? cnt[wave][d] : 0u;
-            rank[k] = prev + first;
-            if (ok && first == 0) cnt[wave][d] = prev + (uint32_t)__popcll(peers);
-        }
-        __syncthreads();
-        {
-            const int d = 2 * threadIdx.x;
-            uint32_t c[2][4], all;
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                c[0][w] = cnt[w][d];
-                c[1][w] = cnt[w][d + 1];
+            for (int k = 0; k < EX_IPL; ++k) {
+                const bool ok = at + 64 * k < end;
+                const uint32_t d = (key[k] >> a.shift) & a.mask;
+                unsigned long long peers = __ballot(ok);  // lanes with the same digit
+#pragma unroll
+                for (int b = 0; b < EX_BITS; ++b) {
+                    if (b < a.bits) {
+                        const unsigned long long bal = __ballot((d >> b) & 1u);
+                        peers &= ((d >> b) & 1u) ? bal : ~bal;
+                    }
+                }
+                const uint32_t first = (uint32_t)__popcll(peers & below);
+                const uint32_t prev = ok ? cnt[wave][d] : 0u;
+                rank[k] = prev + first;
+                if (ok && first == 0) cnt[wave][d] = prev + (uint32_t)__popcll(peers);
             }
-            const uint32_t n0 = c[0][0] + c[0][1] + c[0][2] + c[0][3], n1 = c[1][0] + c[1][1] + c[1][2] + c[1][3];
-            uint32_t g = ex_scan(n0 + n1, wsum, all);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                shift_to[d + h] = running[d + h] - g;
-                running[d + h] += h ? n1 : n0;
+            __syncthreads();
+            {
+                const int d = 2 * threadIdx.x;
+                uint32_t c[2][4], all;
 #pragma unroll
                 for (int w = 0; w < 4; ++w) {
-                    cnt[w][d + h] = g;
-                    g += c[h][w];
+                    c[0][w] = cnt[w][d];
+                    c[1][w] = cnt[w][d + 1];
+                }
+                const uint32_t n0 = c[0][0] + c[0][1] + c[0][2] + c[0][3], n1 = c[1][0] + c[1][1] + c[1][2] + c[1][3];
+                uint32_t g = ex_scan(n0 + n1, wsum, all);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    shift_to[d + h] = running[d + h] - g;
+                    running[d + h] += h ? n1 : n0;
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        cnt[w][d + h] = g;
+                        g += c[h][w];
+                    }
                 }
             }
-        }
-        __syncthreads();
-        // through LDS: written from there, the tokens of a digit are neighbours (a store of 64 lanes touches a few runs and
-        // not 64 places; 13 us instead of 21 for a pass of 6 bits over 2,000,000)
+            __syncthreads();
+            // through LDS: written from there, the tokens of a digit are neighbours (a store of 64 lanes touches a few runs and
+            // not 64 places; 13 us instead of 21 for a pass of 6 bits over 2,000,000)
 #pragma unroll
-        for (int k = 0; k < EX_IPL; ++k) {
-            if (at + 64 * k < end) {
-                const uint32_t to = cnt[wave][(key[k] >> a.shift) & a.mask] + rank[k];
-                ordered[to] = make_uint2(key[k], tok[k]);
+            for (int k = 0; k < EX_IPL; ++k) {
+                if (at + 64 * k < end) {
+                    const uint32_t to = cnt[wave][(key[k] >> a.shift) & a.mask] + rank[k];
+                    ordered[to] = make_uint2(key[k], tok[k]);
+                }
             }
+            __syncthreads();
+            const int have = min(end - tile, EX_TILE(EX_IPL));
+            for (int j = threadIdx.x; j < have; j += EX_THREADS) {
+                const uint2 e = ordered[j];
+                a.out[shift_to[(e.x >> a.shift) & a.mask] + (uint32_t)j] = e;
+            }
+            __syncthreads();
         }
-        __syncthreads();
-        const int have = min(end - tile, EX_TILE(EX_IPL));
-        for (int j = threadIdx.x; j < have; j += EX_THREADS) {
-            const uint2 e = ordered[j];
-            a.out[shift_to[(e.x >> a.shift) & a.mask] + (uint32_t)j] = e;
-        }
-        __syncthreads();
     }
-}
+};
 
 // ---- the walk ----
 #define EW_THREADS 256
 #define EW_SHARE 64                                  // items of a share at most
 #define EW_ITEMS 2048                                // items of a workgroup's shares at most: their tokens lie in LDS
 #define EW_BATCH 4                                   // tokens whose rows are loaded before the first is added
-#define EW_SMALL 128                                 // so few tokens are sorted by every workgroup for itself
+#define EW_SMALL FDGS_EMBEDDING_FEW                  // so few tokens are sorted by every workgroup for itself
 
 struct EmBwd {
     const uint2* sorted;                             // (key, token)
@@ -799,13 +837,25 @@ embedding_join_kernel(EmBwd a) {
 }
 
 // ---- host: sizes, workspace, launches ----
+// Where a sort's work lies in the workspace.
+struct EmSortPlan { size_t other, hist, totals, bytes; };
+static EmSortPlan em_sort_plan(long long tokens) {
+    EmSortPlan p;
+    size_t at = 0;
+    auto take = [&at](size_t n) { const size_t o = at; at += (n + 255) / 256 * 256; return o; };
+    const bool radix = tokens > ER_MAX_TOKENS, buckets = tokens > ER_DIRECT && !radix;
+    p.other = take(radix || buckets ? tokens * 8 : 0);
+    p.hist = take(radix ? (size_t)EX_BINS * EX_MAX_BLOCKS * 4 : buckets ? (size_t)EB_STARTS * (ER_MAX_TOKENS / EB_LIST) * 4 : 0);
+    p.totals = take(radix ? EX_BINS * 4 : 0);
+    p.bytes = at;
+    return p;
+}
+
 struct EmPlan {
     int vec, nv, tiles, lanes, groups, share;
     long long shares, blocks;
-    size_t sorted, other, hist, totals, info, fresh, head, tail, bytes;   // offsets into the workspace
+    size_t sorted, sort, info, fresh, head, tail, bytes;   // offsets into the workspace
 };
-
-static int em_full(int type) { return type == FDGS_TYPE_F32 ? EmF32::full : EmBf16::full; }
 
 static EmPlan em_plan(long long tokens, long long rows, int dim, int type) {
     EmPlan p;
@@ -829,10 +879,7 @@ static EmPlan em_plan(long long tokens, long long rows, int dim, int type) {
     size_t at = 0;
     auto take = [&at](size_t n) { const size_t o = at; at += (n + 255) / 256 * 256; return o; };
     p.sorted = take(tokens * 8);
-    const bool radix = tokens > ER_MAX_TOKENS, buckets = tokens > ER_DIRECT && !radix;
-    p.other = take(radix || buckets ? tokens * 8 : 0);
-    p.hist = take(radix ? (size_t)EX_BINS * EX_MAX_BLOCKS * 4 : buckets ? (size_t)EB_STARTS * (ER_MAX_TOKENS / EB_LIST) * 4 : 0);
-    p.totals = take(radix ? EX_BINS * 4 : 0);
+    p.sort = take(em_sort_plan(tokens).bytes);
     const bool small = tokens <= EW_SMALL;           // no row is cut
     p.info = take(small ? 0 : p.shares * 4);
     p.fresh = take(small ? 0 : p.shares + 16) + 16;
@@ -847,31 +894,49 @@ extern "C" size_t fdgs_embedding_bwd_workspace_bytes(int64_t num_tokens, int32_t
     return em_plan(num_tokens, num_rows, dim, type).bytes;
 }
 
-// The sorted pairs end up at ws + p.sorted.
-static int em_sort(const fdgs_embedding_bwd_args* a, const EmPlan& p, char* ws, hipStream_t s) {
-    const int tokens = (int)a->num_tokens;
-    const long long padding = a->padding_id >= 0 ? a->padding_id : -1;
-    const int wide = a->id_bytes == 8;
-    int key_bits = 1;
-    while (key_bits < 31 && (1ll << key_bits) <= (long long)a->num_rows) ++key_bits;   // keys 0 .. num_rows
-    if (tokens <= ER_DIRECT) {
-        hipLaunchKernelGGL(embedding_rank_kernel, dim3((tokens + 63) / 64), dim3(ER_THREADS), 0, s, a->ids, tokens, wide, padding,
-                           (uint32_t)a->num_rows, (uint2*)(ws + p.sorted));
+// The launches of a sort, each with its part of a lookup.
+struct EmSteps {
+    EmPart part;
+    long long groups;                                // of the lookup, 0: none
+    int whole, at;                                   // weights of the launches: of all, of those that are done
+    hipStream_t s;
+    template <class Step>
+    int run(const Step& step, int blocks, int weight) {
+        const int each = Step::threads / EF_THREADS;
+        part.first = (int)(groups * at / whole);
+        at += weight;
+        part.last = (int)(groups * at / whole);
+        const int more = (part.last - part.first + each - 1) / each;
+        const int period = more >= 2 * blocks ? 3 : 1;
+        hipLaunchKernelGGL((embedding_step_kernel<Step>), dim3((unsigned)(blocks + more)), dim3(Step::threads), 0, s, step, blocks, period, part);
         FDGS_CHECK_LAUNCH();
         return FDGS_OK;
     }
+};
+
+#define EM_RUN(call) do { const int rc_ = (call); if (rc_ != FDGS_OK) return rc_; } while (0)
+// sorted [tokens] pairs, ws: a workspace of em_sort_plan(tokens).bytes; lookup: its workgroups run beside (NULL: none)
+static int em_sort(const EmIds& in, uint2* sorted, char* ws, const EmPart* lookup, long long groups, hipStream_t s) {
+    const int tokens = in.tokens;
+    const EmSortPlan p = em_sort_plan(tokens);
+    EmSteps steps = {};
+    steps.s = s;
+    steps.whole = 1;
+    if (lookup) {
+        steps.part = *lookup;
+        steps.groups = groups;
+    }
+    int key_bits = 1;
+    while (key_bits < 31 && (1ll << key_bits) <= (long long)in.rows) ++key_bits;       // keys 0 .. rows
+    if (tokens <= ER_DIRECT) return steps.run(EmRank{in, sorted}, (tokens + 63) / 64, 1);
     if (tokens <= ER_MAX_TOKENS) {
         const int shift = key_bits > 11 ? key_bits - 11 : 0, nlists = (tokens + EB_LIST - 1) / EB_LIST;
         static_assert(EB_BUCKETS == 1 << 11 && EB_BUCKETS == 2 * EB_THREADS, "buckets of the upper 11 bits, two to a thread");
         uint2* lists = (uint2*)(ws + p.other);
         uint32_t* starts = (uint32_t*)(ws + p.hist);
-        hipLaunchKernelGGL(embedding_bucket_kernel, dim3(nlists), dim3(EB_THREADS), 0, s, a->ids, tokens, wide, padding,
-                           (uint32_t)a->num_rows, shift, lists, starts);
-        FDGS_CHECK_LAUNCH();
-        hipLaunchKernelGGL(embedding_place_kernel, dim3((tokens + 63) / 64), dim3(ER_THREADS), 0, s, lists, starts, tokens, nlists,
-                           shift, (uint32_t)a->num_rows, (uint2*)(ws + p.sorted));
-        FDGS_CHECK_LAUNCH();
-        return FDGS_OK;
+        steps.whole = 2;
+        EM_RUN(steps.run(EmBucket{in, shift, lists, starts}, nlists, 1));
+        return steps.run(EmPlace{lists, starts, tokens, nlists, shift, in.rows, sorted}, (tokens + 63) / 64, 1);
     }
     const int passes = (key_bits + EX_BITS - 1) / EX_BITS;
     // a workgroup's tile takes 5 us whatever its length: short tiles while there are workgroups to be had for them
@@ -880,34 +945,68 @@ static int em_sort(const fdgs_embedding_bwd_args* a, const EmPlan& p, char* ws, 
     const long long per_block = (tiles + blocks - 1) / blocks * EX_TILE(ipl);
     blocks = (tokens + per_block - 1) / per_block;
     EmSort k = {};
-    k.ids = a->ids; k.wide = wide; k.padding = padding; k.rows = (uint32_t)a->num_rows; k.tokens = tokens;
+    k.ids = in; k.tokens = tokens;
     k.per_block = (int)per_block; k.nblocks = (int)blocks;
     k.hist = (uint32_t*)(ws + p.hist); k.totals = (uint32_t*)(ws + p.totals);
+    // The lookup goes where workgroups wait most, and in large parts (a part takes 2 us at least): to the scatters, and a little
+    // of it to the scans, which leave most of the chip idle.  Sort and lookup of 300,000 tokens of 48 floats 37.5 us and of
+    // 2,000,000 152 (one after the other 43 and 163; all of it in the scatters 40 and 153; the same in every launch 41 and 164).
+    const int with_scan = 1, with_scatter = 5;
+    steps.whole = (with_scan + with_scatter) * passes;
     for (int pass = 0; pass < passes; ++pass) {
         k.bits = (key_bits - k.shift + passes - pass - 1) / (passes - pass);           // the remaining bits, evenly
         k.mask = (1u << k.bits) - 1u;
         const bool to_first = ((passes - 1 - pass) & 1) == 0;                          // the last pass ends in `sorted`
-        k.out = (uint2*)(ws + (to_first ? p.sorted : p.other));
-        k.in = (const uint2*)(ws + (to_first ? p.other : p.sorted));
-        const dim3 grid((unsigned)blocks), threads(EX_THREADS);
-        if (pass == 0) hipLaunchKernelGGL(embedding_hist_kernel<true>, grid, threads, 0, s, k);
-        else hipLaunchKernelGGL(embedding_hist_kernel<false>, grid, threads, 0, s, k);
-        FDGS_CHECK_LAUNCH();
-        hipLaunchKernelGGL(embedding_scan_kernel, dim3(((1u << k.bits) + 31) / 32), dim3(EX_SCAN_THREADS), 0, s, k.hist, k.totals, k.nblocks, 1 << k.bits);
-        FDGS_CHECK_LAUNCH();
-        if (pass == 0) {
-            if (ipl == 2) hipLaunchKernelGGL((embedding_scatter_kernel<true, 2>), grid, threads, 0, s, k);
-            else if (ipl == 4) hipLaunchKernelGGL((embedding_scatter_kernel<true, 4>), grid, threads, 0, s, k);
-            else hipLaunchKernelGGL((embedding_scatter_kernel<true, 8>), grid, threads, 0, s, k);
-        } else {
-            if (ipl == 2) hipLaunchKernelGGL((embedding_scatter_kernel<false, 2>), grid, threads, 0, s, k);
-            else if (ipl == 4) hipLaunchKernelGGL((embedding_scatter_kernel<false, 4>), grid, threads, 0, s, k);
-            else hipLaunchKernelGGL((embedding_scatter_kernel<false, 8>), grid, threads, 0, s, k);
-        }
-        FDGS_CHECK_LAUNCH();
+        k.out = to_first ? sorted : (uint2*)(ws + p.other);
+        k.in = to_first ? (const uint2*)(ws + p.other) : sorted;
+        const int n = (int)blocks;
+        EM_RUN(pass == 0 ? steps.run(EmHist<true>{k}, n, 0) : steps.run(EmHist<false>{k}, n, 0));
+        EM_RUN(steps.run(EmScan{k.hist, k.totals, k.nblocks, 1 << k.bits}, ((1 << k.bits) + 31) / 32, with_scan));
+        if (pass == 0) EM_RUN(ipl == 2 ? steps.run(EmScatter<true, 2>{k}, n, with_scatter) : ipl == 4 ? steps.run(EmScatter<true, 4>{k}, n, with_scatter) : steps.run(EmScatter<true, 8>{k}, n, with_scatter));
+        else EM_RUN(ipl == 2 ? steps.run(EmScatter<false, 2>{k}, n, with_scatter) : ipl == 4 ? steps.run(EmScatter<false, 4>{k}, n, with_scatter) : steps.run(EmScatter<false, 8>{k}, n, with_scatter));
         k.shift += k.bits;
     }
     return FDGS_OK;
+}
+
+extern "C" size_t fdgs_embedding_sort_workspace_bytes(int64_t num_tokens) {
+    return num_tokens < 0 || num_tokens > FDGS_EMBEDDING_MAX_TOKENS ? 0 : em_sort_plan(num_tokens).bytes;
+}
+
+extern "C" int fdgs_embedding_fwd(const fdgs_embedding_fwd_args* a, void* stream) {
+    if (!a || a->num_tokens < 0 || a->num_rows < 0 || a->dim < 0 || !em_type_ok(a->type)) return FDGS_EINVAL;
+    if (a->id_bytes != 4 && a->id_bytes != 8) return FDGS_EINVAL;
+    if (a->num_tokens == 0 || a->dim == 0) return FDGS_OK;
+    if (!a->ids || !a->out || (a->num_rows > 0 && !a->table)) return FDGS_EINVAL;
+    if (a->num_rows > 0 && a->table_row_stride < 0) return FDGS_EINVAL;
+    if (a->dim > FDGS_EMBEDDING_MAX_DIM || a->num_tokens > (a->sorted ? FDGS_EMBEDDING_MAX_TOKENS : 0x7fffffffLL)) return FDGS_ETOOLARGE;
+    EmPart f = {};
+    EmFwd& k = f.a;
+    k.ids = a->ids; k.table = a->table; k.out = a->out;
+    k.tokens = (int)a->num_tokens; k.table_stride = a->table_row_stride;
+    k.padding = a->padding_id >= 0 ? a->padding_id : -1;
+    k.rows = a->num_rows; k.dim = a->dim; k.wide = a->id_bytes == 8; k.scale = a->scale;
+    f.type = a->type;
+    f.vec = k.dim >= em_full(a->type) ? em_full(a->type) : 1;
+    k.nv = (k.dim + f.vec - 1) / f.vec;
+    k.by_nv = em_div_of((uint32_t)k.nv);
+    k.per_group = k.nv < EF_VECTORS ? EF_VECTORS / k.nv : 1;
+    const int tiles = (k.nv + EF_VECTORS - 1) / EF_VECTORS;
+    const long long groups = ((long long)k.tokens + k.per_group - 1) / k.per_group;
+    hipStream_t s = (hipStream_t)stream;
+    const bool sort = a->sorted && a->num_tokens > EW_SMALL;     // fewer are sorted where they are added
+    if (sort) {
+        if (a->workspace_bytes < em_sort_plan(a->num_tokens).bytes || (a->workspace_bytes > 0 && !a->workspace)) return FDGS_EWORKSPACE;
+        const EmIds in = {a->ids, k.padding, (uint32_t)a->num_rows, k.tokens, k.wide};
+        f.by_tiles = em_div_of((uint32_t)tiles);
+        const bool beside = groups * tiles <= 0x3fffffffLL;
+        EM_RUN(em_sort(in, (uint2*)a->sorted, (char*)a->workspace, beside ? &f : nullptr, groups * tiles, s));
+        if (beside) return FDGS_OK;
+    }
+    const dim3 grid((unsigned)groups, (unsigned)tiles);
+    if (a->type == FDGS_TYPE_F32) return em_fwd_launch<EmF32>(k, f.vec, grid, s);
+    if (a->type == FDGS_TYPE_BF16) return em_fwd_launch<EmBf16>(k, f.vec, grid, s);
+    return em_fwd_launch<EmF16>(k, f.vec, grid, s);
 }
 
 template <class T>
@@ -947,16 +1046,17 @@ extern "C" int fdgs_embedding_bwd(const fdgs_embedding_bwd_args* a, void* stream
     if (!a->workspace || a->workspace_bytes < p.bytes) return FDGS_EWORKSPACE;
     hipStream_t s = (hipStream_t)stream;
     char* ws = (char*)a->workspace;
-    if (a->num_tokens > EW_SMALL) {
-        const int rc = em_sort(a, p, ws, s);
-        if (rc != FDGS_OK) return rc;
-    }
+    const long long padding = a->padding_id >= 0 ? a->padding_id : -1;
     EmBwd k = {};
-    k.sorted = (const uint2*)(ws + p.sorted);
+    k.sorted = (const uint2*)(a->sorted ? a->sorted : ws + p.sorted);
+    if (a->num_tokens > EW_SMALL && !a->sorted) {
+        const EmIds in = {a->ids, padding, (uint32_t)a->num_rows, (int)a->num_tokens, a->id_bytes == 8};
+        EM_RUN(em_sort(in, (uint2*)(ws + p.sorted), ws + p.sort, nullptr, 0, s));
+    }
     k.dout = a->grad_out; k.dtable = a->grad_table;
     k.head = (float*)(ws + p.head); k.tail = (float*)(ws + p.tail); k.fresh = (uint8_t*)(ws + p.fresh);
     k.info = (uint32_t*)(ws + p.info); k.shares = (int)p.shares;
-    k.ids = a->ids; k.wide = a->id_bytes == 8; k.padding = a->padding_id >= 0 ? a->padding_id : -1;
+    k.ids = a->ids; k.wide = a->id_bytes == 8; k.padding = padding;
     k.dout_stride = a->grad_out_row_stride; k.items = a->num_rows + a->num_tokens;
     k.tokens = (int)a->num_tokens; k.rows = a->num_rows; k.dim = a->dim; k.nv = p.nv; k.lanes = p.lanes; k.groups = p.groups;
     k.share = p.share; k.scale = a->scale;

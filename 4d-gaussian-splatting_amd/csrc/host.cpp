@@ -125,6 +125,7 @@ struct Library {
     const char* (*strerror)(int) = nullptr;
     size_t (*adamw_ws)(int32_t) = nullptr;
     size_t (*moment8_ws)(int32_t) = nullptr;
+    size_t (*sort_ws)(int64_t) = nullptr;
     PyObject* module = nullptr;
 } library;
 
@@ -365,7 +366,9 @@ Tensor rows_of(const Tensor& t, int64_t lead, int64_t& width, int64_t& stride) {
     return t;
 }
 
-Tensor lookup(const Tensor& ids0, const Tensor& table0, double scale, int64_t padding) {
+// sorted: where it is given, it is set to the tokens by row, which spare the gradient its sort (undefined where there is
+// nothing to sort).
+Tensor lookup(const Tensor& ids0, const Tensor& table0, double scale, int64_t padding, Tensor* sorted = nullptr) {
     const int type = type_of(table0, "the table");
     const Tensor ids = ids_of(ids0, table0.device());
     int64_t width, stride;
@@ -387,17 +390,27 @@ Tensor lookup(const Tensor& ids0, const Tensor& table0, double scale, int64_t pa
     a.padding_id = padding;
     a.out = out.data_ptr();
     a.scale = (float)scale;
+    Tensor workspace;
+    if (sorted && a.num_tokens > FDGS_EMBEDDING_FEW && a.num_tokens <= FDGS_EMBEDDING_MAX_TOKENS && a.num_rows > 0 && width > 0) {
+        const auto bytes = table.options().dtype(at::kByte).requires_grad(false);
+        *sorted = at::empty({8 * a.num_tokens}, bytes);
+        a.workspace_bytes = library.sort_ws(a.num_tokens);
+        if (a.workspace_bytes) workspace = at::empty({(int64_t)a.workspace_bytes}, bytes);
+        a.sorted = sorted->data_ptr();
+        a.workspace = a.workspace_bytes ? workspace.data_ptr() : nullptr;
+    }
     launch("fdgs_embedding_fwd", library.fwd, a, table.device());
     return out;
 }
 
-Tensor table_grad(const Tensor& grad_out0, const Tensor& ids0, int64_t rows, double scale, int64_t padding) {
+Tensor table_grad(const Tensor& grad_out0, const Tensor& ids0, int64_t rows, double scale, int64_t padding, const Tensor& sorted = Tensor()) {
     on_gpu(grad_out0);
     const int type = type_of(grad_out0, "grad_out");
     const Tensor ids = ids_of(ids0, grad_out0.device());
     int64_t lead = ids.dim();
     if (grad_out0.dim() <= lead || grad_out0.sizes().slice(0, lead) != ids.sizes()) value_error("grad_out has to be [*ids.shape, ...]");
     if (rows < 0 || rows > INT32_MAX) value_error("num_rows is between 0 and 2^31 - 1");
+    if (sorted.defined() && sorted.numel() != 8 * ids.numel()) value_error("ids have another size than in the lookup");
     std::vector<int64_t> shape{rows};
     shape.insert(shape.end(), grad_out0.sizes().begin() + lead, grad_out0.sizes().end());
     Tensor view = grad_out0;
@@ -425,6 +438,7 @@ Tensor table_grad(const Tensor& grad_out0, const Tensor& ids0, int64_t rows, dou
     a.padding_id = padding;
     a.grad_table = out.data_ptr();
     a.scale = (float)scale;
+    a.sorted = sorted.defined() ? sorted.data_ptr() : nullptr;
     a.workspace = workspace.data_ptr();
     a.workspace_bytes = bytes;
     launch("fdgs_embedding_bwd", library.bwd, a, g.device());
@@ -437,37 +451,42 @@ struct Lookup : torch::autograd::Function<Lookup> {
     static Tensor forward(AutogradContext* ctx, const Tensor& table, const Tensor& ids, double scale, int64_t padding);
     static variable_list backward(AutogradContext* ctx, variable_list grads);
 };
+struct Sorted { Tensor pairs; };                      // not one of a function's inputs; undefined: not sorted yet
 struct TableGrad : torch::autograd::Function<TableGrad> {
-    static Tensor forward(AutogradContext* ctx, const Tensor& grad_out, const Tensor& ids, int64_t rows, double scale, int64_t padding);
+    static Tensor forward(AutogradContext* ctx, const Tensor& grad_out, const Tensor& ids, const Sorted& sorted, int64_t rows, double scale, int64_t padding);
     static variable_list backward(AutogradContext* ctx, variable_list grads);
 };
 
 Tensor Lookup::forward(AutogradContext* ctx, const Tensor& table, const Tensor& ids, double scale, int64_t padding) {
-    ctx->save_for_backward({ids});
+    Tensor sorted;
+    const Tensor out = lookup(ids, table, scale, padding, &sorted);
+    ctx->save_for_backward({ids, sorted});
     ctx->saved_data["rows"] = table.size(0);
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["padding"] = padding;
-    return lookup(ids, table, scale, padding);
+    return out;
 }
 variable_list Lookup::backward(AutogradContext* ctx, variable_list grads) {
-    const Tensor ids = ctx->get_saved_variables()[0];
+    const variable_list saved = ctx->get_saved_variables();
+    const Tensor &ids = saved[0], &sorted = saved[1];
     const int64_t rows = ctx->saved_data["rows"].toInt(), padding = ctx->saved_data["padding"].toInt();
     const double scale = ctx->saved_data["scale"].toDouble();
     const bool graph = at::GradMode::is_enabled() && grads[0].requires_grad();
-    return {graph ? TableGrad::apply(grads[0], ids, rows, scale, padding) : table_grad(grads[0], ids, rows, scale, padding), Tensor(), Tensor(), Tensor()};
+    return {graph ? TableGrad::apply(grads[0], ids, Sorted{sorted}, rows, scale, padding) : table_grad(grads[0], ids, rows, scale, padding, sorted),
+            Tensor(), Tensor(), Tensor()};
 }
-Tensor TableGrad::forward(AutogradContext* ctx, const Tensor& grad_out, const Tensor& ids, int64_t rows, double scale, int64_t padding) {
+Tensor TableGrad::forward(AutogradContext* ctx, const Tensor& grad_out, const Tensor& ids, const Sorted& sorted, int64_t rows, double scale, int64_t padding) {
     ctx->save_for_backward({ids});
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["padding"] = padding;
-    return table_grad(grad_out, ids, rows, scale, padding);
+    return table_grad(grad_out, ids, rows, scale, padding, sorted.pairs);
 }
 variable_list TableGrad::backward(AutogradContext* ctx, variable_list grads) {
     const Tensor ids = ctx->get_saved_variables()[0];
     const int64_t padding = ctx->saved_data["padding"].toInt();
     const double scale = ctx->saved_data["scale"].toDouble();
     const bool graph = at::GradMode::is_enabled() && grads[0].requires_grad();
-    return {graph ? Lookup::apply(grads[0], ids, scale, padding) : lookup(ids, grads[0], scale, padding), Tensor(), Tensor(), Tensor(), Tensor()};
+    return {graph ? Lookup::apply(grads[0], ids, scale, padding) : lookup(ids, grads[0], scale, padding), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
 }
 
 int64_t padding_of(PyObject* o) {
@@ -544,11 +563,11 @@ PyObject* rows_layout(PyObject* a) {
 }
 
 // bind(module, addresses of fdgs_embedding_fwd, _bwd_workspace_bytes, _bwd, fdgs_adamw_step, fdgs_moment8_unpack, _pack,
-// fdgs_strerror, fdgs_adamw_workspace_bytes, fdgs_moment8_workspace_bytes)
+// fdgs_strerror, fdgs_adamw_workspace_bytes, fdgs_moment8_workspace_bytes, fdgs_embedding_sort_workspace_bytes)
 PyObject* bind(PyObject* a) {
-    unsigned long long fwd, ws, bwd, adamw, unpack, pack, err, adamw_ws, moment8_ws;
+    unsigned long long fwd, ws, bwd, adamw, unpack, pack, err, adamw_ws, moment8_ws, sort_ws;
     PyObject* module;
-    if (!PyArg_ParseTuple(a, "OKKKKKKKKK", &module, &fwd, &ws, &bwd, &adamw, &unpack, &pack, &err, &adamw_ws, &moment8_ws)) throw Raised();
+    if (!PyArg_ParseTuple(a, "OKKKKKKKKKK", &module, &fwd, &ws, &bwd, &adamw, &unpack, &pack, &err, &adamw_ws, &moment8_ws, &sort_ws)) throw Raised();
     Py_INCREF(module);
     Py_XDECREF(library.module);
     library.module = module;
@@ -561,6 +580,7 @@ PyObject* bind(PyObject* a) {
     library.strerror = (decltype(library.strerror))(uintptr_t)err;
     library.adamw_ws = (decltype(library.adamw_ws))(uintptr_t)adamw_ws;
     library.moment8_ws = (decltype(library.moment8_ws))(uintptr_t)moment8_ws;
+    library.sort_ws = (decltype(library.sort_ws))(uintptr_t)sort_ws;
     Py_RETURN_NONE;
 }
 

@@ -236,6 +236,7 @@ SYMBOLS = {
     "fdgs_moment8_workspace_bytes": (c_sz, [c_i32]),
     "fdgs_moment8_unpack": (C.c_int, [C.POINTER(_records.Moment8Args), c_p]),
     "fdgs_embedding_fwd": (C.c_int, [C.POINTER(_records.EmbeddingFwdArgs), c_p]),
+    "fdgs_embedding_sort_workspace_bytes": (c_sz, [c_i64]),
     "fdgs_embedding_bwd_workspace_bytes": (c_sz, [c_i64, c_i32, c_i32, c_i32]),
     "fdgs_embedding_bwd": (C.c_int, [C.POINTER(_records.EmbeddingBwdArgs), c_p]),
     "fdgs_moment8_pack": (C.c_int, [C.POINTER(_records.Moment8Args), c_p]),
@@ -342,7 +343,8 @@ def _bind_host():
     from . import _host
     _host.bind(sys.modules[__name__], *(C.cast(getattr(lib, n), c_p).value for n in (
         "fdgs_embedding_fwd", "fdgs_embedding_bwd_workspace_bytes", "fdgs_embedding_bwd", "fdgs_adamw_step", "fdgs_moment8_unpack",
-        "fdgs_moment8_pack", "fdgs_strerror", "fdgs_adamw_workspace_bytes", "fdgs_moment8_workspace_bytes")))
+        "fdgs_moment8_pack", "fdgs_strerror", "fdgs_adamw_workspace_bytes", "fdgs_moment8_workspace_bytes",
+        "fdgs_embedding_sort_workspace_bytes")))
 
 
 _bind_host()

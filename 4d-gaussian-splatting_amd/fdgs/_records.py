@@ -36,11 +36,12 @@ EMBEDDING_MAX_TOKENS = 1 << 30          # FDGS_EMBEDDING_MAX_TOKENS
 class EmbeddingFwdArgs(C.Structure):
     _fields_ = [("num_tokens", C.c_int64), ("num_rows", C.c_int32), ("dim", C.c_int32), ("type", C.c_int32),
                 ("id_bytes", C.c_int32), ("ids", C.c_void_p), ("table", C.c_void_p), ("table_row_stride", C.c_int64),
-                ("padding_id", C.c_int64), ("out", C.c_void_p), ("scale", C.c_float)]
+                ("padding_id", C.c_int64), ("out", C.c_void_p), ("scale", C.c_float), ("sorted", C.c_void_p),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
 
 
 class EmbeddingBwdArgs(C.Structure):
     _fields_ = [("num_tokens", C.c_int64), ("num_rows", C.c_int32), ("dim", C.c_int32), ("type", C.c_int32),
                 ("id_bytes", C.c_int32), ("ids", C.c_void_p), ("grad_out", C.c_void_p),
                 ("grad_out_row_stride", C.c_int64), ("padding_id", C.c_int64), ("grad_table", C.c_void_p),
-                ("scale", C.c_float), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+                ("scale", C.c_float), ("sorted", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]

@@ -556,6 +556,7 @@ int fdgs_moment8_pack(const fdgs_moment8_args* a, void* stream);
  * or more gives a row of NaN, and nothing in the gradient.                                            */
 #define FDGS_EMBEDDING_MAX_TOKENS (1 << 30)          /* of the gradient; the lookup takes 2^31 - 1 */
 #define FDGS_EMBEDDING_MAX_DIM (1 << 22)
+#define FDGS_EMBEDDING_FEW 128                       /* so few tokens need no sort of their own: `sorted` is not used */
 typedef struct {
     int64_t num_tokens;
     int32_t num_rows, dim;
@@ -567,7 +568,11 @@ typedef struct {
     int64_t padding_id;              /* -1: none                                        */
     void* out;                       /* [num_tokens, dim]                               */
     float scale;
+    void* sorted;                    /* NULL, or [num_tokens] records of 8 bytes out: the tokens by row, which spare the
+                                        gradient its sort (beside the lookup it costs little)              */
+    void* workspace; size_t workspace_bytes;   /* with sorted: fdgs_embedding_sort_workspace_bytes(num_tokens) */
 } fdgs_embedding_fwd_args;
+size_t fdgs_embedding_sort_workspace_bytes(int64_t num_tokens);
 typedef struct {
     int64_t num_tokens;
     int32_t num_rows, dim;
@@ -579,6 +584,7 @@ typedef struct {
     int64_t padding_id;
     void* grad_table;                /* [num_rows, dim] out                             */
     float scale;
+    const void* sorted;              /* NULL, or what fdgs_embedding_fwd made of the same ids, rows and padding_id */
     void* workspace; size_t workspace_bytes;   /* fdgs_embedding_bwd_workspace_bytes(...) */
 } fdgs_embedding_bwd_args;
 int fdgs_embedding_fwd(const fdgs_embedding_fwd_args* a, void* stream);

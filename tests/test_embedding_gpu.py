@@ -361,3 +361,35 @@ def test_refusals_on_the_device():
     assert embedding(torch.tensor([0, 1], device="cuda"), torch.zeros(0, 4, device="cuda")).isnan().all()
     assert embedding(ids, torch.zeros(4, 0, device="cuda")).shape == (2, 0)
     assert embedding_grad(torch.zeros(2, 0, device="cuda"), ids, 4).shape == (4, 0)
+
+
+@pytest.mark.parametrize("tokens, rows, dim", [(128, 40, 7), (129, 40, 3), (2000, 17, 5), (4096, 300, 8), (4097, 300, 2), (9000, 5000, 4100),
+                                               (16384, 40000, 33), (16385, 40000, 1), (70001, 90, 48), (300000, 8192, 12), (600001, 300000, 3)])
+@pytest.mark.parametrize("dtype, idt", [(torch.float32, torch.int32), (torch.bfloat16, torch.int64), (torch.float16, torch.int32)])
+def test_lookup_that_sorts_for_its_gradient(tokens, rows, dim, dtype, idt):
+    """A lookup that is recorded sorts the tokens beside its own work: the output and the gradient have the bits of the plain
+    lookup and of the gradient that sorts by itself, also when the pass is walked back twice."""
+    from fdgs.embedding import embedding, embedding_grad
+    gen = torch.Generator().manual_seed(tokens)
+    table = torch.randn(rows, dim, generator=gen).to(dtype).cuda().requires_grad_(True)
+    ids = torch.randint(-3, rows + 2, (tokens,), generator=gen)
+    ids[torch.rand(tokens, generator=gen) < 0.3] = rows // 2     # a row with many tokens
+    ids = ids.to(idt).cuda()
+    gy = torch.randn(tokens, dim, generator=gen).to(dtype).cuda()
+    y = embedding(ids, table, scale=0.75, padding_id=1)
+    with torch.no_grad():
+        assert torch.equal(y.view(torch.uint8), embedding(ids, table, scale=0.75, padding_id=1).view(torch.uint8))
+    want = embedding_grad(gy, ids, rows, scale=0.75, padding_id=1)
+    for _ in range(2):
+        got, = torch.autograd.grad(y, table, gy, retain_graph=True)
+        assert torch.equal(got.view(torch.uint8), want.view(torch.uint8))
+
+
+def test_ids_that_change_after_the_lookup_are_noticed():
+    from fdgs.embedding import embedding
+    table = torch.randn(50, 4, device="cuda", requires_grad=True)
+    ids = torch.arange(50, device="cuda").repeat(5)
+    y = embedding(ids, table)
+    ids.zero_()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()

@@ -34,6 +34,17 @@ def test_library_refuses_before_any_launch():
     assert _bwd(workspace=0) == -3 and _bwd(workspace_bytes=16) == -3
 
 
+def test_sorted_tokens_need_a_workspace():
+    from fdgs import _lib
+    size = _lib.lib.fdgs_embedding_sort_workspace_bytes
+    assert size(-1) == 0 and size((1 << 30) + 1) == 0 and size(4096) == 0 and size(4097) >= 8 * 4097 and size(1 << 30) >= 8 << 30
+    for tokens in (5000, 20000):
+        assert _fwd(num_tokens=tokens, sorted=64) == -3
+        assert _fwd(num_tokens=tokens, sorted=64, workspace=64, workspace_bytes=size(tokens) - 1) == -3
+        assert _fwd(num_tokens=tokens, sorted=64, workspace=0, workspace_bytes=size(tokens)) == -3
+    assert _fwd(num_tokens=(1 << 30) + 1, sorted=64) == -4
+
+
 @pytest.mark.parametrize("kind", [0, 1, 2])
 def test_workspace_grows_with_the_work(kind):
     from fdgs._lib import lib
