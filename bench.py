@@ -358,7 +358,7 @@ def main():
         if share_gpu:
             dist.init_process_group(backend="gloo")
         else:
-            os.environ.setdefault("NCCL_ALGO", "Ring")      # see fdgs/dp.py: no packed fp32 in RCCL's ring sum kernels
+            os.environ.setdefault("NCCL_ALGO", "Ring")      # see fdgs/dp.py
             dist.init_process_group(backend="nccl", device_id=dev)
         if dist.get_world_size() != args.gpus:
             raise SystemExit(f"--gpus {args.gpus} but the process group has {dist.get_world_size()} ranks")

@@ -1,4 +1,5 @@
-"""Disassembles the gfx950 code objects inside a HIP shared library and counts instructions by mnemonic.
+"""Disassembles the gfx950 code objects inside a HIP shared library that was built here from its sources (libfdgs.so) and
+counts instructions by mnemonic.
 
 A HIP library carries its device code as clang offload bundles in the `.hip_fatbin` section (one bundle per
 translation unit): magic `__CLANG_OFFLOAD_BUNDLE__`, a 64-bit entry count, then per entry (offset, size, triple
