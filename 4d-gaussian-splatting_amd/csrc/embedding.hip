@@ -360,8 +360,8 @@ struct EmPlace {
     }
 };
 
-// Many tokens: a radix sort by digits of at most 9 bits (two passes for tables of up to 262,143 rows), three launches a
-// pass: counts of each workgroup, their scan, scatter.  2,000,000 tokens of 65,536 rows 57 us, 300,000 of 8,192 29 us.
+// Many tokens: a radix sort by digits of at most 9 bits (two passes for tables of up to 262,143 rows), two or three launches
+// a pass: counts of each block of tokens, their scan, scatter.  2,000,000 tokens of 65,536 rows 43 us, 300,000 of 8,192 25 us.
 #define EX_THREADS 256
 #define EX_TILE(ipl) (EX_THREADS * (ipl))             // tokens that a workgroup takes at a time, ipl to a lane
 #define EX_BITS 9
@@ -374,7 +374,7 @@ struct EmSort {
     uint2* out;
     uint32_t* hist; uint32_t* totals;
     uint32_t mask;
-    int tokens, per_block, nblocks, shift, bits;
+    int tokens, per_block, nblocks, shift, bits, ngroups;        // ngroups: totals of four blocks each, 0: of all
 };
 
 template <bool FIRST>
@@ -393,6 +393,39 @@ struct EmHist {
         for (int i = begin + threadIdx.x; i < end; i += EX_THREADS) atomicAdd(&h[(ex_key<FIRST>(a, i) >> a.shift) & a.mask], 1u);
         __syncthreads();
         for (int d = threadIdx.x; d < bins; d += EX_THREADS) a.hist[(size_t)block * bins + d] = h[d];
+    }
+};
+
+// The same for four blocks of tokens in a workgroup: their counts become the places among the four of each block's first
+// token, and totals [groups of four][bins] holds the four's counts.  Each workgroup of the scatter adds up the totals
+// before its own by itself: a launch less, worth it while they read few counts in all (EX_READS).  Gradients of rows of 8, in a
+// graph: 300,000 tokens of 8,192 rows (2.7 million counts read) 45.7 -> 42.6 us, 100,000 of 65,536 (4.9) 40.0 -> 38.4, 500,000 of
+// 8,192 (7.7) 50.9 -> 49.7, 300,000 of 65,536 (11) 53.2 -> 53.6, 1,000,000 of 8,192 (31) 68.2 -> 72.3.
+#define EX_READS (1 << 23)
+#define EX_TOTALS 40960                              // at most: groups of four of 256 blocks and 512 bins read 2^23 of them
+template <bool FIRST>
+struct EmHist4 {
+    static const int threads = 4 * EX_THREADS;
+    EmSort a;
+    __device__ __forceinline__ void run(int block) const {
+        __shared__ uint32_t h[4][EX_BINS];
+        const int bins = 1 << a.bits, sub = threadIdx.x / EX_THREADS, own = 4 * block + sub;
+        for (int d = threadIdx.x; d < 4 * EX_BINS; d += threads) (&h[0][0])[d] = 0;
+        __syncthreads();
+        if (own < a.nblocks) {
+            const int begin = own * a.per_block, end = min(begin + a.per_block, a.tokens);
+            for (int i = begin + threadIdx.x % EX_THREADS; i < end; i += EX_THREADS) atomicAdd(&h[sub][(ex_key<FIRST>(a, i) >> a.shift) & a.mask], 1u);
+        }
+        __syncthreads();
+        for (int d = threadIdx.x; d < bins; d += threads) {
+            uint32_t sum = 0;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                if (4 * block + k < a.nblocks) a.hist[(size_t)(4 * block + k) * bins + d] = sum;
+                sum += h[k][d];
+            }
+            a.totals[(size_t)block * bins + d] = sum;
+        }
     }
 };
 
@@ -468,9 +501,40 @@ struct EmScatter {
             uint32_t total;
             const int d = 2 * threadIdx.x;
             const bool in0 = d < bins, in1 = d + 1 < bins;
-            const uint32_t t0 = in0 ? a.totals[d] : 0u, t1 = in1 ? a.totals[d + 1] : 0u;
-            const uint32_t h0 = in0 ? a.hist[(size_t)block * bins + d] : 0u;
-            const uint32_t h1 = in1 ? a.hist[(size_t)block * bins + d + 1] : 0u;
+            uint32_t t0 = 0, t1 = 0, h0 = 0, h1 = 0;
+            if (a.ngroups) {
+                // two digits to a thread; where there are fewer than 512, several threads to the two divide the groups
+                static_assert(sizeof(ordered) >= EX_THREADS * sizeof(uint4), "a sum of each thread");
+                uint4* part = (uint4*)ordered;
+                const int pairs = bins / 2, apart = EX_THREADS / pairs, q = threadIdx.x % pairs;
+                uint4 sum = make_uint4(0, 0, 0, 0);
+#pragma unroll 8
+                for (int g = threadIdx.x / pairs; g < a.ngroups; g += apart) {
+                    const uint2 c = ((const uint2*)a.totals)[(size_t)g * pairs + q];
+                    sum.x += c.x;
+                    sum.y += c.y;
+                    if (g < block / 4) {
+                        sum.z += c.x;
+                        sum.w += c.y;
+                    }
+                }
+                part[threadIdx.x] = sum;
+                __syncthreads();
+                if (in0) {
+                    for (int k = 0; k < apart; ++k) {
+                        const uint4 c = part[threadIdx.x + k * pairs];
+                        t0 += c.x;
+                        t1 += c.y;
+                        h0 += c.z;
+                        h1 += c.w;
+                    }
+                }
+            } else {
+                t0 = in0 ? a.totals[d] : 0u;
+                t1 = in1 ? a.totals[d + 1] : 0u;
+            }
+            if (in0) h0 += a.hist[(size_t)block * bins + d];
+            if (in1) h1 += a.hist[(size_t)block * bins + d + 1];
             const uint32_t base = ex_scan(t0 + t1, wsum, total);
             running[d] = base + h0;
             running[d + 1] = base + t0 + h1;
@@ -846,7 +910,7 @@ static EmSortPlan em_sort_plan(long long tokens) {
     const bool radix = tokens > ER_MAX_TOKENS, buckets = tokens > ER_DIRECT && !radix;
     p.other = take(radix || buckets ? tokens * 8 : 0);
     p.hist = take(radix ? (size_t)EX_BINS * EX_MAX_BLOCKS * 4 : buckets ? (size_t)EB_STARTS * (ER_MAX_TOKENS / EB_LIST) * 4 : 0);
-    p.totals = take(radix ? EX_BINS * 4 : 0);
+    p.totals = take(radix ? EX_TOTALS * 4 : 0);
     p.bytes = at;
     return p;
 }
@@ -948,10 +1012,15 @@ static int em_sort(const EmIds& in, uint2* sorted, char* ws, const EmPart* looku
     k.ids = in; k.tokens = tokens;
     k.per_block = (int)per_block; k.nblocks = (int)blocks;
     k.hist = (uint32_t*)(ws + p.hist); k.totals = (uint32_t*)(ws + p.totals);
+    const long long ngroups = (blocks + 3) / 4;
+    const int most_bits = (key_bits + passes - 1) / passes;
+    const long long counts = ngroups << most_bits;
+    k.ngroups = counts <= EX_TOTALS && counts * blocks <= EX_READS ? (int)ngroups : 0;
     // The lookup goes where workgroups wait most, and in large parts (a part takes 2 us at least): to the scatters, and a little
-    // of it to the scans, which leave most of the chip idle.  Sort and lookup of 300,000 tokens of 48 floats 37.5 us and of
-    // 2,000,000 152 (one after the other 43 and 163; all of it in the scatters 40 and 153; the same in every launch 41 and 164).
-    const int with_scan = 1, with_scatter = 5;
+    // of it to the scans, which leave most of the chip idle.  Sort and lookup of 2,000,000 tokens of 48 floats 152 us (one after
+    // the other 163, all of it in the scatters 153, the same in every launch 164); without scans, of 300,000 tokens 33 us (a
+    // quarter of it in the counts 36; with scans 37, with scans and one after the other 43).
+    const int with_scan = k.ngroups ? 0 : 1, with_scatter = 5;
     steps.whole = (with_scan + with_scatter) * passes;
     for (int pass = 0; pass < passes; ++pass) {
         k.bits = (key_bits - k.shift + passes - pass - 1) / (passes - pass);           // the remaining bits, evenly
@@ -960,8 +1029,12 @@ static int em_sort(const EmIds& in, uint2* sorted, char* ws, const EmPart* looku
         k.out = to_first ? sorted : (uint2*)(ws + p.other);
         k.in = to_first ? (const uint2*)(ws + p.other) : sorted;
         const int n = (int)blocks;
-        EM_RUN(pass == 0 ? steps.run(EmHist<true>{k}, n, 0) : steps.run(EmHist<false>{k}, n, 0));
-        EM_RUN(steps.run(EmScan{k.hist, k.totals, k.nblocks, 1 << k.bits}, ((1 << k.bits) + 31) / 32, with_scan));
+        if (k.ngroups) {
+            EM_RUN(pass == 0 ? steps.run(EmHist4<true>{k}, k.ngroups, 0) : steps.run(EmHist4<false>{k}, k.ngroups, 0));
+        } else {
+            EM_RUN(pass == 0 ? steps.run(EmHist<true>{k}, n, 0) : steps.run(EmHist<false>{k}, n, 0));
+            EM_RUN(steps.run(EmScan{k.hist, k.totals, k.nblocks, 1 << k.bits}, ((1 << k.bits) + 31) / 32, with_scan));
+        }
         if (pass == 0) EM_RUN(ipl == 2 ? steps.run(EmScatter<true, 2>{k}, n, with_scatter) : ipl == 4 ? steps.run(EmScatter<true, 4>{k}, n, with_scatter) : steps.run(EmScatter<true, 8>{k}, n, with_scatter));
         else EM_RUN(ipl == 2 ? steps.run(EmScatter<false, 2>{k}, n, with_scatter) : ipl == 4 ? steps.run(EmScatter<false, 4>{k}, n, with_scatter) : steps.run(EmScatter<false, 8>{k}, n, with_scatter));
         k.shift += k.bits;

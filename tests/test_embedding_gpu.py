@@ -364,7 +364,7 @@ def test_refusals_on_the_device():
 
 
 @pytest.mark.parametrize("tokens, rows, dim", [(128, 40, 7), (129, 40, 3), (2000, 17, 5), (4096, 300, 8), (4097, 300, 2), (9000, 5000, 4100),
-                                               (16384, 40000, 33), (16385, 40000, 1), (70001, 90, 48), (300000, 8192, 12), (600001, 300000, 3)])
+                                               (16384, 40000, 33), (16385, 40000, 1), (70001, 90, 48), (300000, 8192, 12), (600001, 300000, 3), (20000, 1, 3)])
 @pytest.mark.parametrize("dtype, idt", [(torch.float32, torch.int32), (torch.bfloat16, torch.int64), (torch.float16, torch.int32)])
 def test_lookup_that_sorts_for_its_gradient(tokens, rows, dim, dtype, idt):
     """A lookup that is recorded sorts the tokens beside its own work: the output and the gradient have the bits of the plain
