@@ -16,11 +16,9 @@
 #include <type_traits>
 
 #define AW_MAX 40                                // tensors whose records fill 4 KB of kernel arguments
-// Blocks of 256 per wave, and elements per workgroup of four waves.  One block with float32 moments (97 bfloat16 tensors:
-// 203 us, 213 with two, 232 with four), two with 8-bit ones (2,000,000 Gaussians: 405 us, 418 with one, 405 with four; 211
-// bfloat16 tensors 157, 157, 198).
-static constexpr int aw_blocks(bool eight) { return eight ? 2 : 1; }
-static constexpr int aw_per_group(bool eight) { return 4 * 256 * aw_blocks(eight); }
+// Elements of a workgroup: four waves have a block of 256 each.  With two blocks a wave the step over 97 bfloat16 tensors takes
+// 209 us, not 202, the one over 2,000,000 Gaussians with 8-bit moments and their read-out 527, not 513.
+#define AW_PER_GROUP (4 * M8_BLOCK)
 
 struct AwTensor {
     void* p; const void* g; void* m; void* v;
@@ -44,8 +42,8 @@ static_assert(sizeof(AwStep) + sizeof(AwPart<AwTensor, AW_MAX>) <= 4096, "kernel
 
 // Where the records of a launch lie: in its arguments, or (more tensors than two launches' arguments hold) in a table in
 // device memory that small launches before it have filled from theirs.  211 bfloat16 tensors with 8-bit moments and the
-// conversion of these: 244 us in six launches and five, 199 in one each and as many that fill; 97 bfloat16 tensors 198 us
-// in three launches, 199 in one and three that fill.
+// conversion of these: 250 us in six launches and five, 208 in one each and as many that fill (2 us each); 97 bfloat16 tensors
+// 204 us in three launches, 203 in one and three that fill.
 template <class Record, int MAX>
 struct AwInArgs {
     AwPart<Record, MAX> part;
@@ -199,7 +197,7 @@ __device__ __forceinline__ float aw_exact(float w, float m, float v, const AwSte
 }
 
 // The tensor that workgroup `b` works on (scalar; six steps for 40 tensors.  Comparing with every start is more work than
-// the waiting it saves: 405 -> 436 us for the 8-bit step over 2,000,000 Gaussians, a lane each through vector loads 413.)
+// the waiting it saves: 8 % for the 8-bit step over 2,000,000 Gaussians, a lane each through vector loads 2 %.)
 template <class Ints>
 __device__ __forceinline__ int aw_find(Ints start, int num, int b) {
     int lo = 0, hi = num;
@@ -427,25 +425,18 @@ adamw_kernel(AwStep k, Source source) {
     const int ti = aw_find(source.starts(), source.num(), (int)blockIdx.x);
     const AwTensor& t = source.record(ti);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    constexpr int AW_BLOCKS = aw_blocks(EIGHT);
-    const long long base = (long long)((int)blockIdx.x - source.starts()[ti]) * aw_per_group(EIGHT) + wave * (AW_BLOCKS * M8_BLOCK);
-    AwLane<BF16, EIGHT> x[AW_BLOCKS];
-    if (base + AW_BLOCKS * M8_BLOCK <= t.n) {    // whole blocks: all loads before the first use
-#pragma unroll
-        for (int u = 0; u < AW_BLOCKS; ++u) aw_load<BF16, EIGHT, true>(t, base + u * M8_BLOCK, 4, x[u]);
-#pragma unroll
-        for (int u = 0; u < AW_BLOCKS; ++u) aw_finish<BF16, EIGHT, true>(k, t, base + u * M8_BLOCK, 4, x[u]);
+    const long long block = (long long)((int)blockIdx.x - source.starts()[ti]) * AW_PER_GROUP + wave * M8_BLOCK;
+    AwLane<BF16, EIGHT> x;
+    if (block + M8_BLOCK <= t.n) {
+        aw_load<BF16, EIGHT, true>(t, block, 4, x);
+        aw_finish<BF16, EIGHT, true>(k, t, block, 4, x);
         return;
     }
-#pragma unroll 1
-    for (int u = 0; u < AW_BLOCKS; ++u) {
-        const long long b = base + u * M8_BLOCK;
-        if (b >= t.n) return;
-        const long long left = t.n - (b + 4 * (threadIdx.x & 63));
-        const int valid = left >= 4 ? 4 : left > 0 ? (int)left : 0;
-        aw_load<BF16, EIGHT, false>(t, b, valid, x[0]);
-        aw_finish<BF16, EIGHT, false>(k, t, b, valid, x[0]);
-    }
+    if (block >= t.n) return;
+    const long long left = t.n - (block + 4 * (threadIdx.x & 63));
+    const int valid = left >= 4 ? 4 : left > 0 ? (int)left : 0;
+    aw_load<BF16, EIGHT, false>(t, block, valid, x);
+    aw_finish<BF16, EIGHT, false>(k, t, block, valid, x);
 }
 
 extern "C" int fdgs_adamw_step(const fdgs_adamw_args* a, void* stream) {
@@ -454,14 +445,13 @@ extern "C" int fdgs_adamw_step(const fdgs_adamw_args* a, void* stream) {
     if (!bf16 && a->param_type != FDGS_TYPE_F32) return FDGS_EINVAL;
     if (!eight && a->state_bits != 32) return FDGS_EINVAL;
     if (!(a->beta1 >= 0.0 && a->beta1 < 1.0 && a->beta2 >= 0.0 && a->beta2 < 1.0 && a->eps >= 0.0)) return FDGS_EINVAL;
-    const int per_group = aw_per_group(eight);
     long long total = 0;                         // workgroups
     for (int i = 0; i < a->num_tensors; ++i) {   // all of them before the first launch: no step is half done
         const fdgs_adamw_tensor& s = a->tensors[i];
         if (s.numel < 0 || s.step < 1 || s.grad_row_len < 0) return FDGS_EINVAL;
         if (s.grad_row_len > 0 && s.grad_row_stride < s.grad_row_len) return FDGS_EINVAL;
         if (s.numel == 0) continue;
-        total += (s.numel - 1) / per_group + 1;
+        total += (s.numel - 1) / AW_PER_GROUP + 1;
         if (total > 0x7fffffffLL) return FDGS_ETOOLARGE;
         if (!s.param || !s.grad || !s.exp_avg || !s.exp_avg_sq || (bf16 && !s.residual)) return FDGS_EINVAL;
         if (eight && (!s.exp_avg_exponents || !s.exp_avg_sq_exponents)) return FDGS_EINVAL;
@@ -476,7 +466,7 @@ extern "C" int fdgs_adamw_step(const fdgs_adamw_args* a, void* stream) {
         while (i < a->num_tensors && a->tensors[i].numel == 0) ++i;
         if (i == a->num_tensors) return false;
         const fdgs_adamw_tensor& s = a->tensors[i++];
-        groups = (int)((s.numel + per_group - 1) / per_group);
+        groups = (int)((s.numel + AW_PER_GROUP - 1) / AW_PER_GROUP);
         t.p = s.param; t.g = s.grad; t.m = s.exp_avg; t.v = s.exp_avg_sq;
         t.low = s.residual; t.me = s.exp_avg_exponents; t.ve = s.exp_avg_sq_exponents;
         t.n = s.numel; t.gstride = s.grad_row_stride; t.glen = s.grad_row_len;
