@@ -16,9 +16,10 @@
 #include <type_traits>
 
 #define AW_MAX 40                                // tensors whose records fill 4 KB of kernel arguments
-// Elements of a workgroup: four waves have a block of 256 each.  With two blocks a wave the step over 97 bfloat16 tensors takes
-// 209 us, not 202, the one over 2,000,000 Gaussians with 8-bit moments and their read-out 527, not 513.
-#define AW_PER_GROUP (4 * M8_BLOCK)
+// A wave has one block (with two the step over 2,000,000 Gaussians with 8-bit moments, and their read-out, takes 527 us, not 513),
+// a workgroup eight of them (97 bfloat16 tensors: 194 us, 202 with four, 193 with sixteen, with which 8-bit moments lose 3 %).
+#define AW_THREADS 512
+#define AW_PER_GROUP (AW_THREADS / 64 * M8_BLOCK)
 
 struct AwTensor {
     void* p; const void* g; void* m; void* v;
@@ -420,7 +421,7 @@ __device__ __forceinline__ void aw_finish(const AwStep& k, const AwTensor& t, lo
 }
 
 template <bool BF16, bool EIGHT, class Source>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(AW_THREADS)
 adamw_kernel(AwStep k, Source source) {
     const int ti = aw_find(source.starts(), source.num(), (int)blockIdx.x);
     const AwTensor& t = source.record(ti);
@@ -479,7 +480,7 @@ extern "C" int fdgs_adamw_step(const fdgs_adamw_args* a, void* stream) {
     hipStream_t st = (hipStream_t)stream;
     auto launch = [&](const auto& source, int blocks) {
         typedef std::remove_cv_t<std::remove_reference_t<decltype(source)>> Source;
-        const dim3 grid((unsigned)blocks), threads(256);
+        const dim3 grid((unsigned)blocks), threads(AW_THREADS);
         if (bf16 && eight) hipLaunchKernelGGL((adamw_kernel<true, true, Source>), grid, threads, 0, st, k, source);
         else if (bf16) hipLaunchKernelGGL((adamw_kernel<true, false, Source>), grid, threads, 0, st, k, source);
         else if (eight) hipLaunchKernelGGL((adamw_kernel<false, true, Source>), grid, threads, 0, st, k, source);
