@@ -448,3 +448,31 @@ def test_conversions_refuse_overlapping_results():
     with pytest.raises(ValueError, match="one value"):
         pack8([torch.ones(4, device="cuda")], True, keys=[1, 2])
     assert isinstance(ms[0], Moment8)
+
+
+@pytest.mark.parametrize("count", [3, 200])
+def test_captured_conversions(count):
+    """Values to codes and back in a graph (its records in the launch's arguments, or in a table that the graph fills again at
+    every replay), replayed with new values and with eager conversions of other lists in between."""
+    from fdgs.adamw import pack8, unpack8
+    gen = torch.Generator().manual_seed(count)
+    sizes = [int(n) for n in torch.randint(0, 900, (count,), generator=gen)]
+    x = [torch.zeros(n, device="cuda") for n in sizes]
+    signed = [i % 2 == 0 for i in range(count)]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ms = pack8(x, signed)
+        back = unpack8(ms)
+    for k in range(3):
+        new = [torch.randn(n, generator=gen).abs() * 10.0 ** (k - 1) for n in sizes]
+        for a, b in zip(x, new):
+            a.copy_(b)
+        graph.replay()
+        other = unpack8(pack8([v.cuda() + 1 for v in new], signed))      # eager, from a table of its own
+        want = unpack8(pack8(x, signed))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(back, want)), k
+        for v, m, s, b in zip(new, ms, signed, back):
+            codes, exps = ac.encode(v.numpy(), 0x8000, s)
+            assert np.array_equal(m.codes.cpu().numpy(), codes) and np.array_equal(m.exponents.cpu().numpy(), exps)
+        del other
