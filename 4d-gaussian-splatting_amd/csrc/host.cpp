@@ -5,6 +5,7 @@
 // about 0.3 us a tensor.  Every check raises the Python exception that a caller sees.
 // The lookup of one token takes the GPU 4 us; its checks, output and call take 12 from Python, its training pass 130.
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <ATen/ATen.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
@@ -13,6 +14,7 @@
 #include <cstring>
 #include <stdexcept>
 #include <string>
+#include <unordered_set>
 #include <vector>
 #include "fdgs.h"
 
@@ -499,17 +501,30 @@ int64_t padding_of(PyObject* o) {
 }
 
 // A backward pass that is captured while a graph of the same leaf made on another stream lives waits for that stream, from
-// autograd's own thread, where the error that the capture makes of it ends the process.  Refused here, where it can be.
+// autograd's own thread, where the error that the capture makes of it ends the process.  Refused here, where it can be: the
+// leaves that the table was made of are looked up, while a capture runs.
 void capture_alone(const Tensor& table) {
-    if (!table.is_leaf()) return;
     const c10::DeviceGuard guard(table.device());
     if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
-    const auto node = torch::autograd::impl::try_get_grad_accumulator(table);
-    if (!node) return;
-    const auto made_on = node->stream();
-    if (made_on.has_value() && made_on->id() == c10::hip::getCurrentHIPStream(table.device().index()).id()) return;
-    throw Refused{PyExc_RuntimeError, "embedding: an autograd graph of this table from outside the capture is alive; delete its "
-                                      "outputs before capturing a pass that wants gradients"};
+    const auto stream = c10::hip::getCurrentHIPStream(table.device().index());
+    std::vector<torch::autograd::Node*> next;
+    std::unordered_set<torch::autograd::Node*> seen;
+    const auto of_leaf = table.is_leaf() ? torch::autograd::impl::try_get_grad_accumulator(table) : nullptr;
+    if (of_leaf) next.push_back(of_leaf.get());
+    if (!table.is_leaf()) next.push_back(table.grad_fn().get());
+    while (!next.empty()) {
+        torch::autograd::Node* node = next.back();
+        next.pop_back();
+        if (!seen.insert(node).second) continue;
+        if (dynamic_cast<torch::autograd::AccumulateGrad*>(node)) {
+            const auto made_on = node->stream();
+            if (!made_on.has_value() || made_on->id() != stream.id())
+                throw Refused{PyExc_RuntimeError, "embedding: an autograd graph of this table from outside the capture is alive; delete "
+                                                  "its outputs before capturing a pass that wants gradients"};
+        }
+        for (const auto& e : node->next_edges())
+            if (e.function) next.push_back(e.function.get());
+    }
 }
 
 // A tensor here would lose its gradient without a word.

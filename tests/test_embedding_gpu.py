@@ -393,3 +393,27 @@ def test_ids_that_change_after_the_lookup_are_noticed():
     ids.zero_()
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.sum().backward()
+
+
+def test_capture_beside_a_living_eager_graph_of_a_leaf_behind_the_table():
+    from fdgs.embedding import embedding
+    ids = torch.tensor([1, 0, 1], device="cuda")
+    leaf = torch.randn(2, 8, device="cuda", requires_grad=True)
+    eager = leaf * 2
+    first = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(first):
+        with pytest.raises(RuntimeError, match="outside the capture"):
+            embedding(ids, (leaf + 1).bfloat16())
+        plain = embedding(ids, (leaf + 1).detach())
+    first.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(plain, (leaf + 1)[ids])
+    del eager
+    second = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(second):
+        y = embedding(ids, 3 * leaf)
+        grad, = torch.autograd.grad(y, leaf, torch.ones_like(y))
+    for _ in range(3):
+        second.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, (3 * leaf)[ids].detach()) and torch.equal(grad, torch.tensor([3.0, 6.0], device="cuda")[:, None].expand(2, 8))
