@@ -84,7 +84,7 @@ struct Written {
     std::vector<std::pair<uintptr_t, size_t>> pieces;
     void add(const void* p, size_t bytes) { if (bytes) pieces.emplace_back((uintptr_t)p, bytes); }
     void check() {
-        std::sort(pieces.begin(), pieces.end());
+        std::sort(pieces.begin(), pieces.end(), [](const auto& a, const auto& b) { return a.first < b.first; });
         for (size_t i = 1; i < pieces.size(); ++i)
             if (pieces[i - 1].first + pieces[i - 1].second > pieces[i].first) value_error("a tensor is in the lists twice, or two of them overlap");
     }

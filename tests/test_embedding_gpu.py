@@ -417,3 +417,28 @@ def test_capture_beside_a_living_eager_graph_of_a_leaf_behind_the_table():
         second.replay()
         torch.cuda.synchronize()
         assert torch.equal(y, (3 * leaf)[ids].detach()) and torch.equal(grad, torch.tensor([3.0, 6.0], device="cuda")[:, None].expand(2, 8))
+
+
+def test_a_table_of_very_many_rows():
+    """Keys of 28 bits: four digits.  Rows of one element, nearly all of them without a token."""
+    from fdgs.embedding import embedding, embedding_grad
+    rows, tokens = (1 << 27) + 5, 20000
+    gen = torch.Generator().manual_seed(0)
+    ids = torch.randint(0, rows, (tokens,), generator=gen)
+    ids[:5000] = ids[5000]
+    ids[5000:5003] = torch.tensor([rows - 1, 0, rows])           # the last one's is beyond the table
+    gy = torch.randn(tokens, 1, generator=gen).half()
+    got = embedding_grad(gy.cuda(), ids.cuda(), rows)
+    there = ids < rows
+    where, index = torch.unique(ids[there], return_inverse=True)
+    want = torch.zeros(len(where), dtype=torch.float64).index_add_(0, index, gy[there, 0].double())
+    size = torch.zeros(len(where), dtype=torch.float64).index_add_(0, index, gy[there, 0].double().abs())
+    many = torch.bincount(index).double()
+    # a sum of n terms in float32, then half a step of float16
+    off = (got.cpu()[where, 0].double() - want).abs()
+    assert (off <= many * 2.0 ** -24 * size + 2.0 ** -11 * want.abs() * 1.001 + 2.0 ** -25).all()
+    assert int(got.count_nonzero()) == int((want.half() != 0).sum())
+    table = torch.zeros(rows, 1, dtype=torch.float16, device="cuda", requires_grad=True)
+    y = embedding(ids.cuda(), table)
+    again, = torch.autograd.grad(y, table, gy.cuda())
+    assert torch.equal(again, got) and int(y.isnan().sum()) == int((~there).sum())
