@@ -180,8 +180,7 @@ embedding_step_kernel(Step step, int blocks, int period, EmPart part) {
 }
 
 #define ER_THREADS 256
-#define ER_DIRECT 4096                               // up to here in one launch; beyond, by buckets:
-#define ER_MAX_TOKENS 16384                          // beyond, T^2 comparisons of equal ids would take long
+#define ER_TOKENS 768                                // a sort by digits takes so long for each of its passes (at most four)
 
 struct EmIds {
     const void* ids;
@@ -196,7 +195,7 @@ struct EmRank {
     EmIds in;
     uint2* sorted;
     __device__ __forceinline__ void run(int block) const {
-        __shared__ __align__(16) uint32_t sk[ER_DIRECT];
+        __shared__ __align__(16) uint32_t sk[4 * ER_TOKENS];
         __shared__ uint32_t part[4][64];
         const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, tokens = in.tokens;
         const int own = block * 64;             // first token of the workgroup
@@ -231,132 +230,141 @@ struct EmRank {
     }
 };
 
-// More: every workgroup puts 4096 tokens into 2048 buckets by the upper bits of their keys, in LDS and in no particular
-// order, which makes a list of each 4096; then a token's place is counted among the tokens of its bucket alone (and of those
-// that the same 64 places touch) in every list, by key and then by token, a wave for a list.  T^2 comparisons remain only
-// where most tokens have one id.  At 16,384 tokens of 65,536 rows, a frequent one among them and a fifth of the tokens without a
-// row, 16 us; with one list of all tokens 22, against all tokens without buckets 68.
-#define EB_THREADS 1024
-#define EB_LIST 4096
-#define EB_PER (EB_LIST / EB_THREADS)
-#define EB_BUCKETS 2048
-#define EB_STARTS (EB_BUCKETS + 1)                   // where a list's buckets start, and where its last one ends
+// More: a workgroup sorts 4096 tokens in LDS, by digits of at most 9 bits from the lowest on.  Several such lists are merged by
+// search: a token's place is its place in its own list and, in each other one, the number of tokens that come before it,
+// those of equal keys among them where that list lies before its own.  Both launches take the same time whatever the ids
+// are.  (Lists in buckets of neighbouring keys, whose tokens are compared with each other, make the gradient of 16,384 tokens of
+// 65,536 rows of 8 21 us, not 31, where the ids are even, 71, not 34, where a few have most of the tokens, and 115, not 33,
+// where one has all.)
+#define EL_THREADS 1024
+#define EL_WAVES (EL_THREADS / 64)
+#define EL_TOKENS 4096
+#define EL_PER (EL_TOKENS / EL_THREADS)
+#define EL_LISTS 4
+#define EX_BITS 9
+#define EX_BINS (1 << EX_BITS)
 
-struct EmBucket {
-    static const int threads = EB_THREADS;
+// The lanes whose digit (of at most EX_BITS bits) is the lane's own, of those that are `ok`.
+__device__ __forceinline__ unsigned long long ex_peers(uint32_t d, int bits, bool ok) {
+    unsigned long long peers = __ballot(ok);
+#pragma unroll
+    for (int b = 0; b < EX_BITS; ++b) {
+        if (b < bits) {
+            const unsigned long long bal = __ballot((d >> b) & 1u);
+            peers &= ((d >> b) & 1u) ? bal : ~bal;
+        }
+    }
+    return peers;
+}
+
+struct EmList {
+    static const int threads = EL_THREADS;
     EmIds in;
-    int shift;
-    uint2* __restrict__ lists;
-    uint32_t* __restrict__ starts;
+    int key_bits, passes;
+    uint2* lists;
     __device__ __forceinline__ void run(int block) const {
-        __shared__ uint2 ordered[EB_LIST];
-        __shared__ uint32_t count[EB_BUCKETS], wsum[EB_THREADS / 64], without;
+        __shared__ uint2 ordered[EL_TOKENS];
+        __shared__ __align__(16) uint16_t cnt[EL_WAVES][EX_BINS];    // a wave's count of each digit, then where its first one lies
+        __shared__ uint32_t wsum[EX_BINS / 64];
         const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-        const int from = block * EB_LIST, have = min(in.tokens - from, EB_LIST);
-        const uint32_t rows = in.rows;
-        uint32_t* start = starts + block * EB_STARTS;
-        count[threadIdx.x] = 0;
-        count[threadIdx.x + EB_THREADS] = 0;
-        uint32_t key[EB_PER], slot[EB_PER];
+        const int from = block * EL_TOKENS, have = min(in.tokens - from, EL_TOKENS);
+        const int at = wave * (64 * EL_PER) + lane;
+        const unsigned long long below = lane == 0 ? 0ull : (~0ull >> (64 - lane));
+        uint2 e[EL_PER];
 #pragma unroll
-        for (int k = 0; k < EB_PER; ++k) {
-            const int i = threadIdx.x + k * EB_THREADS;
-            key[k] = i < have ? in.key(from + i) : 0xFFFFFFFFu;
+        for (int k = 0; k < EL_PER; ++k) {           // what is missing goes to the end: it has the largest key, and is last
+            const int i = at + 64 * k;
+            e[k] = i < have ? make_uint2(in.key(from + i), (uint32_t)(from + i)) : make_uint2(0xFFFFFFFFu, 0u);
         }
-        if (threadIdx.x == 0) without = 0;
-        __syncthreads();
-        // tokens without a row are not put in order: they go to the end, a wave's together (one count of all of them would
-        // take an LDS atomic each to the same word)
+        int shift = 0;
+        for (int pass = 0; pass < passes; ++pass) {
+            const int bits = (key_bits - shift + passes - pass - 1) / (passes - pass), bins = 1 << bits;
+            static_assert(sizeof(cnt) == EL_THREADS * sizeof(uint4), "cleared by one store a thread");
+            ((uint4*)cnt)[threadIdx.x] = make_uint4(0, 0, 0, 0);
+            __syncthreads();
+            uint32_t digit[EL_PER], rank[EL_PER];
 #pragma unroll
-        for (int k = 0; k < EB_PER; ++k) {
-            const unsigned long long none = __ballot(key[k] == rows);
-            uint32_t b = 0;
-            if (none && lane == 0) b = atomicAdd(&without, (uint32_t)__popcll(none));
-            b = (uint32_t)__builtin_amdgcn_readfirstlane((int)b);
-            slot[k] = key[k] == rows ? b + (uint32_t)__popcll(none & ((1ull << lane) - 1ull))
-                      : key[k] < rows ? atomicAdd(&count[key[k] >> shift], 1u) : 0u;
+            for (int k = 0; k < EL_PER; ++k) {
+                const uint32_t d = digit[k] = (e[k].x >> shift) & (uint32_t)(bins - 1);
+                const unsigned long long peers = ex_peers(d, bits, true);
+                const uint32_t first = (uint32_t)__popcll(peers & below), prev = cnt[wave][d];
+                rank[k] = prev + first;
+                if (first == 0) cnt[wave][d] = (uint16_t)(prev + (uint32_t)__popcll(peers));
+            }
+            __syncthreads();
+            uint32_t incl = 0, own = 0;
+            if (threadIdx.x < EX_BINS) {             // eight whole waves
+#pragma unroll
+                for (int w = 0; w < EL_WAVES; ++w) own += cnt[w][threadIdx.x];
+                incl = own;
+#pragma unroll
+                for (int d = 1; d < 64; d <<= 1) {
+                    const uint32_t o = __shfl_up(incl, d);
+                    if (lane >= d) incl += o;
+                }
+                if (lane == 63) wsum[wave] = incl;
+            }
+            __syncthreads();
+            if (threadIdx.x < EX_BINS) {
+                uint32_t g = incl - own;
+#pragma unroll
+                for (int w = 0; w < EX_BINS / 64; ++w) g += w < wave ? wsum[w] : 0u;
+#pragma unroll
+                for (int w = 0; w < EL_WAVES; ++w) {
+                    const uint32_t c = cnt[w][threadIdx.x];
+                    cnt[w][threadIdx.x] = (uint16_t)g;
+                    g += c;
+                }
+            }
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < EL_PER; ++k) ordered[cnt[wave][digit[k]] + rank[k]] = e[k];
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < EL_PER; ++k) e[k] = ordered[at + 64 * k];
+            shift += bits;
         }
-        __syncthreads();
-        const uint32_t c0 = count[2 * threadIdx.x], c1 = count[2 * threadIdx.x + 1];
-        uint32_t incl = c0 + c1;
 #pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const uint32_t o = __shfl_up(incl, d);
-            if (lane >= d) incl += o;
-        }
-        if (lane == 63) wsum[wave] = incl;
-        __syncthreads();
-        uint32_t base = 0;
-#pragma unroll
-        for (int w = 0; w < EB_THREADS / 64; ++w)
-            if (w < wave) base += wsum[w];
-        const uint32_t first = base + incl - c0 - c1, valid = (uint32_t)have - without;
-        count[2 * threadIdx.x] = first;
-        count[2 * threadIdx.x + 1] = first + c0;
-        start[2 * threadIdx.x] = first;
-        start[2 * threadIdx.x + 1] = first + c0;
-        if (threadIdx.x == 0) start[EB_BUCKETS] = valid;
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < EB_PER; ++k) {
-            const int i = threadIdx.x + k * EB_THREADS;
-            if (i < have) ordered[slot[k] + (key[k] == rows ? valid : count[key[k] >> shift])] = make_uint2(key[k], (uint32_t)(from + i));
-        }
-        __syncthreads();
-        for (int i = threadIdx.x; i < have; i += EB_THREADS) lists[from + i] = ordered[i];
+        for (int k = 0; k < EL_PER; ++k)
+            if (at + 64 * k < have) lists[from + at + 64 * k] = e[k];
     }
 };
 
-struct EmPlace {
-    static const int threads = ER_THREADS;
+struct EmMerge {
+    static const int threads = 1024;
     const uint2* __restrict__ lists;
-    const uint32_t* __restrict__ starts;
-    int tokens, nlists, shift;
-    uint32_t rows;
+    int tokens;
     uint2* __restrict__ sorted;
     __device__ __forceinline__ void run(int block) const {
-        __shared__ uint32_t part[4][64];
-        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-        const int own = block * 64, me = min(own + lane, tokens - 1);   // 64 places of one list
-        const uint2 mine2 = lists[me];
-        const uint32_t key = mine2.x;
-        const unsigned long long mine = ((unsigned long long)key << 32) | mine2.y;
-        // the buckets that the 64 places touch, the first one's and the last one's
-        const uint32_t kf = (uint32_t)__builtin_amdgcn_readfirstlane((int)key), kl = (uint32_t)__builtin_amdgcn_readlane((int)key, 63);
-        const int bf = kf == rows ? EB_BUCKETS : (int)(kf >> shift), bl = kl == rows ? EB_BUCKETS : (int)(kl >> shift) + 1;
-        uint32_t before = 0;
-        if (kf != rows) {
-            for (int l = wave; l < nlists; l += 4) {
-                const uint2* __restrict__ list = lists + (size_t)l * EB_LIST;
-                const int lo = (int)starts[l * EB_STARTS + bf], hi = (int)starts[l * EB_STARTS + bl];
-                before += (uint32_t)lo;                  // all of the list's smaller buckets
-                // the buckets themselves, 64 tokens at a time: a lane loads one, all lanes compare with each
-                for (int b = lo; b < hi; b += 64) {
-                    const uint2 other = b + lane < hi ? list[b + lane] : make_uint2(0xFFFFFFFFu, 0xFFFFFFFFu);
-#pragma unroll 16
-                    for (int q = 0; q < 64; ++q) {
-                        const uint32_t kq = (uint32_t)__builtin_amdgcn_readlane((int)other.x, q), tq = (uint32_t)__builtin_amdgcn_readlane((int)other.y, q);
-                        before += (((unsigned long long)kq << 32) | tq) < mine ? 1u : 0u;
-                    }
-                }
-            }
-        }
-        part[wave][lane] = before;
+        __shared__ uint32_t keys[EL_LISTS * EL_TOKENS];
+        const int i = block * threads + (int)threadIdx.x;
+        const uint2 mine = i < tokens ? lists[i] : make_uint2(0u, 0u);
+#pragma unroll 8
+        for (int j = threadIdx.x; j < EL_LISTS * EL_TOKENS; j += threads)
+            if (j < tokens) keys[j] = lists[j].x;
         __syncthreads();
-        if (wave == 0 && own + lane < tokens) {
-            uint32_t r = part[0][lane] + part[1][lane] + part[2][lane] + part[3][lane];
-            if (key == rows) {                           // behind all that have a row: list by list, as they lie
-                const int at = own / EB_LIST;
-                r = 0;
-                for (int l = 0; l < nlists; ++l) {
-                    const uint32_t valid = starts[l * EB_STARTS + EB_BUCKETS];
-                    r += valid;
-                    if (l < at) r += (uint32_t)EB_LIST - valid;
-                    if (l == at) r += (uint32_t)(me - at * EB_LIST) - valid;
-                }
+        if (i >= tokens) return;
+        const int own = i / EL_TOKENS;
+        int before[EL_LISTS];
+#pragma unroll
+        for (int l = 0; l < EL_LISTS; ++l) before[l] = 0;
+        // all lists step by step side by side: as many tokens come before as the largest sum of steps that reaches none behind
+#pragma unroll 1
+        for (int step = EL_TOKENS; step > 0; step >>= 1) {
+            uint32_t key[EL_LISTS];
+#pragma unroll
+            for (int l = 0; l < EL_LISTS; ++l) {
+                const int have = min(tokens - l * EL_TOKENS, EL_TOKENS), to = before[l] + step;
+                key[l] = to <= have ? keys[l * EL_TOKENS + to - 1] : 0xFFFFFFFFu;
             }
-            sorted[r] = mine2;
+#pragma unroll
+            for (int l = 0; l < EL_LISTS; ++l)
+                if (key[l] < mine.x + (l < own ? 1u : 0u)) before[l] += step;
         }
+        int place = i - own * EL_TOKENS;
+#pragma unroll
+        for (int l = 0; l < EL_LISTS; ++l) place += l == own ? 0 : before[l];
+        sorted[place] = mine;
     }
 };
 
@@ -364,8 +372,6 @@ struct EmPlace {
 // a pass: counts of each block of tokens, their scan, scatter.  2,000,000 tokens of 65,536 rows 43 us, 300,000 of 8,192 25 us.
 #define EX_THREADS 256
 #define EX_TILE(ipl) (EX_THREADS * (ipl))             // tokens that a workgroup takes at a time, ipl to a lane
-#define EX_BITS 9
-#define EX_BINS (1 << EX_BITS)
 #define EX_MAX_BLOCKS 1024
 
 struct EmSort {
@@ -563,14 +569,7 @@ struct EmScatter {
             for (int k = 0; k < EX_IPL; ++k) {
                 const bool ok = at + 64 * k < end;
                 const uint32_t d = (key[k] >> a.shift) & a.mask;
-                unsigned long long peers = __ballot(ok);  // lanes with the same digit
-#pragma unroll
-                for (int b = 0; b < EX_BITS; ++b) {
-                    if (b < a.bits) {
-                        const unsigned long long bal = __ballot((d >> b) & 1u);
-                        peers &= ((d >> b) & 1u) ? bal : ~bal;
-                    }
-                }
+                const unsigned long long peers = ex_peers(d, a.bits, ok);
                 const uint32_t first = (uint32_t)__popcll(peers & below);
                 const uint32_t prev = ok ? cnt[wave][d] : 0u;
                 rank[k] = prev + first;
@@ -800,7 +799,9 @@ embedding_walk_kernel(EmBwd a) {
 }
 
 // ---- rows that were cut: the partial sums of the shares from the row's first token on, in order ----
-#define EC_SCAN 4                                   // shares that a workgroup looks at, at least
+// A workgroup looks at as many shares as it has groups of lanes, 4 to 16: no more, because a row of more than 16 partial sums
+// takes all of it, and no two of those end within 16 shares (16,384 tokens of 100 rows of 8: 21 us, 42 with up to 256).
+#define EC_SCAN(groups) ((groups) < 4 ? 4 : (groups) > 16 ? 16 : (groups))
 #define EC_LONG (-2)                                 // more partial sums than two looks at the flags reach: 16
 
 template <class T, int VEC>
@@ -824,15 +825,15 @@ struct __attribute__((packed, aligned(1))) EmFlags8 { unsigned long long x; };
 template <class T, int VEC>
 __global__ void __launch_bounds__(EW_THREADS)
 embedding_join_kernel(EmBwd a) {
-    __shared__ int first_of[EW_THREADS], end_of[EW_THREADS];     // first and last share of the cut rows
-    __shared__ uint32_t row_of[EW_THREADS], count;
+    __shared__ int first_of[EC_SCAN(EW_THREADS)], end_of[EC_SCAN(EW_THREADS)];     // first and last share of the cut rows
+    __shared__ uint32_t row_of[EC_SCAN(EW_THREADS)], count;
     __shared__ float sums[EW_THREADS * VEC];
     const int lane = threadIdx.x & 63;
     const int group = threadIdx.x / a.lanes;
     const int c = blockIdx.y * a.lanes + (int)threadIdx.x - group * a.lanes;
     const bool in = group < a.groups && c < a.nv;
     const int col = in ? em_col<VEC>(c, a.nv, a.dim) : 0;
-    const int scan = max(a.groups, EC_SCAN);
+    const int scan = EC_SCAN(a.groups);
     if (threadIdx.x == 0) count = 0;
     __syncthreads();
     const int s = blockIdx.x * scan + (int)threadIdx.x;
@@ -877,7 +878,7 @@ embedding_join_kernel(EmBwd a) {
             lo += (less - 1) * step + 1;
         }
         const int first = (int)(((long long)lo + (long long)row) / a.share);
-        const int each = (end - first + a.groups - 1) / a.groups;
+        const int each = (end - first + a.groups - 1) / a.groups, used = (end - first + each - 1) / each;
         float acc[VEC];
 #pragma unroll
         for (int j = 0; j < VEC; ++j) acc[j] = 0.0f;
@@ -891,7 +892,7 @@ embedding_join_kernel(EmBwd a) {
         for (int j = 0; j < VEC; ++j) sums[threadIdx.x * VEC + j] = acc[j];
         __syncthreads();
         if (in && group == 0) {
-            for (int q = 1; q < a.groups; ++q)
+            for (int q = 1; q < used; ++q)
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) acc[j] += sums[(threadIdx.x + q * a.lanes) * VEC + j];
             ec_add<VEC>(a.head + (long long)end * a.dim + col, acc);
@@ -907,9 +908,9 @@ static EmSortPlan em_sort_plan(long long tokens) {
     EmSortPlan p;
     size_t at = 0;
     auto take = [&at](size_t n) { const size_t o = at; at += (n + 255) / 256 * 256; return o; };
-    const bool radix = tokens > ER_MAX_TOKENS, buckets = tokens > ER_DIRECT && !radix;
-    p.other = take(radix || buckets ? tokens * 8 : 0);
-    p.hist = take(radix ? (size_t)EX_BINS * EX_MAX_BLOCKS * 4 : buckets ? (size_t)EB_STARTS * (ER_MAX_TOKENS / EB_LIST) * 4 : 0);
+    const bool radix = tokens > EL_TOKENS;
+    p.other = take(radix ? tokens * 8 : 0);
+    p.hist = take(radix ? (size_t)EX_BINS * EX_MAX_BLOCKS * 4 : 0);
     p.totals = take(radix ? EX_TOTALS * 4 : 0);
     p.bytes = at;
     return p;
@@ -992,17 +993,15 @@ static int em_sort(const EmIds& in, uint2* sorted, char* ws, const EmPart* looku
     }
     int key_bits = 1;
     while (key_bits < 31 && (1ll << key_bits) <= (long long)in.rows) ++key_bits;       // keys 0 .. rows
-    if (tokens <= ER_DIRECT) return steps.run(EmRank{in, sorted}, (tokens + 63) / 64, 1);
-    if (tokens <= ER_MAX_TOKENS) {
-        const int shift = key_bits > 11 ? key_bits - 11 : 0, nlists = (tokens + EB_LIST - 1) / EB_LIST;
-        static_assert(EB_BUCKETS == 1 << 11 && EB_BUCKETS == 2 * EB_THREADS, "buckets of the upper 11 bits, two to a thread");
-        uint2* lists = (uint2*)(ws + p.other);
-        uint32_t* starts = (uint32_t*)(ws + p.hist);
-        steps.whole = 2;
-        EM_RUN(steps.run(EmBucket{in, shift, lists, starts}, nlists, 1));
-        return steps.run(EmPlace{lists, starts, tokens, nlists, shift, in.rows, sorted}, (tokens + 63) / 64, 1);
-    }
     const int passes = (key_bits + EX_BITS - 1) / EX_BITS;
+    if (tokens <= ER_TOKENS * passes) return steps.run(EmRank{in, sorted}, (tokens + 63) / 64, 1);
+    if (tokens <= EL_TOKENS) return steps.run(EmList{in, key_bits, passes, sorted}, 1, 1);
+    if (tokens <= EL_LISTS * EL_TOKENS && passes > 1) {
+        uint2* lists = (uint2*)(ws + p.other);
+        steps.whole = 2;
+        EM_RUN(steps.run(EmList{in, key_bits, passes, lists}, (tokens + EL_TOKENS - 1) / EL_TOKENS, 1));
+        return steps.run(EmMerge{lists, tokens, sorted}, (tokens + EmMerge::threads - 1) / EmMerge::threads, 1);
+    }
     // a workgroup's tile takes 5 us whatever its length: short tiles while there are workgroups to be had for them
     const int ipl = tokens <= EX_MAX_BLOCKS * EX_TILE(2) / 2 ? 2 : tokens <= EX_MAX_BLOCKS * EX_TILE(4) ? 4 : 8;
     long long tiles = ((long long)tokens + EX_TILE(ipl) - 1) / EX_TILE(ipl), blocks = tiles < EX_MAX_BLOCKS ? tiles : EX_MAX_BLOCKS;
@@ -1099,7 +1098,7 @@ static int em_bwd_launch(const EmBwd& k, const EmPlan& p, hipStream_t s) {
     const int tiles = (p.nv + 63) / 64;
     j.lanes = (p.nv + tiles - 1) / tiles;
     j.groups = EW_THREADS / j.lanes;
-    const int scan = j.groups > EC_SCAN ? j.groups : EC_SCAN;
+    const int scan = EC_SCAN(j.groups);
     const dim3 joins((unsigned)((p.shares + scan - 1) / scan), (unsigned)tiles);
     if (p.vec > 1) hipLaunchKernelGGL((embedding_join_kernel<T, T::full>), joins, threads, 0, s, j);
     else hipLaunchKernelGGL((embedding_join_kernel<T, 1>), joins, threads, 0, s, j);
