@@ -442,3 +442,29 @@ def test_a_table_of_very_many_rows():
     y = embedding(ids.cuda(), table)
     again, = torch.autograd.grad(y, table, gy.cuda())
     assert torch.equal(again, got) and int(y.isnan().sum()) == int((~there).sum())
+
+
+@pytest.mark.parametrize("dim, dtype", [(1, torch.float32), (3, torch.bfloat16), (8, torch.float32), (48, torch.float32), (100, torch.float16),
+                                        (1030, torch.float32), (2048, torch.bfloat16)])
+@pytest.mark.parametrize("rows, where", [(1, "one"), (5000, "one"), (5000, "two"), (40, "even"), (5000, "half")])
+def test_rows_with_very_many_tokens(dim, dtype, rows, where):
+    """Rows that whole workgroups of the walk lie inside of, that begin and end anywhere, beside rows with few tokens or none."""
+    from fdgs.embedding import embedding_grad
+    tokens = 2000000 // max(dim, 20)
+    gen = torch.Generator().manual_seed(dim + rows)
+    ids = torch.randint(0, rows, (tokens,), generator=gen)
+    if where == "one":
+        ids[:] = rows // 2
+    elif where == "two":
+        ids = rows // 2 + (torch.rand(tokens, generator=gen) < 0.3).long()
+    elif where == "half":
+        ids[torch.rand(tokens, generator=gen) < 0.5] = rows - 1
+        ids[torch.rand(tokens, generator=gen) < 0.1] = -1
+    gy = torch.randn(tokens, dim, generator=gen).to(dtype)
+    got = embedding_grad(gy.cuda(), ids.int().cuda(), rows).cpu().double()
+    ok = ids >= 0
+    want = torch.zeros(rows, dim, dtype=torch.float64).index_add_(0, ids[ok], gy[ok].double())
+    size = torch.zeros(rows, dim, dtype=torch.float64).index_add_(0, ids[ok], gy[ok].double().abs())
+    many = torch.bincount(ids[ok], minlength=rows).double()[:, None]
+    # n additions in float32, each off by at most half a step of a partial sum that is at most the sum of the magnitudes
+    assert ((got - want).abs() <= many * 2.0 ** -24 * size + torch.finfo(dtype).eps / 2 * want.abs() * 1.001 + 2.0 ** -25).all()
