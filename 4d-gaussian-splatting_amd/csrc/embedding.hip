@@ -858,25 +858,40 @@ __device__ __forceinline__ void ec_add(const float* p, float* acc) {
     for (int j = 0; j < VEC; ++j) acc[j] += x.x[j];
 }
 
-// The partial sums of a row from share `first` on, before the share `end` in which it ends: one of each share, but one, its
-// last share's, of a workgroup of the walk that lies inside the row.
+// The partial sums of a row from share `first` on, before the share `end` in which it ends: one of each share, but (SOME) one,
+// its last share's, of a workgroup of the walk that has several shares and lies inside the row.
+template <bool SOME>
 struct EmSums {
     int first, head, whole, count, behind, walkers;
     __device__ __forceinline__ EmSums(int f, int end, int w) : first(f), walkers(w) {
         const int b0 = f / w, b1 = end / w;
-        head = b1 - b0 < 2 ? end - f : (b0 + 1) * w - f;
-        whole = b1 - b0 < 2 ? 0 : b1 - b0 - 1;
+        const bool all = !SOME || b1 - b0 < 2;
+        head = all ? end - f : (b0 + 1) * w - f;
+        whole = all ? 0 : b1 - b0 - 1;
         behind = b1 * w;
-        count = b1 - b0 < 2 ? head : head + whole + end - behind;
+        count = all ? head : head + whole + end - behind;
     }
-    __device__ __forceinline__ int share(int k) const {
-        return k < head ? first + k : k < head + whole ? first + head + (k - head + 1) * walkers - 1 : behind + k - head - whole;
+    // adds the sums from .. to, in order; tail: the column's sum of share 0
+    template <int VEC>
+    __device__ __forceinline__ void add(int from, int to, const float* tail, int dim, float* acc) const {
+        auto run = [&](int lo, int hi, int share, int step) {    // sums lo .. hi, the first one of `share`
+#pragma unroll 4
+            for (int q = 0; q < hi - lo; ++q) ec_add<VEC>(tail + (long long)(share + q * step) * dim, acc);
+        };
+        if (!SOME || whole == 0) {
+            run(from, to, first + from, 1);
+        } else {
+            run(from, min(to, head), first + from, 1);
+            const int w0 = max(from, head), b0 = max(from, head + whole);
+            run(w0, min(to, head + whole), first + head + (w0 - head + 1) * walkers - 1, walkers);
+            run(b0, to, behind + b0 - head - whole, 1);
+        }
     }
 };
 
 struct __attribute__((packed, aligned(1))) EmFlags8 { unsigned long long x; };
 
-template <class T, int VEC>
+template <class T, int VEC, bool SOME>
 __global__ void __launch_bounds__(EW_THREADS)
 embedding_join_kernel(EmBwd a) {
     __shared__ int first_of[EC_SCAN(EW_THREADS)], end_of[EC_SCAN(EW_THREADS)];     // first and last share of the cut rows
@@ -913,9 +928,8 @@ embedding_join_kernel(EmBwd a) {
 #pragma unroll
             for (int j = 0; j < VEC; ++j) acc[j] = 0.0f;
             ec_add<VEC>(a.head + (long long)end_of[e] * a.dim + col, acc);
-            const EmSums sum(first_of[e], end_of[e], a.walkers);
-#pragma unroll 4
-            for (int q = 0; q < sum.count; ++q) ec_add<VEC>(a.tail + (long long)sum.share(q) * a.dim + col, acc);
+            const EmSums<SOME> sum(first_of[e], end_of[e], a.walkers);
+            sum.template add<VEC>(0, sum.count, a.tail + col, a.dim, acc);
             ec_write<T, VEC>(a, row_of[e], col, acc);
         }
     }
@@ -933,16 +947,12 @@ embedding_join_kernel(EmBwd a) {
             lo += (less - 1) * step + 1;
         }
         const int first = (int)(((long long)lo + (long long)row) / a.share);
-        const EmSums sum(first, end, a.walkers);
+        const EmSums<SOME> sum(first, end, a.walkers);
         const int each = (sum.count + a.groups - 1) / a.groups, used = (sum.count + each - 1) / each;
         float acc[VEC];
 #pragma unroll
         for (int j = 0; j < VEC; ++j) acc[j] = 0.0f;
-        if (in) {
-            const int stop = min((group + 1) * each, sum.count);
-#pragma unroll 4
-            for (int q = group * each; q < stop; ++q) ec_add<VEC>(a.tail + (long long)sum.share(q) * a.dim + col, acc);
-        }
+        if (in) sum.template add<VEC>(group * each, min((group + 1) * each, sum.count), a.tail + col, a.dim, acc);
         __syncthreads();
 #pragma unroll
         for (int j = 0; j < VEC; ++j) sums[threadIdx.x * VEC + j] = acc[j];
@@ -1156,8 +1166,9 @@ static int em_bwd_launch(const EmBwd& k, const EmPlan& p, hipStream_t s) {
     j.groups = EW_THREADS / j.lanes;
     const int scan = EC_SCAN(j.groups);
     const dim3 joins((unsigned)((p.shares + scan - 1) / scan), (unsigned)tiles);
-    if (p.vec > 1) hipLaunchKernelGGL((embedding_join_kernel<T, T::full>), joins, threads, 0, s, j);
-    else hipLaunchKernelGGL((embedding_join_kernel<T, 1>), joins, threads, 0, s, j);
+    if (p.vec == 1) hipLaunchKernelGGL((embedding_join_kernel<T, 1, true>), joins, threads, 0, s, j);
+    else if (p.groups > 1) hipLaunchKernelGGL((embedding_join_kernel<T, T::full, true>), joins, threads, 0, s, j);
+    else hipLaunchKernelGGL((embedding_join_kernel<T, T::full, false>), joins, threads, 0, s, j);
     FDGS_CHECK_LAUNCH();
     return FDGS_OK;
 }
