@@ -468,3 +468,22 @@ def test_rows_with_very_many_tokens(dim, dtype, rows, where):
     many = torch.bincount(ids[ok], minlength=rows).double()[:, None]
     # n additions in float32, each off by at most half a step of a partial sum that is at most the sum of the magnitudes
     assert ((got - want).abs() <= many * 2.0 ** -24 * size + torch.finfo(dtype).eps / 2 * want.abs() * 1.001 + 2.0 ** -25).all()
+
+
+@pytest.mark.parametrize("rows", [1, 2, 300, 511, 512, 70000, 262143, 262144, (1 << 27) + 1])
+def test_every_sort_at_its_limits(rows):
+    """Sums of whole numbers, exact in float32, at the numbers of tokens where one way to sort ends and the next begins."""
+    from fdgs.embedding import embedding_grad
+    gen = torch.Generator().manual_seed(rows)
+    for tokens in (127, 128, 129, 767, 768, 769, 1536, 1537, 2304, 2305, 3072, 3073, 4095, 4096, 4097, 8192, 8193, 12289, 16384, 16385, 33000):
+        even = torch.randint(0, rows, (tokens,), generator=gen)
+        kinds = {"even": even, "skewed": (rows * torch.rand(tokens, generator=gen, dtype=torch.float64) ** 8).long(),
+                 "one": torch.full((tokens,), rows - 1), "none": torch.full((tokens,), -1), "rising": even.sort()[0],
+                 "falling": even.sort(descending=True)[0], "padded": torch.where(torch.rand(tokens, generator=gen) < 0.4, -1, even)}
+        gy = torch.randint(-8, 9, (tokens, 1), generator=gen).float().cuda()
+        for name, ids in kinds.items():
+            ids = ids.int().cuda()
+            got = embedding_grad(gy, ids, rows)
+            ok = ids >= 0
+            want = torch.zeros(rows, 1, device="cuda").index_add_(0, ids[ok].long(), gy[ok])     # whole numbers: in any order
+            assert torch.equal(got, want), (tokens, name)
