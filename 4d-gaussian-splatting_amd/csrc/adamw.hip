@@ -43,7 +43,7 @@ static_assert(sizeof(AwStep) + sizeof(AwPart<AwTensor, AW_MAX>) <= 4096, "kernel
 
 // Where the records of a launch lie: in its arguments, or (more tensors than two launches' arguments hold) in a table in
 // device memory that small launches before it have filled from theirs.  211 bfloat16 tensors with 8-bit moments and the
-// conversion of these: 250 us in six launches and five, 208 in one each and as many that fill (2 us each); 97 bfloat16 tensors
+// conversion of these: 250 us in six launches and five, 208 in one each and as many that fill (1.5 us each); 97 bfloat16 tensors
 // 204 us in three launches, 203 in one and three that fill.
 template <class Record, int MAX>
 struct AwInArgs {
