@@ -39,31 +39,50 @@ struct AwPart {
     int start[MAX];                              // first workgroup of each tensor
     int num;
 };
-static_assert(sizeof(AwStep) + sizeof(AwPart<AwTensor, AW_MAX>) <= 4096, "kernel arguments of one launch");
+// The one that workgroup `b` works on (scalar; six steps for 40 tensors.  Comparing with every start is more work than
+// the waiting it saves: 8 % for the 8-bit step over 2,000,000 Gaussians, a lane each through vector loads 2 %.)
+template <class Ints>
+__device__ __forceinline__ int aw_find(Ints start, int num, int b) {
+    int lo = 0, hi = num;
+    while (hi - lo > 1) {
+        const int m = (lo + hi) >> 1;
+        if (start[m] <= b) lo = m; else hi = m;
+    }
+    return lo;
+}
 
-// Where the records of a launch lie: in its arguments, or (more tensors than two launches' arguments hold) in a table in
-// device memory that small launches before it have filled from theirs.  211 bfloat16 tensors with 8-bit moments and the
-// conversion of these: 250 us in six launches and five, 208 in one each and as many that fill (1.5 us each); 97 bfloat16 tensors
-// 204 us in three launches, 203 in one and three that fill.
+// Where the records of a launch lie: in its arguments, or (more tensors than these hold) the last ones there and the others in a
+// table in device memory that small launches before it have filled from theirs, 1.5 to 2.5 us each.  60 float32 tensors of 5,000
+// elements: 6.5 us (8.4 in two launches over arguments), 100: 9.4 (11.1 with all records in the table); 211 bfloat16 tensors
+// with 8-bit moments and their read-out 181 (250 in six launches and five).
 template <class Record, int MAX>
 struct AwInArgs {
     AwPart<Record, MAX> part;
-    __device__ __forceinline__ int num() const { return part.num; }
-    __device__ __forceinline__ const int* starts() const { return part.start; }
-    __device__ __forceinline__ const Record& record(int i) const { return part.t[i]; }
+    __device__ __forceinline__ const Record& find(int b, int& first) const {
+        const int i = aw_find(part.start, part.num, b);
+        first = part.start[i];
+        return part.t[i];
+    }
 };
 // (The table is read through the constant address space: nothing in the launch writes it, so a record is loaded once and into
 // scalar registers like the arguments.  As ordinary memory the 8-bit step reads it again behind every store: 131 us, not 94, for
 // 40,000,000 elements.)
 template <class Record, int MAX>
-struct AwInTable {
+struct AwInBoth {
+    AwPart<Record, MAX> part;
+    int n;
     const Record* t;
     const int* start;
-    int n;
     typedef const __attribute__((address_space(4))) int* Ints;
-    __device__ __forceinline__ int num() const { return n; }
-    __device__ __forceinline__ Ints starts() const { return (Ints)(uintptr_t)start; }
-    __device__ __forceinline__ Record record(int i) const {
+    __device__ __forceinline__ Record find(int b, int& first) const {
+        if (b >= part.start[0]) {
+            const int i = aw_find(part.start, part.num, b);
+            first = part.start[i];
+            return part.t[i];
+        }
+        const Ints starts = (Ints)(uintptr_t)start;
+        const int i = aw_find(starts, n, b);
+        first = starts[i];
         int words[sizeof(Record) / 4];
         const Ints from = (Ints)(uintptr_t)(t + i);
 #pragma unroll
@@ -71,6 +90,7 @@ struct AwInTable {
         return __builtin_bit_cast(Record, words);
     }
 };
+static_assert(sizeof(AwStep) + sizeof(AwInBoth<AwTensor, AW_MAX>) <= 4096, "kernel arguments of one launch");
 template <class Record, int MAX>
 __global__ void __launch_bounds__(256)
 list_table_kernel(AwPart<Record, MAX> part, Record* table, int* start) {
@@ -89,37 +109,38 @@ list_table_kernel(AwPart<Record, MAX> part, Record* table, int* start) {
 static size_t list_table_bytes(int num, size_t record) { return (size_t)num * (record + sizeof(int)) + 512; }
 
 // Runs `launch(source, workgroups)` for all the records that `next(record, workgroups)` gives (false: no more): in one launch
-// over the table where there is a workspace and more of them than the arguments hold, else in as many launches as it takes.
+// where the arguments hold them all or there is a workspace for the others, else in as many launches as it takes.
 template <class Record, int MAX, class Next, class Launch>
 static int list_launch(int count, void* workspace, size_t bytes, hipStream_t s, Next next, Launch launch) {
-    const bool table = count > 2 * MAX && workspace && bytes >= list_table_bytes(count, sizeof(Record));
+    const bool table = count > MAX && workspace && bytes >= list_table_bytes(count, sizeof(Record));
     Record* records = (Record*)(((uintptr_t)workspace + 255) / 256 * 256);
     int* starts = (int*)(records + count);
-    int blocks = 0, filled = 0;
-    for (bool more = true; more;) {
-        AwInArgs<Record, MAX> args;
-        args.part.num = 0;
-        if (!table) blocks = 0;
-        while (args.part.num < MAX) {
-            int groups = 0;
-            more = next(args.part.t[args.part.num], groups);
-            if (!more) break;
-            args.part.start[args.part.num++] = blocks;
-            blocks += groups;
+    AwInBoth<Record, MAX> both;
+    AwPart<Record, MAX>& part = both.part;
+    int blocks = 0, filled = 0, groups = 0;
+    part.num = 0;
+    for (Record r; next(r, groups); blocks += groups) {
+        if (part.num == MAX) {
+            if (table) {
+                hipLaunchKernelGGL((list_table_kernel<Record, MAX>), dim3(1), dim3(256), 0, s, part, records + filled, starts + filled);
+                filled += MAX;
+            } else {
+                launch(AwInArgs<Record, MAX>{part}, blocks);
+                blocks = 0;
+            }
+            FDGS_CHECK_LAUNCH();
+            part.num = 0;
         }
-        if (args.part.num == 0) break;
-        if (table) {
-            hipLaunchKernelGGL((list_table_kernel<Record, MAX>), dim3(1), dim3(256), 0, s, args.part, records + filled, starts + filled);
-            filled += args.part.num;
-        } else {
-            launch(args, blocks);
-        }
-        FDGS_CHECK_LAUNCH();
+        part.t[part.num] = r;
+        part.start[part.num++] = blocks;
     }
-    if (table && filled) {
-        launch(AwInTable<Record, MAX>{records, starts, filled}, blocks);
-        FDGS_CHECK_LAUNCH();
-    }
+    if (part.num == 0) return FDGS_OK;
+    both.n = filled;
+    both.t = records;
+    both.start = starts;
+    if (filled) launch(both, blocks);
+    else launch(AwInArgs<Record, MAX>{part}, blocks);
+    FDGS_CHECK_LAUNCH();
     return FDGS_OK;
 }
 
@@ -195,18 +216,6 @@ __device__ __forceinline__ float aw_exact(float w, float m, float v, const AwSte
 #pragma clang fp contract(off)
     const float denom = sqrtf(v) * t.inv_root + k.eps;
     return w * t.decay - (m * t.step_size) / denom;
-}
-
-// The tensor that workgroup `b` works on (scalar; six steps for 40 tensors.  Comparing with every start is more work than
-// the waiting it saves: 8 % for the 8-bit step over 2,000,000 Gaussians, a lane each through vector loads 2 %.)
-template <class Ints>
-__device__ __forceinline__ int aw_find(Ints start, int num, int b) {
-    int lo = 0, hi = num;
-    while (hi - lo > 1) {
-        const int m = (lo + hi) >> 1;
-        if (start[m] <= b) lo = m; else hi = m;
-    }
-    return lo;
 }
 
 template <bool BF16>
@@ -423,10 +432,10 @@ __device__ __forceinline__ void aw_finish(const AwStep& k, const AwTensor& t, lo
 template <bool BF16, bool EIGHT, class Source>
 __global__ void __launch_bounds__(AW_THREADS)
 adamw_kernel(AwStep k, Source source) {
-    const int ti = aw_find(source.starts(), source.num(), (int)blockIdx.x);
-    const AwTensor& t = source.record(ti);
+    int first;
+    const AwTensor& t = source.find((int)blockIdx.x, first);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const long long block = (long long)((int)blockIdx.x - source.starts()[ti]) * AW_PER_GROUP + wave * M8_BLOCK;
+    const long long block = (long long)((int)blockIdx.x - first) * AW_PER_GROUP + wave * M8_BLOCK;
     AwLane<BF16, EIGHT> x;
     if (block + M8_BLOCK <= t.n) {
         aw_load<BF16, EIGHT, true>(t, block, 4, x);
@@ -490,13 +499,13 @@ extern "C" int fdgs_adamw_step(const fdgs_adamw_args* a, void* stream) {
 }
 
 extern "C" size_t fdgs_adamw_workspace_bytes(int32_t num_tensors) {
-    return num_tensors > 2 * AW_MAX ? list_table_bytes(num_tensors, sizeof(AwTensor)) : 0;
+    return num_tensors > AW_MAX ? list_table_bytes(num_tensors, sizeof(AwTensor)) : 0;
 }
 
 // ---- 8-bit moments to values and back ----
 #define M8_MAX 92                                // tensors whose records fill 4 KB of kernel arguments
 struct M8Tensor { uint8_t* codes; uint8_t* exps; void* value; long long n; uint32_t key; int is_signed; };
-static_assert(sizeof(AwPart<M8Tensor, M8_MAX>) + 8 <= 4096, "kernel arguments of one launch");
+static_assert(sizeof(AwInBoth<M8Tensor, M8_MAX>) + 8 <= 4096, "kernel arguments of one launch");
 
 // What a lane takes at a time: as many codes as make 16 bytes of values, a wave's stores being neighbours (8 codes for two
 // stores of float32: 116,000,000 elements 150 us, not 101).  Ordinary loads: with streaming ones the next step finds the codes
@@ -572,9 +581,9 @@ __device__ __forceinline__ void m8_unpack_group(const M8Tensor& t, long long fir
 template <bool BF16, class Source>
 __global__ void __launch_bounds__(256)
 moment8_unpack_kernel(Source source) {
-    const int ti = aw_find(source.starts(), source.num(), (int)blockIdx.x);
-    const M8Tensor& t = source.record(ti);
-    const long long first = (long long)((int)blockIdx.x - source.starts()[ti]) * M8_PER_GROUP;
+    int group;
+    const M8Tensor& t = source.find((int)blockIdx.x, group);
+    const long long first = (long long)((int)blockIdx.x - group) * M8_PER_GROUP;
     if (t.is_signed) m8_unpack_group<BF16, true>(t, first);
     else m8_unpack_group<BF16, false>(t, first);
 }
@@ -613,10 +622,10 @@ __device__ __forceinline__ void m8_pack4(bool nearest, const M8Tensor& t, long l
 template <class Source>
 __global__ void __launch_bounds__(256)
 moment8_pack_kernel(int nearest, Source source) {
-    const int ti = aw_find(source.starts(), source.num(), (int)blockIdx.x);
-    const M8Tensor& t = source.record(ti);
+    int first;
+    const M8Tensor& t = source.find((int)blockIdx.x, first);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const long long base = (long long)((int)blockIdx.x - source.starts()[ti]) * M8_PER_GROUP + wave * (M8_PER_GROUP / 4);
+    const long long base = (long long)((int)blockIdx.x - first) * M8_PER_GROUP + wave * (M8_PER_GROUP / 4);
     const float* value = (const float*)t.value + 4 * (int)(threadIdx.x & 63);
     float x[M8_WAVE_BLOCKS][4];
 #pragma unroll
@@ -675,7 +684,7 @@ static int moment8_launch(const fdgs_moment8_args* a, void* stream, bool pack) {
 }
 
 extern "C" size_t fdgs_moment8_workspace_bytes(int32_t num_tensors) {
-    return num_tensors > 2 * M8_MAX ? list_table_bytes(num_tensors, sizeof(M8Tensor)) : 0;
+    return num_tensors > M8_MAX ? list_table_bytes(num_tensors, sizeof(M8Tensor)) : 0;
 }
 
 extern "C" int fdgs_moment8_unpack(const fdgs_moment8_args* a, void* stream) { return moment8_launch(a, stream, false); }

@@ -521,7 +521,7 @@ typedef struct {
     void* workspace; size_t workspace_bytes;   /* fdgs_adamw_workspace_bytes(num_tensors) of device memory for the one
                                                   launch, or NULL: then a launch for each 40 tensors            */
 } fdgs_adamw_args;
-size_t fdgs_adamw_workspace_bytes(int32_t num_tensors);   /* 0 up to 80 tensors: nothing to be gained */
+size_t fdgs_adamw_workspace_bytes(int32_t num_tensors);   /* 0 up to 40 tensors: nothing to be gained */
 int fdgs_adamw_step(const fdgs_adamw_args* a, void* stream);
 
 /* 8-bit moments to the values they stand for (value_type float32 or bfloat16, both exact), and float32 values to
@@ -543,7 +543,7 @@ typedef struct {
     void* workspace; size_t workspace_bytes;   /* fdgs_moment8_workspace_bytes(num_tensors), or NULL: then a launch for
                                                   each 92 tensors                                                */
 } fdgs_moment8_args;
-size_t fdgs_moment8_workspace_bytes(int32_t num_tensors);   /* 0 up to 184 tensors */
+size_t fdgs_moment8_workspace_bytes(int32_t num_tensors);   /* 0 up to 92 tensors */
 int fdgs_moment8_unpack(const fdgs_moment8_args* a, void* stream);
 int fdgs_moment8_pack(const fdgs_moment8_args* a, void* stream);
 
