@@ -471,7 +471,9 @@ extern "C" int fdgs_adamw_step(const fdgs_adamw_args* a, void* stream) {
     k.b2 = (float)a->beta2; k.omb2 = (float)(1.0 - a->beta2);
     k.eps = (float)a->eps;
     k.exact = k.eps > 0.0f && k.eps < 1.17549435e-38f;
-    int i = 0;
+    int i = 0, step = 0;
+    double correct1 = 1.0;
+    float inv_root = 1.0f;
     auto next = [&](AwTensor& t, int& groups) {
         while (i < a->num_tensors && a->tensors[i].numel == 0) ++i;
         if (i == a->num_tensors) return false;
@@ -480,8 +482,13 @@ extern "C" int fdgs_adamw_step(const fdgs_adamw_args* a, void* stream) {
         t.p = s.param; t.g = s.grad; t.m = s.exp_avg; t.v = s.exp_avg_sq;
         t.low = s.residual; t.me = s.exp_avg_exponents; t.ve = s.exp_avg_sq_exponents;
         t.n = s.numel; t.gstride = s.grad_row_stride; t.glen = s.grad_row_len;
-        t.step_size = (float)(s.lr / (1.0 - pow(a->beta1, (double)s.step)));
-        t.inv_root = (float)(1.0 / sqrt(1.0 - pow(a->beta2, (double)s.step)));
+        if (s.step != step) {                    // most tensors of a list have the same count
+            step = s.step;
+            correct1 = 1.0 - pow(a->beta1, (double)step);
+            inv_root = (float)(1.0 / sqrt(1.0 - pow(a->beta2, (double)step)));
+        }
+        t.step_size = (float)(s.lr / correct1);
+        t.inv_root = inv_root;
         t.decay = (float)(1.0 - s.lr * s.weight_decay);
         t.key = s.round_key; t.pad = 0;
         return true;
