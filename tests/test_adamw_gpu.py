@@ -476,3 +476,37 @@ def test_captured_conversions(count):
             codes, exps = ac.encode(v.numpy(), 0x8000, s)
             assert np.array_equal(m.codes.cpu().numpy(), codes) and np.array_equal(m.exponents.cpu().numpy(), exps)
         del other
+
+
+def test_long_lists_without_a_workspace():
+    """Through the C ABI, without the device memory that one launch over all tensors needs: as many launches as it takes, and the
+    same bits."""
+    import ctypes as C
+    from fdgs import _lib, _records
+    from fdgs.adamw import Moment8, adamw_step, pack8, unpack8
+    gen = torch.Generator().manual_seed(0)
+    sizes = [int(n) for n in torch.randint(0, 600, (201,), generator=gen)]
+    p = [torch.randn(n, generator=gen).cuda() for n in sizes]
+    g = [torch.randn(n, generator=gen).cuda() for n in sizes]
+    q = [x.clone() for x in p]
+    state = [[Moment8.zeros_like(x, s) for x in p] for s in (True, False, True, False)]
+    adamw_step(p, g, state[0], state[1], steps=2, lr=1e-2, keys=list(range(201)))
+    rows = (_records.AdamWTensor * 201)(*[_records.AdamWTensor(
+        param=a.data_ptr(), grad=b.data_ptr(), exp_avg=m.codes.data_ptr(), exp_avg_sq=v.codes.data_ptr(),
+        exp_avg_exponents=m.exponents.data_ptr(), exp_avg_sq_exponents=v.exponents.data_ptr(), numel=a.numel(), step=2, lr=1e-2,
+        weight_decay=1e-2, round_key=i) for i, (a, b, m, v) in enumerate(zip(q, g, state[2], state[3]))])
+    args = _records.AdamWArgs(num_tensors=201, param_type=0, state_bits=8, beta1=0.9, beta2=0.999, eps=1e-8,
+                              tensors=C.cast(rows, C.c_char_p))
+    _lib.call("fdgs_adamw_step", args)
+    for a, b in zip(p + [x for s in state[:2] for m in s for x in m[:2]], q + [x for s in state[2:] for m in s for x in m[:2]]):
+        assert torch.equal(a, b)
+    moments = state[0] + state[1]
+    out = [torch.full(m.codes.shape, -1.0, device="cuda") for m in moments]
+    rows = (_records.Moment8Tensor * 402)(*[_records.Moment8Tensor(
+        codes=m.codes.data_ptr(), exponents=m.exponents.data_ptr(), value=o.data_ptr(), numel=o.numel(), is_signed=m.signed)
+        for m, o in zip(moments, out)])
+    args = _records.Moment8Args(num_tensors=402, value_type=0, tensors=C.cast(rows, C.c_char_p))
+    _lib.call("fdgs_moment8_unpack", args)
+    for a, b in zip(out, unpack8(moments)):
+        assert torch.equal(a, b)
+    assert len(pack8(out, [m.signed for m in moments])) == 402
