@@ -13,6 +13,7 @@
 // of one frequent row or the zeros of many rows that nobody asked for.  A row that is cut by a share's end leaves
 // partial sums in the workspace, which a last launch adds up in the shares' order.  No atomic touches a sum.
 #include "fdgs_common.h"
+#include <type_traits>
 
 // ---- element types: 16 bytes to a vector where the row is that long, else one element ----
 typedef uint32_t em_u4 __attribute__((ext_vector_type(4)));
@@ -77,55 +78,60 @@ __device__ __forceinline__ void em_store(typename T::raw* p, const EmVec<T, VEC>
 // ---- forward ----
 #define EF_THREADS 256
 #define EF_UNROLL 4
-#define EF_VECTORS (EF_THREADS * EF_UNROLL)
+#define EF_VECTORS (EF_THREADS * EF_UNROLL)          // of a workgroup at most
 
 struct EmFwd {
     const void* ids; const void* table; void* out;
     long long table_stride, padding;
-    int tokens, rows, dim, nv, wide, per_group;          // per_group: tokens of a workgroup
+    int tokens, rows, dim, nv, wide, per_group, vectors; // tokens and vectors of a workgroup
     float scale;
     EmDiv by_nv;
 };
 
-// A workgroup has whole tokens, as many as make up to 1024 vectors (or, of a longer row, 1024 vectors of one token): a
-// thread has up to four vectors, all of whose ids and then all of whose rows are asked for before the first is used.
+// A workgroup has whole tokens, as many as make up to 512 or 1024 vectors (or, of a longer row, so many of one token): a
+// thread has up to two or four vectors, all of whose ids and then all of whose rows are asked for before the first is used.
 // Bound by the output's lines and, where the table does not fit an XCD's 4 MB of L2, by the rows that come from behind it:
-// 300,000 x 48 floats 14 us (4.4 TB/s), 2,000,000 x 48 from 65,536 rows 120 us, from 8,192 rows 66 us (5.8 TB/s).
+// 300,000 x 48 floats 12.6 us (4.8 TB/s), 2,000,000 x 48 from 65,536 rows 120 us, from 8,192 rows 66 us (5.8 TB/s).
 template <class T, int VEC>
 __device__ __forceinline__ void ef_group(const EmFwd& a, int group, int tile, uint32_t thread) {
     typedef EmVec<T, VEC> Vec;
     typedef typename T::raw raw;
     const int tok0 = group * a.per_group, have = min(a.per_group, a.tokens - tok0);
-    const int c0 = tile * EF_VECTORS, cols = min(a.nv - c0, EF_VECTORS);   // all of them, or a part of one row
+    const int c0 = tile * a.vectors, cols = min(a.nv - c0, a.vectors);   // all of them, or a part of one row
     const uint32_t end = (uint32_t)have * (uint32_t)cols;
-    Vec v[EF_UNROLL];
-    int tok[EF_UNROLL], col[EF_UNROLL];
-    long long id[EF_UNROLL];
+    auto part = [&](auto unroll) {
+        constexpr int U = decltype(unroll)::value;
+        Vec v[U];
+        int tok[U], col[U];
+        long long id[U];
 #pragma unroll
-    for (int u = 0; u < EF_UNROLL; ++u) {
-        const uint32_t e = u * EF_THREADS + thread;
-        const uint32_t t = a.per_group > 1 ? em_div(e, a.by_nv) : 0u;
-        tok[u] = e < end ? tok0 + (int)t : -1;
-        col[u] = em_col<VEC>(c0 + (int)(e - t * (uint32_t)a.nv), a.nv, a.dim);
-        id[u] = -1;
-        if (tok[u] >= 0) {
-            id[u] = a.wide ? ((const long long*)a.ids)[tok[u]] : (long long)((const int*)a.ids)[tok[u]];
-            if (id[u] == a.padding) id[u] = -1;
+        for (int u = 0; u < U; ++u) {
+            const uint32_t e = u * EF_THREADS + thread;
+            const uint32_t t = a.per_group > 1 ? em_div(e, a.by_nv) : 0u;
+            tok[u] = e < end ? tok0 + (int)t : -1;
+            col[u] = em_col<VEC>(c0 + (int)(e - t * (uint32_t)a.nv), a.nv, a.dim);
+            id[u] = -1;
+            if (tok[u] >= 0) {
+                id[u] = a.wide ? ((const long long*)a.ids)[tok[u]] : (long long)((const int*)a.ids)[tok[u]];
+                if (id[u] == a.padding) id[u] = -1;
+            }
         }
-    }
 #pragma unroll
-    for (int u = 0; u < EF_UNROLL; ++u)
-        if (id[u] >= 0 && id[u] < a.rows) v[u] = *(const Vec*)((const raw*)a.table + id[u] * a.table_stride + col[u]);
+        for (int u = 0; u < U; ++u)
+            if (id[u] >= 0 && id[u] < a.rows) v[u] = *(const Vec*)((const raw*)a.table + id[u] * a.table_stride + col[u]);
 #pragma unroll
-    for (int u = 0; u < EF_UNROLL; ++u) {
-        if (tok[u] < 0) continue;
-        const bool there = id[u] >= 0 && id[u] < a.rows;
-        const float other = id[u] < 0 ? 0.0f : __builtin_nanf("");
-        Vec o;
+        for (int u = 0; u < U; ++u) {
+            if (tok[u] < 0) continue;
+            const bool there = id[u] >= 0 && id[u] < a.rows;
+            const float other = id[u] < 0 ? 0.0f : __builtin_nanf("");
+            Vec o;
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) o.x[j] = em_down<T>(there ? em_up<T>(v[u].x[j]) * a.scale : other);
-        em_store<T, VEC>((raw*)a.out + (long long)tok[u] * a.dim + col[u], o);
-    }
+            for (int j = 0; j < VEC; ++j) o.x[j] = em_down<T>(there ? em_up<T>(v[u].x[j]) * a.scale : other);
+            em_store<T, VEC>((raw*)a.out + (long long)tok[u] * a.dim + col[u], o);
+        }
+    };
+    if (a.vectors > EF_VECTORS / 2) part(std::integral_constant<int, EF_UNROLL>());
+    else part(std::integral_constant<int, EF_UNROLL / 2>());
 }
 
 template <class T, int VEC>
@@ -1132,8 +1138,12 @@ extern "C" int fdgs_embedding_fwd(const fdgs_embedding_fwd_args* a, void* stream
     f.vec = k.dim >= em_full(a->type) ? em_full(a->type) : 1;
     k.nv = (k.dim + f.vec - 1) / f.vec;
     k.by_nv = em_div_of((uint32_t)k.nv);
-    k.per_group = k.nv < EF_VECTORS ? EF_VECTORS / k.nv : 1;
-    const int tiles = (k.nv + EF_VECTORS - 1) / EF_VECTORS;
+    // Four vectors a thread where rows come from behind L2 for long (2,000,000 x 48 floats from 12.6 MB of table, with the sort:
+    // 153 us, 160 with two), else two (300,000 x 48 floats 12.5 us, 14 with four, 17 with eight; one token 2.5, 2.7, 3.2).
+    const long long size = a->type == FDGS_TYPE_F32 ? 4 : 2, row = (long long)k.dim * size;
+    k.vectors = row * k.rows > (4 << 20) && row * k.tokens > (64 << 20) ? EF_VECTORS : EF_VECTORS / 2;
+    k.per_group = k.nv < k.vectors ? k.vectors / k.nv : 1;
+    const int tiles = (k.nv + k.vectors - 1) / k.vectors;
     const long long groups = ((long long)k.tokens + k.per_group - 1) / k.per_group;
     hipStream_t s = (hipStream_t)stream;
     const bool sort = a->sorted && a->num_tokens > EW_SMALL;     // fewer are sorted where they are added
