@@ -788,6 +788,7 @@ embedding_walk_kernel(EmBwd a) {
         while (i < ie && key_at(i) == v) ++i;
         if (!inside) ++v;
     }
+    bool any = !SMALL && began;                      // the row has tokens
     auto flush = [&](uint32_t row) {
         if (head) {
             float* h = a.head + share * a.dim + col;
@@ -796,12 +797,25 @@ embedding_walk_kernel(EmBwd a) {
             head = false;
         } else {
             Vec o;
+            const float scale = any ? a.scale : 0.0f;
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) o.x[j] = em_down<T>(acc[j] * a.scale);
+            for (int j = 0; j < VEC; ++j) o.x[j] = em_down<T>(acc[j] * scale);
             em_store<T, VEC>((raw*)a.dtable + (long long)row * a.dim + col, o);
         }
+        any = false;
 #pragma unroll
         for (int j = 0; j < VEC; ++j) acc[j] = 0.0f;
+    };
+    // Writes the rows up to `end`: the one that is being added, and behind it rows without tokens, which are zeros whatever
+    // the scale is.
+    auto write = [&](uint32_t end) {
+        if (v >= end) return;
+        flush(v);
+        ++v;
+        const Vec zero = {};
+        raw* p = (raw*)a.dtable + (long long)v * a.dim + col;
+#pragma unroll 4
+        for (; v < end; ++v, p += a.dim) em_store<T, VEC>(p, zero);
     };
     // adds tokens p .. q, writing the rows that end in between; tokens without a row come last of all
     auto walk = [&](int p, int q) {
@@ -814,7 +828,8 @@ embedding_walk_kernel(EmBwd a) {
             for (int u = 0; u < EW_BATCH; ++u) {
                 if (p + u < q) {
                     const uint32_t key = sk[p + u - k0];
-                    while (v < key) { flush(v); ++v; }
+                    write(key);
+                    any = true;
 #pragma unroll
                     for (int j = 0; j < VEC; ++j) acc[j] += em_up<T>(x[u].x[j]);
                 }
@@ -828,7 +843,7 @@ embedding_walk_kernel(EmBwd a) {
         while (valid > i && key_at(valid - 1) >= rows) --valid;
     }
     walk(i, valid);
-    while (v < ve) { flush(v); ++v; }
+    write(ve);
     const bool open = ie > 0 && key_at(ie - 1) == ve && ve < rows;   // a row that a later share ends in the sequence
     if (!SMALL && open) {
         float* t = a.tail + share * a.dim + col;

@@ -487,3 +487,15 @@ def test_every_sort_at_its_limits(rows):
             ok = ids >= 0
             want = torch.zeros(rows, 1, device="cuda").index_add_(0, ids[ok].long(), gy[ok])     # whole numbers: in any order
             assert torch.equal(got, want), (tokens, name)
+
+
+@pytest.mark.parametrize("scale", [-2.0, math.inf, math.nan])
+@pytest.mark.parametrize("tokens, apart", [(3, 7), (100, 7), (5000, 7), (128, 6), (100, 11), (700, 13), (900, 17)])
+def test_rows_without_tokens_are_zeros_whatever_the_scale(scale, tokens, apart):
+    from fdgs.embedding import embedding_grad
+    ids = apart * torch.arange(tokens, device="cuda") % 901
+    got = embedding_grad(torch.ones(tokens, 6, device="cuda"), ids, 6000, scale=scale)
+    none = torch.ones(6000, dtype=torch.bool, device="cuda")
+    none[ids] = False
+    assert int(none.sum()) > 5000 and (got[none].view(torch.int32) == 0).all()           # and no negative zero
+    assert not torch.isfinite(got[~none]).any() if math.isinf(scale) or math.isnan(scale) else (got[~none] < 0).all()
