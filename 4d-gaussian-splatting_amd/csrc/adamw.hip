@@ -171,9 +171,17 @@ __device__ __forceinline__ void aw_split(float w, uint16_t& hi, int16_t& lo) {
     hi = (uint16_t)(nan ? 0x7FC0u : (b + 0x8000u) >> 16);
     lo = (int16_t)(nan ? 0u : b);
 }
-__device__ __forceinline__ float aw_join(uint16_t hi, int16_t lo) {
-    return __uint_as_float(((uint32_t)hi << 16) + (uint32_t)(int)lo);
+// The weight: pattern plus residual, as far as the two belong together.  A zero has no residual below it and an infinity none above
+// it; one that is written from outside (a mask, a reset) beside another weight's residual stays what it is instead of the NaN that the
+// plain sum would make of it.
+__device__ __forceinline__ float aw_weight(uint32_t hi, int lo) {     // hi: the pattern in the upper half, zeros below
+    const int size = (int)(hi & 0x7FFFFFFFu), most = size > 0x7F800000 ? size : 0x7F800000;
+    int w = size + lo;
+    w = w > 0 ? w : 0;
+    w = w < most ? w : most;
+    return __uint_as_float((uint32_t)w | (hi & 0x80000000u));
 }
+__device__ __forceinline__ float aw_join(uint16_t hi, int16_t lo) { return aw_weight((uint32_t)hi << 16, lo); }
 __device__ __forceinline__ void aw_split4(const float* w, aw_h4& h, aw_h4& l) {
     if (__ballot(__builtin_isunordered(w[0], w[1]) || __builtin_isunordered(w[2], w[3])) == 0) {     // no NaN in the wave
 #pragma unroll
@@ -197,8 +205,8 @@ __device__ __forceinline__ void aw_split4(const float* w, aw_h4& h, aw_h4& l) {
 __device__ __forceinline__ void aw_join4(const aw_h4& h, const aw_h4& l, float* w) {
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-        w[2 * j] = __uint_as_float((h.x[j] << 16) + (uint32_t)((int)(l.x[j] << 16) >> 16));
-        w[2 * j + 1] = __uint_as_float((h.x[j] & 0xFFFF0000u) + (uint32_t)((int)l.x[j] >> 16));
+        w[2 * j] = aw_weight(h.x[j] << 16, (int)(l.x[j] << 16) >> 16);
+        w[2 * j + 1] = aw_weight(h.x[j] & 0xFFFF0000u, (int)l.x[j] >> 16);
     }
 }
 __device__ __forceinline__ float aw_bf16(uint16_t h) { return __uint_as_float((uint32_t)h << 16); }

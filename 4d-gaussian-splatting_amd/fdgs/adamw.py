@@ -9,7 +9,7 @@ torch.optim.AdamW's parameter groups, state and state_dict (beside fdgs.adam.Fus
 that the step and the densification surgery move for them.  Their format and rounding are described in
 include/fdgs.h.  bfloat16 parameters keep the 16 bits that bfloat16 drops in `residual`: parameter and residual
 together are the float32 weight, so updates smaller than a bfloat16 step add up instead of vanishing, and a parameter
-that is written from outside (a checkpoint) simply is the new weight, up to half a bfloat16 step."""
+that is written from outside (a checkpoint, a mask) simply is the new weight, up to half a bfloat16 step."""
 from typing import NamedTuple
 
 import torch

@@ -480,7 +480,9 @@ int fdgs_adam_step(const fdgs_adam_args* a, void* stream);
  *
  * param_type FDGS_TYPE_BF16: the parameter and the gradient are bfloat16, and `residual` holds, per element, the signed
  * 16 bits by which the float32 weight's bit pattern lies beside the bfloat16 one's ((param << 16) + residual is the
- * weight): updates smaller than a bfloat16 step add up.  Zeros to begin with.
+ * weight): updates smaller than a bfloat16 step add up.  Zeros to begin with.  A parameter of zero with a
+ * negative residual is zero and an infinite one with a positive residual infinite: the step leaves no such pairs, a parameter that
+ * is written from outside does.
  *
  * state_bits 8: exp_avg / exp_avg_sq are one byte per element and each has one exponent byte per block of
  * FDGS_MOMENT8_BLOCK consecutive elements.  With E the block's exponent byte (the biased float32 exponent of its largest

@@ -510,3 +510,22 @@ def test_long_lists_without_a_workspace():
     for a, b in zip(out, unpack8(moments)):
         assert torch.equal(a, b)
     assert len(pack8(out, [m.signed for m in moments])) == 402
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("n", [512, 300])
+def test_bfloat16_parameters_set_to_zero_or_infinity(n, bits):
+    """A parameter that is masked or reset while its residual stays is the new weight: no pair of a zero or an infinity and a residual
+    that cannot belong to it is read as a NaN, and every other pair as pattern plus residual.  Blocks of 256 and what is left."""
+    from fdgs.adamw import Moment8, adamw_step
+    word = torch.tensor([0x0000, 0x8000, 0x7F80, 0xFF80, 0x3F80], dtype=torch.int32)
+    low = torch.tensor([-0x8000, -5, -1, 0, 1, 123, 0x7FFF], dtype=torch.int32)
+    hi, lo = (x.reshape(-1).repeat(-(-n // 35))[:n] for x in torch.broadcast_tensors(word[:, None], low[None]))
+    p, res = hi.to(torch.int16).cuda().view(torch.bfloat16), lo.to(torch.int16).cuda()
+    m, v = (Moment8.zeros_like(p, s) if bits == 8 else torch.zeros(n, device="cuda") for s in (True, False))
+    adamw_step([p], [torch.zeros_like(p)], [m], [v], steps=1, lr=1e-3, weight_decay=0.0, residuals=[res], keys=[1] if bits == 8 else None)
+    size = hi & 0x7FFF
+    gone = ((size == 0) & (lo < 0)) | ((size == 0x7F80) & (lo > 0))
+    want = (hi << 16) + torch.where(gone, torch.zeros_like(lo), lo)
+    got = (p.view(torch.int16).to(torch.int32) << 16) + res.to(torch.int32)
+    assert torch.equal(got.cpu(), want)
