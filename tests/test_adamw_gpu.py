@@ -529,3 +529,25 @@ def test_bfloat16_parameters_set_to_zero_or_infinity(n, bits):
     want = (hi << 16) + torch.where(gone, torch.zeros_like(lo), lo)
     got = (p.view(torch.int16).to(torch.int32) << 16) + res.to(torch.int32)
     assert torch.equal(got.cpu(), want)
+
+
+@pytest.mark.parametrize("eps", [1e-8, 1e-15])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_update_is_the_formula_rounded_once_an_operation(bits, eps):
+    """float32 parameters move by the bits that the formula gives in float32 with every operation rounded to the nearest, whatever
+    form the moments have."""
+    from fdgs import adamw
+    f, b1, b2, lr, wd, t = np.float32, 0.9, 0.999, 3e-3, 0.1, 7
+    (w, g, m0, v0), = _inputs([70001], 11)
+    p, gd = torch.from_numpy(w).cuda(), torch.from_numpy(g).cuda()
+    if bits == 8:
+        cm, cv = ac.encode(m0, 0x8000, True), ac.encode(v0, 0x8000, False)
+        m0, v0 = ac.decode(*cm, True), ac.decode(*cv, False)
+        m, v = (adamw.Moment8(*(torch.from_numpy(x).cuda() for x in c), s) for c, s in ((cm, True), (cv, False)))
+    else:
+        m, v = torch.from_numpy(m0).cuda(), torch.from_numpy(v0).cuda()
+    adamw.adamw_step([p], [gd], [m], [v], steps=t, lr=lr, betas=(b1, b2), eps=eps, weight_decay=wd, keys=[5] if bits == 8 else None)
+    m1, v1 = ac.adamw32(g, m0, v0, b1, b2)
+    denom = np.sqrt(v1) * f(1.0 / math.sqrt(1.0 - b2 ** t)) + f(eps)
+    want = w * f(1.0 - lr * wd) - (m1 * f(lr / (1.0 - b1 ** t))) / denom
+    assert want.dtype == f and np.array_equal(p.cpu().numpy().view(np.int32), want.view(np.int32))
