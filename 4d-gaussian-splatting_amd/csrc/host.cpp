@@ -368,10 +368,16 @@ Tensor rows_of(const Tensor& t, int64_t lead, int64_t& width, int64_t& stride) {
     return t;
 }
 
+// What leaves here carries no tangent, so a tensor that has one is refused.
+void no_tangent(const Tensor& t, const char* what) {
+    if (t._fw_grad(/*level=*/0).defined()) throw Refused{PyExc_NotImplementedError, std::string(what) + " has a forward-mode derivative, which embedding() does not carry on"};
+}
+
 // sorted: where it is given, it is set to the tokens by row, which spare the gradient its sort (undefined where there is
 // nothing to sort).
 Tensor lookup(const Tensor& ids0, const Tensor& table0, double scale, int64_t padding, Tensor* sorted = nullptr) {
     const int type = type_of(table0, "the table");
+    no_tangent(table0, "the table");
     const Tensor ids = ids_of(ids0, table0.device());
     int64_t width, stride;
     const Tensor table = rows_of(table0, 1, width, stride);
@@ -406,6 +412,7 @@ Tensor lookup(const Tensor& ids0, const Tensor& table0, double scale, int64_t pa
 }
 
 Tensor table_grad(const Tensor& grad_out0, const Tensor& ids0, int64_t rows, double scale, int64_t padding, const Tensor& sorted = Tensor()) {
+    no_tangent(grad_out0, "grad_out");
     on_gpu(grad_out0);
     const int type = type_of(grad_out0, "grad_out");
     const Tensor ids = ids_of(ids0, grad_out0.device());
@@ -543,6 +550,7 @@ PyObject* embedding(PyObject* a) {
     const Tensor &ids = tensor(io, "ids"), &table = tensor(to, "the table");
     if (table.dim() < 2) value_error("the table is [rows, ...] in float32, bfloat16 or float16");
     type_of(table, "the table");
+    no_tangent(table, "the table");
     on_gpu(table);
     const int64_t padding = padding_of(po);
     Tensor out;

@@ -499,3 +499,18 @@ def test_rows_without_tokens_are_zeros_whatever_the_scale(scale, tokens, apart):
     none[ids] = False
     assert int(none.sum()) > 5000 and (got[none].view(torch.int32) == 0).all()           # and no negative zero
     assert not torch.isfinite(got[~none]).any() if math.isinf(scale) or math.isnan(scale) else (got[~none] < 0).all()
+
+
+def test_forward_derivatives_are_refused_on_the_device():
+    import torch.autograd.forward_ad as forward_ad
+    from fdgs.embedding import embedding, embedding_grad
+    ids, table = torch.tensor([1, 2], device="cuda"), torch.randn(5, 4, device="cuda")
+    tangent = torch.ones(2, 4, device="cuda")
+    with forward_ad.dual_level():
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            embedding(ids, forward_ad.make_dual(table, torch.ones_like(table)))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            embedding_grad(forward_ad.make_dual(table[:2], tangent), ids, 5)
+        y = embedding(ids, table.requires_grad_(True))
+        with pytest.raises(RuntimeError, match="forward-mode"):          # out of a backward pass
+            torch.autograd.grad(y, table, forward_ad.make_dual(tangent, tangent))

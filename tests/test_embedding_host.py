@@ -97,3 +97,19 @@ def test_render_refuses_a_codebook_that_does_not_fit(ids, row):
                          feature_codebook=FeatureCodebook(torch.zeros(7, *row), torch.zeros(ids, dtype=torch.int32)))
     with pytest.raises(ValueError, match="an id each"):
         render(cam, pc, None, torch.zeros(3), stage="coarse")
+
+
+def test_forward_derivatives_are_refused():
+    """The kernels carry no tangent: a result without one would read as a derivative of zero."""
+    import torch.autograd.forward_ad as forward_ad
+    from fdgs.embedding import embedding, embedding_grad
+    ids, x = torch.tensor([0, 1]), torch.ones(2, 4)
+    with forward_ad.dual_level():
+        for wants in (False, True):
+            dual = forward_ad.make_dual(x.clone().requires_grad_(wants), x)
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                embedding(ids, dual)
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                embedding_grad(dual, ids, 3)
+        with pytest.raises(RuntimeError, match="GPU only"):
+            embedding(ids, x)
