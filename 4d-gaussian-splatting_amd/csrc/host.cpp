@@ -92,6 +92,9 @@ struct Written {
 
 std::string name_of(const at::Tensor& t) { return std::string("torch.") + (t.scalar_type() == at::kFloat ? "float32" : t.scalar_type() == at::kBFloat16 ? "bfloat16" : c10::toString(t.scalar_type())); }
 
+// In memory as it reads: elements one after another, and not a view whose negation is still to be done.
+bool plain(const at::Tensor& t) { return t.is_contiguous() && !t.is_neg(); }
+
 struct Moment { const at::Tensor *codes, *exps; bool is_signed; };
 
 bool is_moment(PyObject* o, PyObject* cls) { return (PyObject*)Py_TYPE(o) == cls || PyObject_IsInstance(o, cls) == 1; }
@@ -101,7 +104,7 @@ Moment moment8(PyObject* o, PyObject* cls, int64_t numel, const at::Device& devi
     const at::Tensor &c = tensor(PyTuple_GET_ITEM(o, 0), "codes"), &e = tensor(PyTuple_GET_ITEM(o, 1), "exponents");
     const int truth = PyObject_IsTrue(PyTuple_GET_ITEM(o, 2));
     if (truth < 0) throw Raised();
-    if (c.scalar_type() != at::kByte || e.scalar_type() != at::kByte || !c.is_contiguous() || !e.is_contiguous())
+    if (c.scalar_type() != at::kByte || e.scalar_type() != at::kByte || !plain(c) || !plain(e))
         value_error(what + ": codes and exponents are contiguous uint8 tensors");
     if (c.numel() != numel || e.numel() != (numel + FDGS_MOMENT8_BLOCK - 1) / FDGS_MOMENT8_BLOCK)
         value_error(what + ": one code per element, one exponent per " + std::to_string(FDGS_MOMENT8_BLOCK) + " elements");
@@ -188,13 +191,13 @@ PyObject* adamw_step(PyObject* a) {
         memset(&r, 0, sizeof(r));
         if (pt.scalar_type() != type || gt.scalar_type() != type)
             value_error("parameters and gradients of one step have one type: " + name_of(first) + ", " + name_of(pt) + " and " + name_of(gt) + " given");
-        if (gt.numel() != numel || !pt.is_contiguous()) value_error("a parameter has to be contiguous, and its gradient of its size");
+        if (gt.numel() != numel || !plain(pt)) value_error("a parameter has to be contiguous, and its gradient of its size");
         if (pt.device() != device || gt.device() != device) value_error("every tensor of a call is on one device");
         r.grad = gt.data_ptr();
-        if (!gt.is_contiguous()) {
+        if (!plain(gt)) {
             // rows that are contiguous runs a constant distance apart are read in place
             int64_t len = 1;
-            bool rows = gt.dim() >= 2 && gt.size(0) > 0 && gt.stride(0) > 0;
+            bool rows = !gt.is_neg() && gt.dim() >= 2 && gt.size(0) > 0 && gt.stride(0) > 0;
             for (int64_t d = gt.dim() - 1; rows && d >= 1; --d) {
                 if (gt.size(d) != 1 && gt.stride(d) != len) rows = false;
                 len *= gt.size(d);
@@ -203,7 +206,7 @@ PyObject* adamw_step(PyObject* a) {
                 r.grad_row_len = (int32_t)len;
                 r.grad_row_stride = gt.stride(0);
             } else {
-                hold.push_back(gt.detach().contiguous());
+                hold.push_back(gt.detach().resolve_neg().contiguous());
                 r.grad = hold.back().data_ptr();
             }
         }
@@ -221,14 +224,14 @@ PyObject* adamw_step(PyObject* a) {
                 PyObject* o = (k ? v : m).at(i);
                 if (!THPVariable_Check(o)) value_error("moments are float32 tensors, or all of them Moment8");
                 const at::Tensor& x = THPVariable_Unpack(o);
-                if (x.scalar_type() != at::kFloat || x.numel() != numel || !x.is_contiguous() || x.device() != device)
+                if (x.scalar_type() != at::kFloat || x.numel() != numel || !plain(x) || x.device() != device)
                     value_error("moments are contiguous float32 tensors of the parameter's size on its device, or all of them Moment8");
                 (k ? r.exp_avg_sq : r.exp_avg) = x.data_ptr();
             }
         }
         if (bf16) {
             const at::Tensor& x = tensor(PySequence_Fast_GET_ITEM(rseq.p, i), "residuals");
-            if (x.scalar_type() != at::kShort || x.numel() != numel || !x.is_contiguous() || x.device() != device)
+            if (x.scalar_type() != at::kShort || x.numel() != numel || !plain(x) || x.device() != device)
                 value_error("a residual is a contiguous int16 tensor of the parameter's size on its device");
             r.residual = (int16_t*)x.data_ptr();
         }
@@ -290,7 +293,7 @@ PyObject* moment8_convert(PyObject* a) {
     written.pieces.reserve((pack ? 2 : 1) * n);
     for (Py_ssize_t i = 0; i < n; ++i) {
         const at::Tensor& t = tensor(v.at(i), "values");
-        if (t.scalar_type() != type || t.device() != first.device() || !t.is_contiguous())
+        if (t.scalar_type() != type || t.device() != first.device() || !plain(t))
             value_error("the values of 8-bit moments are contiguous tensors of one type on one device");
         const Moment x = moment8(m.at(i), cls, t.numel(), t.device(), "moments");
         fdgs_moment8_tensor r;
@@ -340,12 +343,13 @@ int type_of(const Tensor& t, const char* what) {
 Tensor ids_of(const Tensor& ids, const at::Device& device) {
     if (ids.scalar_type() != at::kInt && ids.scalar_type() != at::kLong) value_error("ids are int32 or int64");
     if (ids.device() != device) value_error("ids and table have to be on one device");
-    return ids.contiguous();
+    return ids.resolve_neg().contiguous();
 }
 
 // t [lead..., row...] with rows that are contiguous runs a constant, not negative distance apart: t itself where it is
 // laid out so, else a copy.
-Tensor rows_of(const Tensor& t, int64_t lead, int64_t& width, int64_t& stride) {
+Tensor rows_of(const Tensor& t0, int64_t lead, int64_t& width, int64_t& stride) {
+    const Tensor t = t0.resolve_neg();
     width = 1;
     for (int64_t d = lead; d < t.dim(); ++d) width *= t.size(d);
     stride = width;

@@ -83,7 +83,7 @@ def pack8(values, signed, keys=None):
     signed = _each(signed, len(values), "signed")
     device = values[0].device
     _lib.require_gpu(values[0])
-    values = [t.contiguous() for t in values]
+    values = [t.resolve_neg().contiguous() for t in values]
     out = []
     for t, s in zip(values, signed):
         if t.dtype is not torch.float32 or t.device != device:

@@ -551,3 +551,27 @@ def test_update_is_the_formula_rounded_once_an_operation(bits, eps):
     denom = np.sqrt(v1) * f(1.0 / math.sqrt(1.0 - b2 ** t)) + f(eps)
     want = w * f(1.0 - lr * wd) - (m1 * f(lr / (1.0 - b1 ** t))) / denom
     assert want.dtype == f and np.array_equal(p.cpu().numpy().view(np.int32), want.view(np.int32))
+
+
+def test_views_that_are_still_to_be_negated():
+    """A gradient or a value that lies in memory with the other sign is read as what it is; what is written must lie as it reads."""
+    from fdgs.adamw import adamw_step, pack8, unpack8
+    z = torch.randn(6, 1, dtype=torch.complex64, device="cuda")
+    for neg in (z.conj().imag, torch._neg_view(z.imag.contiguous()), torch._neg_view(torch.randn(6, 9, device="cuda"))[:, :4]):
+        assert neg.is_neg()
+        moved = []
+        for g in (neg, neg.resolve_neg().contiguous()):
+            p, m, v = (torch.zeros(g.shape, device="cuda") for _ in range(3))
+            adamw_step([p], [g], [m], [v], steps=1, lr=0.1)
+            moved.append((p, m, v))
+            moved[-1] += (unpack8(pack8([g], True))[0],)
+        assert all(torch.equal(a, b) for a, b in zip(*moved)) and (moved[0][1] != 0).all()
+    x, y = torch._neg_view(torch.ones(8, device="cuda")), [torch.ones(8, device="cuda") for _ in range(3)]
+    for k, match in ((0, "contiguous"), (2, "contiguous"), (3, "contiguous")):
+        args = [[t] for t in (y[0], y[0].clone(), y[1], y[2])]
+        args[k] = [x]
+        with pytest.raises(ValueError, match=match):
+            adamw_step(*args, steps=1, lr=0.1)
+    with pytest.raises(ValueError, match="contiguous"):
+        unpack8(pack8([y[0]], True), out=[x])
+    assert (x == -1).all() and all((t == 1).all() for t in y)

@@ -514,3 +514,15 @@ def test_forward_derivatives_are_refused_on_the_device():
         y = embedding(ids, table.requires_grad_(True))
         with pytest.raises(RuntimeError, match="forward-mode"):          # out of a backward pass
             torch.autograd.grad(y, table, forward_ad.make_dual(tangent, tangent))
+
+
+def test_views_that_are_still_to_be_negated():
+    from fdgs.embedding import embedding, embedding_grad
+    z = torch.randn(6, 1, dtype=torch.complex64, device="cuda")
+    ids = torch.tensor([5, 0, 3, 3], device="cuda")
+    for x in (z.conj().imag, torch._neg_view(torch.randn(6, 4, device="cuda"))):
+        assert x.is_neg()
+        assert torch.equal(embedding(ids, x), embedding(ids, x.clone().resolve_neg()))
+        assert torch.equal(embedding(ids, x), x[ids].resolve_neg())
+        assert torch.equal(embedding_grad(x[:4], ids, 6), embedding_grad(x[:4].resolve_neg().contiguous(), ids, 6))
+    assert torch.equal(embedding(torch._neg_view(-ids), z.imag), z.imag[ids])

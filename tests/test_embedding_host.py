@@ -113,3 +113,12 @@ def test_forward_derivatives_are_refused():
                 embedding_grad(dual, ids, 3)
         with pytest.raises(RuntimeError, match="GPU only"):
             embedding(ids, x)
+
+
+def test_rows_of_views_that_are_still_to_be_negated():
+    """The imaginary part of a conjugate lies in memory with the other sign: it is never read in place."""
+    from fdgs._host import rows_layout
+    z = torch.zeros(6, 1, dtype=torch.complex64)
+    assert z.conj().imag.is_neg()
+    assert rows_layout(z.imag, 1) == (True, 1, 2) and rows_layout(z.conj().imag, 1) == (False, 1, 1)
+    assert rows_layout(torch._neg_view(torch.zeros(3, 4)), 1) == (False, 4, 4)
