@@ -95,11 +95,16 @@ std::string name_of(const at::Tensor& t) { return std::string("torch.") + (t.sca
 // In memory as it reads: elements one after another, and not a view whose negation is still to be done.
 bool plain(const at::Tensor& t) { return t.is_contiguous() && !t.is_neg(); }
 
+// Whether element i of the one is element i of the other, both contiguous: the shapes are equal, or one of them is flat.
+bool same_order(at::IntArrayRef a, at::IntArrayRef b) { return a == b || a.size() <= 1 || b.size() <= 1; }
+
 struct Moment { const at::Tensor *codes, *exps; bool is_signed; };
 
 bool is_moment(PyObject* o, PyObject* cls) { return (PyObject*)Py_TYPE(o) == cls || PyObject_IsInstance(o, cls) == 1; }
 
-Moment moment8(PyObject* o, PyObject* cls, int64_t numel, const at::Device& device, const std::string& what) {
+// of a tensor `like`: its parameter, or its values
+Moment moment8(PyObject* o, PyObject* cls, const at::Tensor& like, const std::string& what) {
+    const int64_t numel = like.numel();
     if (!is_moment(o, cls)) value_error(what + ": an 8-bit moment is an adamw.Moment8; do not mix moments in 8 and in 32 bits");
     const at::Tensor &c = tensor(PyTuple_GET_ITEM(o, 0), "codes"), &e = tensor(PyTuple_GET_ITEM(o, 1), "exponents");
     const int truth = PyObject_IsTrue(PyTuple_GET_ITEM(o, 2));
@@ -108,7 +113,8 @@ Moment moment8(PyObject* o, PyObject* cls, int64_t numel, const at::Device& devi
         value_error(what + ": codes and exponents are contiguous uint8 tensors");
     if (c.numel() != numel || e.numel() != (numel + FDGS_MOMENT8_BLOCK - 1) / FDGS_MOMENT8_BLOCK)
         value_error(what + ": one code per element, one exponent per " + std::to_string(FDGS_MOMENT8_BLOCK) + " elements");
-    if (c.device() != device || e.device() != device) value_error(what + ": every tensor of a call is on one device");
+    if (!same_order(c.sizes(), like.sizes())) value_error(what + ": codes have the shape of the tensor they belong to, or are flat");
+    if (c.device() != like.device() || e.device() != like.device()) value_error(what + ": every tensor of a call is on one device");
     return {&c, &e, truth != 0};
 }
 
@@ -191,7 +197,7 @@ PyObject* adamw_step(PyObject* a) {
         memset(&r, 0, sizeof(r));
         if (pt.scalar_type() != type || gt.scalar_type() != type)
             value_error("parameters and gradients of one step have one type: " + name_of(first) + ", " + name_of(pt) + " and " + name_of(gt) + " given");
-        if (gt.numel() != numel || !plain(pt)) value_error("a parameter has to be contiguous, and its gradient of its size");
+        if (gt.sizes() != pt.sizes() || !plain(pt)) value_error("a parameter has to be contiguous, and its gradient of its size and shape");
         if (pt.device() != device || gt.device() != device) value_error("every tensor of a call is on one device");
         r.grad = gt.data_ptr();
         if (!plain(gt)) {
@@ -211,7 +217,7 @@ PyObject* adamw_step(PyObject* a) {
             }
         }
         if (eight) {
-            const Moment mm = moment8(m.at(i), cls, numel, device, "exp_avgs"), vv = moment8(v.at(i), cls, numel, device, "exp_avg_sqs");
+            const Moment mm = moment8(m.at(i), cls, pt, "exp_avgs"), vv = moment8(v.at(i), cls, pt, "exp_avg_sqs");
             if (!mm.is_signed || vv.is_signed) value_error("the first moment is signed, the second is not");
             r.exp_avg = mm.codes->data_ptr();
             r.exp_avg_sq = vv.codes->data_ptr();
@@ -224,15 +230,15 @@ PyObject* adamw_step(PyObject* a) {
                 PyObject* o = (k ? v : m).at(i);
                 if (!THPVariable_Check(o)) value_error("moments are float32 tensors, or all of them Moment8");
                 const at::Tensor& x = THPVariable_Unpack(o);
-                if (x.scalar_type() != at::kFloat || x.numel() != numel || !plain(x) || x.device() != device)
-                    value_error("moments are contiguous float32 tensors of the parameter's size on its device, or all of them Moment8");
+                if (x.scalar_type() != at::kFloat || x.numel() != numel || !plain(x) || x.device() != device || !same_order(x.sizes(), pt.sizes()))
+                    value_error("moments are contiguous float32 tensors of the parameter's shape (or flat) on its device, or all of them Moment8");
                 (k ? r.exp_avg_sq : r.exp_avg) = x.data_ptr();
             }
         }
         if (bf16) {
             const at::Tensor& x = tensor(PySequence_Fast_GET_ITEM(rseq.p, i), "residuals");
-            if (x.scalar_type() != at::kShort || x.numel() != numel || !plain(x) || x.device() != device)
-                value_error("a residual is a contiguous int16 tensor of the parameter's size on its device");
+            if (x.scalar_type() != at::kShort || x.numel() != numel || !plain(x) || x.device() != device || !same_order(x.sizes(), pt.sizes()))
+                value_error("a residual is a contiguous int16 tensor of the parameter's shape (or flat) on its device");
             r.residual = (int16_t*)x.data_ptr();
         }
         const long long step = steps.whole(i);
@@ -295,7 +301,7 @@ PyObject* moment8_convert(PyObject* a) {
         const at::Tensor& t = tensor(v.at(i), "values");
         if (t.scalar_type() != type || t.device() != first.device() || !plain(t))
             value_error("the values of 8-bit moments are contiguous tensors of one type on one device");
-        const Moment x = moment8(m.at(i), cls, t.numel(), t.device(), "moments");
+        const Moment x = moment8(m.at(i), cls, t, "moments");
         fdgs_moment8_tensor r;
         memset(&r, 0, sizeof(r));
         r.codes = (uint8_t*)x.codes->data_ptr();

@@ -575,3 +575,39 @@ def test_views_that_are_still_to_be_negated():
     with pytest.raises(ValueError, match="contiguous"):
         unpack8(pack8([y[0]], True), out=[x])
     assert (x == -1).all() and all((t == 1).all() for t in y)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("bf16", [False, True])
+def test_tensors_of_another_shape_are_refused(bits, bf16):
+    """As many elements in another order are not the parameter's; flat ones are."""
+    from fdgs.adamw import Moment8, adamw_step, unpack8
+    kind = torch.bfloat16 if bf16 else torch.float32
+
+    def args(shapes):
+        p, g, m, v, low = shapes
+        make = (lambda s, signed: Moment8.zeros_like(torch.empty(s, device="cuda"), signed)) if bits == 8 else \
+            (lambda s, signed: torch.zeros(s, device="cuda"))
+        return dict(params=[torch.ones(p, dtype=kind, device="cuda")], grads=[torch.ones(g, dtype=kind, device="cuda")],
+                    exp_avgs=[make(m, True)], exp_avg_sqs=[make(v, False)], steps=1, lr=0.1, keys=[3] if bits == 8 else None,
+                    residuals=[torch.zeros(low, dtype=torch.int16, device="cuda")] if bf16 else None)
+    right, other, flat = (30, 40), (40, 30), (1200,)
+    for k in range(5 if bf16 else 4):
+        for shape in (other, (30, 40, 1), (1, 30, 40)):
+            bad = args([shape if j == k else right for j in range(5)])
+            with pytest.raises(ValueError, match="shape"):
+                adamw_step(**bad)
+            assert (bad["params"][0] == 1).all()
+    with pytest.raises(ValueError, match="shape"):
+        adamw_step(**args([right, flat, right, right, right]))           # a flat gradient of a matrix neither
+    ends = []
+    for shapes in ([right] * 5, [right, right, flat, flat, flat], [flat, flat, right, right, right]):
+        a = args(shapes)
+        adamw_step(**a)
+        ends.append(a["params"][0].reshape(-1))
+    assert torch.equal(ends[0], ends[1]) and torch.equal(ends[0], ends[2]) and (ends[0] != 1).all()
+    if bits == 8:
+        m = Moment8.zeros_like(torch.empty(right, device="cuda"), True)
+        with pytest.raises(ValueError, match="shape"):
+            unpack8([m], out=[torch.ones(other, device="cuda")])
+        assert (unpack8([m], out=[torch.ones(flat, device="cuda")])[0] == 0).all()
