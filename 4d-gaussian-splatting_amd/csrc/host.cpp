@@ -12,6 +12,7 @@
 #include <c10/hip/HIPStream.h>
 #include <algorithm>
 #include <cstring>
+#include <memory>
 #include <stdexcept>
 #include <string>
 #include <unordered_set>
@@ -79,14 +80,68 @@ struct Each {
     }
 };
 
-// The memory that a call writes: two pieces that overlap would be written by workgroups that do not wait for each other.
-struct Written {
-    std::vector<std::pair<uintptr_t, size_t>> pieces;
-    void add(const void* p, size_t bytes) { if (bytes) pieces.emplace_back((uintptr_t)p, bytes); }
+// The memory that a call writes, and what it reads beside: a piece that is written and another one that overlaps it would be touched by
+// workgroups that do not wait for each other.  The pieces of a list of tensors often lie in the list's order, so that the lists only need
+// merging (a step over 211 tensors with 8-bit moments looks at 1266 pieces).
+struct Touched {
+    struct Piece { uintptr_t at, end; size_t rows; };                    // rows: 0, or 1 + its place in that list
+    struct Rows { size_t row, step; };                                   // only rows of `row` bytes, `step` apart, are read of a piece
+    const int written, lists;                                            // the first `written` lists are written
+    const size_t n;
+    std::unique_ptr<Piece[]> pieces;                                     // [lists][n]
+    size_t count[8] = {};
+    std::vector<Rows> rows;
+    Touched(int w, int r, size_t each) : written(w), lists(w + r), n(each), pieces(new Piece[(w + r) * each]) {}
+    void add(int list, const void* p, size_t bytes, size_t in_rows = 0) {
+        if (bytes) pieces[list * n + count[list]++] = {(uintptr_t)p, (uintptr_t)p + bytes, in_rows};
+    }
+    void add_rows(int list, const void* p, size_t number, size_t row, size_t step) {
+        rows.push_back({row, step});
+        add(list, p, (number - 1) * step + row, rows.size());
+    }
+    bool meet(const Piece& w, const Piece& o) const {
+        if (o.at >= w.end || w.at >= o.end || o.rows == 0) return o.at < w.end && w.at < o.end;
+        // the first row that ends behind w's beginning: does it begin before w's end?
+        const Rows r = rows[o.rows - 1];
+        const size_t k = w.at < o.at + r.row ? 0 : (w.at - o.at - r.row) / r.step + 1;
+        return o.at + k * r.step < std::min(w.end, o.end);
+    }
     void check() {
-        std::sort(pieces.begin(), pieces.end(), [](const auto& a, const auto& b) { return a.first < b.first; });
-        for (size_t i = 1; i < pieces.size(); ++i)
-            if (pieces[i - 1].first + pieces[i - 1].second > pieces[i].first) value_error("a tensor is in the lists twice, or two of them overlap");
+        for (int l = 0; l < lists; ++l) {
+            Piece *first = &pieces[l * n], *last = first + count[l];
+            const auto less = [](const Piece& a, const Piece& b) { return a.at < b.at; };
+            if (!std::is_sorted(first, last, less)) std::sort(first, last, less);
+        }
+        const Piece none = {UINTPTR_MAX, UINTPTR_MAX, 0}, *head[8], *stop[8];
+        uintptr_t next[8], end_written = 0, end = 0;
+        for (int l = 0; l < lists; ++l) {
+            head[l] = &pieces[l * n];
+            stop[l] = head[l] + count[l];
+            next[l] = count[l] ? head[l]->at : none.at;
+        }
+        for (bool apart = true; apart;) {
+            int l = 0;                               // the list that goes on, and where another one does
+            uintptr_t limit = none.at;
+            for (int k = 1; k < lists; ++k) {
+                limit = std::min(limit, std::max(next[k], next[l]));
+                l = next[k] < next[l] ? k : l;
+            }
+            if (next[l] == none.at) return;
+            const Piece* p = head[l];
+            do {
+                apart = p->at >= (l < written ? end : end_written);
+                end = std::max(end, p->end);
+                if (l < written) end_written = std::max(end_written, p->end);
+            } while (apart && ++p != stop[l] && p->at <= limit);
+            head[l] = p;
+            next[l] = p != stop[l] ? p->at : none.at;
+        }
+        for (int l = 0; l < written; ++l)            // two pieces' spans overlap: also what lies in them?
+            for (size_t i = 0; i < count[l]; ++i)
+                for (int k = l; k < lists; ++k)
+                    for (size_t j = k == l ? i + 1 : 0; j < count[k]; ++j)
+                        if (meet(pieces[l * n + i], pieces[k * n + j]))
+                            value_error(k < written ? "a tensor is in the lists twice, or two of them overlap" : "what a call reads and what it writes must not overlap");
     }
 };
 
@@ -96,7 +151,7 @@ std::string name_of(const at::Tensor& t) { return std::string("torch.") + (t.sca
 bool plain(const at::Tensor& t) { return t.is_contiguous() && !t.is_neg(); }
 
 // Whether element i of the one is element i of the other, both contiguous: the shapes are equal, or one of them is flat.
-bool same_order(at::IntArrayRef a, at::IntArrayRef b) { return a == b || a.size() <= 1 || b.size() <= 1; }
+bool same_order(at::IntArrayRef a, at::IntArrayRef b) { return a.size() <= 1 || b.size() <= 1 || a == b; }
 
 struct Moment { const at::Tensor *codes, *exps; bool is_signed; };
 
@@ -188,16 +243,17 @@ PyObject* adamw_step(PyObject* a) {
         value_error("8-bit moments need keys: a number for each tensor, others at every step");
     std::vector<Tensor> hold;                        // copies of gradients, kept until the kernels are on the stream
     std::vector<fdgs_adamw_tensor> out(n);
-    Written written;
-    written.pieces.reserve((eight ? 5 : 3) * n + (bf16 ? n : 0));
+    const int P = 0, M = 1, V = 2, LOW = 3, ME = bf16 ? 4 : 3, VE = ME + 1, G = eight ? VE + 1 : ME;    // the gradients behind what is written
+    Touched touched(G, 1, n);
     for (Py_ssize_t i = 0; i < n; ++i) {
         const at::Tensor &pt = tensor(p.at(i), "params"), &gt = tensor(g.at(i), "grads");
         const int64_t numel = pt.numel();
+        const at::IntArrayRef shape = pt.sizes();
         fdgs_adamw_tensor r;
         memset(&r, 0, sizeof(r));
         if (pt.scalar_type() != type || gt.scalar_type() != type)
             value_error("parameters and gradients of one step have one type: " + name_of(first) + ", " + name_of(pt) + " and " + name_of(gt) + " given");
-        if (gt.sizes() != pt.sizes() || !plain(pt)) value_error("a parameter has to be contiguous, and its gradient of its size and shape");
+        if (gt.sizes() != shape || !plain(pt)) value_error("a parameter has to be contiguous, and its gradient of its size and shape");
         if (pt.device() != device || gt.device() != device) value_error("every tensor of a call is on one device");
         r.grad = gt.data_ptr();
         if (!plain(gt)) {
@@ -211,10 +267,14 @@ PyObject* adamw_step(PyObject* a) {
             if (rows && len > 0 && gt.stride(0) >= len && len <= INT32_MAX) {
                 r.grad_row_len = (int32_t)len;
                 r.grad_row_stride = gt.stride(0);
+                const size_t size = bf16 ? 2 : 4;
+                touched.add_rows(G, r.grad, gt.size(0), len * size, gt.stride(0) * size);
             } else {
                 hold.push_back(gt.detach().resolve_neg().contiguous());
                 r.grad = hold.back().data_ptr();
             }
+        } else {
+            touched.add(G, r.grad, numel * (bf16 ? 2 : 4));
         }
         if (eight) {
             const Moment mm = moment8(m.at(i), cls, pt, "exp_avgs"), vv = moment8(v.at(i), cls, pt, "exp_avg_sqs");
@@ -230,14 +290,14 @@ PyObject* adamw_step(PyObject* a) {
                 PyObject* o = (k ? v : m).at(i);
                 if (!THPVariable_Check(o)) value_error("moments are float32 tensors, or all of them Moment8");
                 const at::Tensor& x = THPVariable_Unpack(o);
-                if (x.scalar_type() != at::kFloat || x.numel() != numel || !plain(x) || x.device() != device || !same_order(x.sizes(), pt.sizes()))
+                if (x.scalar_type() != at::kFloat || x.numel() != numel || !plain(x) || x.device() != device || !same_order(x.sizes(), shape))
                     value_error("moments are contiguous float32 tensors of the parameter's shape (or flat) on its device, or all of them Moment8");
                 (k ? r.exp_avg_sq : r.exp_avg) = x.data_ptr();
             }
         }
         if (bf16) {
             const at::Tensor& x = tensor(PySequence_Fast_GET_ITEM(rseq.p, i), "residuals");
-            if (x.scalar_type() != at::kShort || x.numel() != numel || !plain(x) || x.device() != device || !same_order(x.sizes(), pt.sizes()))
+            if (x.scalar_type() != at::kShort || x.numel() != numel || !plain(x) || x.device() != device || !same_order(x.sizes(), shape))
                 value_error("a residual is a contiguous int16 tensor of the parameter's shape (or flat) on its device");
             r.residual = (int16_t*)x.data_ptr();
         }
@@ -248,18 +308,18 @@ PyObject* adamw_step(PyObject* a) {
         r.step = (int32_t)step;
         r.lr = lr.number(i);
         r.weight_decay = wd.number(i);
-        written.add(r.param, numel * (bf16 ? 2 : 4));
-        written.add(r.exp_avg, numel * (eight ? 1 : 4));
-        written.add(r.exp_avg_sq, numel * (eight ? 1 : 4));
-        if (bf16) written.add(r.residual, numel * 2);
+        touched.add(P, r.param, numel * (bf16 ? 2 : 4));
+        touched.add(M, r.exp_avg, numel * (eight ? 1 : 4));
+        touched.add(V, r.exp_avg_sq, numel * (eight ? 1 : 4));
+        if (bf16) touched.add(LOW, r.residual, numel * 2);
         if (eight) {
             const int64_t blocks = (numel + FDGS_MOMENT8_BLOCK - 1) / FDGS_MOMENT8_BLOCK;
-            written.add(r.exp_avg_exponents, blocks);
-            written.add(r.exp_avg_sq_exponents, blocks);
+            touched.add(ME, r.exp_avg_exponents, blocks);
+            touched.add(VE, r.exp_avg_sq_exponents, blocks);
         }
         out[i] = r;
     }
-    written.check();
+    touched.check();
     fdgs_adamw_args args;
     memset(&args, 0, sizeof(args));
     args.num_tensors = (int32_t)n;
@@ -295,8 +355,8 @@ PyObject* moment8_convert(PyObject* a) {
     if (type != at::kFloat && type != at::kBFloat16) value_error("the values of 8-bit moments are float32 or bfloat16");
     on_gpu(first);
     std::vector<fdgs_moment8_tensor> out(n);
-    Written written;
-    written.pieces.reserve((pack ? 2 : 1) * n);
+    const int V = pack ? 2 : 0, C = pack ? 0 : 1, E = C + 1;             // values, codes, exponents: what is written first
+    Touched touched(pack ? 2 : 1, pack ? 1 : 2, n);
     for (Py_ssize_t i = 0; i < n; ++i) {
         const at::Tensor& t = tensor(v.at(i), "values");
         if (t.scalar_type() != type || t.device() != first.device() || !plain(t))
@@ -310,15 +370,12 @@ PyObject* moment8_convert(PyObject* a) {
         r.numel = t.numel();
         r.is_signed = x.is_signed;
         r.round_key = ko == Py_None ? 0u : keys.low32(i);
-        if (pack) {
-            written.add(r.codes, r.numel);
-            written.add(r.exponents, (r.numel + FDGS_MOMENT8_BLOCK - 1) / FDGS_MOMENT8_BLOCK);
-        } else {
-            written.add(r.value, r.numel * t.element_size());
-        }
+        touched.add(V, r.value, r.numel * t.element_size());
+        touched.add(C, r.codes, r.numel);
+        touched.add(E, r.exponents, (r.numel + FDGS_MOMENT8_BLOCK - 1) / FDGS_MOMENT8_BLOCK);
         out[i] = r;
     }
-    written.check();
+    touched.check();
     fdgs_moment8_args args;
     memset(&args, 0, sizeof(args));
     args.num_tensors = (int32_t)n;

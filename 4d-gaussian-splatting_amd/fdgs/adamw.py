@@ -54,7 +54,7 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, steps, lr, betas=(0.9, 0
     and for bfloat16 params `residuals` (int16), each of its parameter's shape or flat.  grads: the parameters' type and shape;
     contiguous, or column slices of wider row-major arrays (read in place), anything else is copied.  steps (1-based), lr and weight_decay: one value, or
     one for each tensor.  keys: for 8-bit moments, 32-bit numbers, one for each tensor, others at every step.
-    All tensors are on one GPU, have one type, do not overlap, and the step runs on its current stream.  Tensors
+    All tensors are on one GPU, have one type, and the step runs on its current stream; no tensor that it writes overlaps another one.  Tensors
     without elements are passed over.  The call reads steps, lr and keys on the host: a captured graph would replay
     the ones it was captured with, so a stream that is being captured is refused."""
     _host.adamw_step(params, grads, exp_avgs, exp_avg_sqs, residuals, steps, lr, weight_decay, keys, Moment8, *betas, eps)
@@ -63,7 +63,8 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, steps, lr, betas=(0.9, 0
 
 def unpack8(moments, dtype=torch.float32, out=None):
     """The values that a list of Moment8 stands for: float32 or bfloat16 tensors (both exact) of the codes' shapes,
-    written into `out` (a list of contiguous tensors of one type, of the codes' shapes or flat) where it is given."""
+    written into `out` (a list of contiguous tensors of one type, of the codes' shapes or flat, none of which
+    overlaps another or the moments) where it is given."""
     moments = list(moments)
     if not moments:
         return []

@@ -611,3 +611,88 @@ def test_tensors_of_another_shape_are_refused(bits, bf16):
         with pytest.raises(ValueError, match="shape"):
             unpack8([m], out=[torch.ones(other, device="cuda")])
         assert (unpack8([m], out=[torch.ones(flat, device="cuda")])[0] == 0).all()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("bf16", [False, True])
+def test_reads_that_overlap_writes_are_refused(bits, bf16):
+    """A gradient inside what the step writes, whole or by one element, in one piece or in rows; not rows beside it."""
+    from fdgs.adamw import Moment8, adamw_step
+    kind = torch.bfloat16 if bf16 else torch.float32
+    n = 1203
+
+    def step(p, grads):
+        make = (lambda x, s: Moment8.zeros_like(x, s)) if bits == 8 else (lambda x, s: torch.zeros(x.shape, device="cuda"))
+        args = dict(params=p, grads=grads, exp_avgs=[make(x, True) for x in p], exp_avg_sqs=[make(x, False) for x in p], steps=1, lr=0.1,
+                    residuals=[torch.zeros(x.shape, dtype=torch.int16, device="cuda") for x in p] if bf16 else None,
+                    keys=list(range(len(p))) if bits == 8 else None)
+        return args
+    both = torch.ones(4 * n, dtype=kind, device="cuda")
+    other = [torch.ones(77, dtype=kind, device="cuda"), torch.ones(77, dtype=kind, device="cuda")]
+    p = both[n:2 * n]
+    for g in (p, both[:n + 1][-n:], both[2 * n - 1:3 * n - 1], both[n + 5:2 * n + 5]):
+        for order in (slice(None), slice(None, None, -1)):
+            args = step([other[0], p][order], [other[1], g][order])
+            with pytest.raises(ValueError, match="overlap"):
+                adamw_step(**args)
+    for k in ("exp_avgs", "exp_avg_sqs") + (("residuals",) if bf16 else ()):     # the gradient lies in another tensor of the step
+        args = step([p], [both[:n]])
+        t = args[k][0]
+        pieces = t[:2] if isinstance(t, tuple) else (t,)
+        for x in pieces:
+            raw = torch.empty(0, dtype=kind, device="cuda").set_(x.untyped_storage(), 0, (1,), (1,))
+            args["params"].append(torch.ones(1, dtype=kind, device="cuda"))
+            args["grads"].append(raw)
+            for name in ("exp_avgs", "exp_avg_sqs", "residuals", "keys"):
+                if args[name] is not None:
+                    more = step([args["params"][-1]], [raw])
+                    args[name].append(more[name][0])
+            with pytest.raises(ValueError, match="overlap"):
+                adamw_step(**args)
+            for name in ("params", "grads", "exp_avgs", "exp_avg_sqs", "residuals", "keys"):
+                if args[name] is not None:
+                    args[name].pop()
+    # rows of a wider array: a written piece in their gaps is beside them, one that reaches into a row is not
+    wide = torch.ones(100, 16, dtype=kind, device="cuda")
+    sliced = torch.ones(100, 6, dtype=kind, device="cuda")
+    for row in (0, 50, 99):
+        for lo, hi, fine in ((6, 16, True), (5, 16, False), (0, 6, False), (2, 3, False), (7, 8, True)):
+            piece = wide[row, lo:hi]
+            args = step([sliced, piece], [wide[:, :6], torch.ones_like(piece)])
+            if fine:
+                adamw_step(**args)
+                assert (piece != 1).all() and (wide[:, :6] == 1).all()
+                piece.fill_(1)
+            else:
+                with pytest.raises(ValueError, match="overlap"):
+                    adamw_step(**args)
+    flat = wide.view(-1)
+    for at, fine in ((6 + 50 * 16, True), (5 + 50 * 16, False), (7 + 50 * 16, False), (6 + 99 * 16, True)):      # over a row's end
+        piece = flat[at:at + 10]
+        args = step([sliced, piece], [wide[:, :6], torch.ones_like(piece)])
+        if fine:
+            adamw_step(**args)
+            piece.fill_(1)
+        else:
+            with pytest.raises(ValueError, match="overlap"):
+                adamw_step(**args)
+    assert (wide == 1).all() and (both == 1).all()
+
+
+def test_conversions_refuse_results_in_their_codes():
+    from fdgs.adamw import Moment8, pack8, unpack8
+    raw = torch.zeros(6000, dtype=torch.uint8, device="cuda")
+    values = raw.view(torch.float32)
+    ones, = pack8([torch.ones(300, device="cuda")], True)
+    for codes_at, exps_at, out_at, fine in ((0, 3000, 75, True), (0, 3000, 74, False), (1203, 3000, 0, True), (1199, 3000, 0, False),
+                                            (0, 1199, 0, False), (1200, 1500, 0, True), (3000, 602, 150, False), (3000, 598, 150, True)):
+        m = Moment8(raw[codes_at:codes_at + 300], raw[exps_at:exps_at + 2], True)
+        out = values[out_at:out_at + 300]
+        raw.zero_()
+        m.codes.copy_(ones.codes)
+        m.exponents.copy_(ones.exponents)
+        if fine:
+            assert (unpack8([m, m], out=[out, torch.empty(300, device="cuda")])[0] == 1).all()       # one moment twice may be read
+        else:
+            with pytest.raises(ValueError, match="overlap"):
+                unpack8([ones, m], out=[torch.empty(300, device="cuda"), out])
