@@ -173,6 +173,11 @@ Moment moment8(PyObject* o, PyObject* cls, const at::Tensor& like, const std::st
     return {&c, &e, truth != 0};
 }
 
+// Written in place: a graph that has saved the tensor is to notice, as after torch's own operations.
+void changed(const at::Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 void on_gpu(const at::Tensor& t) {
     if (!t.is_cuda()) throw Refused{PyExc_RuntimeError, "libfdgs kernels run on the GPU only; got a tensor on " + t.device().str()};
 }
@@ -333,11 +338,7 @@ PyObject* adamw_step(PyObject* a) {
     const Tensor workspace = args.workspace_bytes ? at::empty({(int64_t)args.workspace_bytes}, first.options().dtype(at::kByte).requires_grad(false)) : Tensor();
     args.workspace = args.workspace_bytes ? workspace.data_ptr() : nullptr;
     launch("fdgs_adamw_step", library.adamw, args, device);
-    // written in place: a graph that has saved a parameter is to notice, as after torch's own steps
-    for (Py_ssize_t i = 0; i < n; ++i) {
-        const Tensor& t = THPVariable_Unpack(p.at(i));
-        if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
-    }
+    for (Py_ssize_t i = 0; i < n; ++i) changed(THPVariable_Unpack(p.at(i)));     // the state is the optimizer's own
     Py_RETURN_NONE;
 }
 
@@ -387,6 +388,7 @@ PyObject* moment8_convert(PyObject* a) {
     const Tensor workspace = args.workspace_bytes ? at::empty({(int64_t)args.workspace_bytes}, first.options().dtype(at::kByte)) : Tensor();
     args.workspace = args.workspace_bytes ? workspace.data_ptr() : nullptr;
     launch(pack ? "fdgs_moment8_pack" : "fdgs_moment8_unpack", pack ? library.pack8 : library.unpack8, args, first.device());
+    for (Py_ssize_t i = 0; i < n && !pack; ++i) changed(THPVariable_Unpack(v.at(i)));
     Py_RETURN_NONE;
 }
 

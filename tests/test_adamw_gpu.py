@@ -696,3 +696,17 @@ def test_conversions_refuse_results_in_their_codes():
         else:
             with pytest.raises(ValueError, match="overlap"):
                 unpack8([ones, m], out=[torch.empty(300, device="cuda"), out])
+
+
+def test_a_read_out_is_seen_by_saved_graphs():
+    """A graph that has saved the tensor raises in its backward pass once unpack8 has written it."""
+    from fdgs.adamw import pack8, unpack8
+    ms = pack8([torch.ones(8, device="cuda")], False)
+    out, w = torch.full((8,), 3.0, device="cuda"), torch.ones(8, device="cuda", requires_grad=True)
+    loss = (w * out).sum()
+    unpack8(ms, out=[out])
+    assert (out == 1).all()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    with torch.inference_mode():                             # tensors without a version
+        assert (unpack8(pack8([torch.ones(8, device="cuda")], False))[0] == 1).all()
