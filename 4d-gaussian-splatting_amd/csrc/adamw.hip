@@ -447,7 +447,7 @@ extern "C" int fdgs_adamw_step(const fdgs_adamw_args* a, void* stream) {
         if (s.grad_row_len > 0 && s.grad_row_stride < s.grad_row_len) return FDGS_EINVAL;
         if (s.numel == 0) continue;
         total += (s.numel - 1) / AW_PER_GROUP + 1;
-        if (total > 0x7fffffffLL) return FDGS_ETOOLARGE;
+        if (total > FDGS_MAX_GROUPS(AW_THREADS)) return FDGS_ETOOLARGE;
         if (!s.param || !s.grad || !s.exp_avg || !s.exp_avg_sq || (bf16 && !s.residual)) return FDGS_EINVAL;
         if (eight && (!s.exp_avg_exponents || !s.exp_avg_sq_exponents)) return FDGS_EINVAL;
     }
@@ -651,7 +651,7 @@ static int moment8_launch(const fdgs_moment8_args* a, void* stream, bool pack) {
         if (s.numel == 0) continue;
         if (!s.codes || !s.exponents || !s.value) return FDGS_EINVAL;
         total += (s.numel - 1) / M8_PER_GROUP + 1;
-        if (total > 0x7fffffffLL) return FDGS_ETOOLARGE;
+        if (total > FDGS_MAX_GROUPS(256)) return FDGS_ETOOLARGE;
     }
     int i = 0;
     auto next = [&](M8Tensor& t, int& groups) {

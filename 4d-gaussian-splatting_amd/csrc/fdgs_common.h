@@ -12,6 +12,9 @@
         if (hipGetLastError() != hipSuccess) return FDGS_ELAUNCH; \
     } while (0)
 
+// HIP takes fewer than 2^32 threads in a dimension of a grid: the workgroups of `threads` that one launch may have.
+#define FDGS_MAX_GROUPS(threads) ((1ll << 32) / (threads) - 1)
+
 // Rasterizer constants (the published tile-rasterizer algorithm).
 #define FDGS_NEAR_Z 0.2f
 #define FDGS_COV_DILATION 0.3f

@@ -492,7 +492,8 @@ int fdgs_adam_step(const fdgs_adam_args* a, void* stream);
  * stochastically, by 16 bits each of a hash of the element's index and `round_key`: give every tensor and step a key of
  * its own, and every replica the same one.  A second moment that is not zero is never rounded to zero.
  *
- * The tensors must not overlap, and not two records may name the same one.                          */
+ * What the step writes must not overlap another tensor, and not two records may name the same one.  A call has fewer than 2^34
+ * elements (the conversions below 2^36), counting whole workgroups of 2048 (4096) for each tensor: else FDGS_ETOOLARGE.   */
 #define FDGS_TYPE_F32 0
 #define FDGS_TYPE_BF16 1
 #define FDGS_TYPE_F16 2

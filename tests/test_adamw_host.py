@@ -145,3 +145,19 @@ def test_optimizer_refuses_what_it_does_not_do():
     half = torch.zeros(4, dtype=torch.float16)
     with pytest.raises(ValueError, match="float32 and bfloat16"):
         FusedAdamW([half])._new_state(half)
+
+
+def test_steps_and_conversions_that_no_grid_holds_are_refused():
+    """A launch has fewer than 2^32 threads: 2^23 workgroups of 512 for 2048 elements each, 2^24 of 256 for 4096."""
+    from fdgs import _lib, _records
+    lib = _lib.lib
+    for each, most in ((2048, 1 << 23), (4096, 1 << 24)):
+        for sizes in ([each * most], [each * most - each + 1], [each * most // 2, each * most // 2 - 5], [each * (most - 1), 1]):
+            n = len(sizes)
+            if each == 2048:
+                recs = (_records.AdamWTensor * n)(*[_records.AdamWTensor(param=64, grad=64, exp_avg=64, exp_avg_sq=64, numel=k, step=1) for k in sizes])
+                assert lib.fdgs_adamw_step(C.byref(_records.AdamWArgs(n, 0, 32, 0, 0.9, 0.9, 0.0, C.cast(recs, C.c_char_p))), None) == -4
+                continue
+            for name in ("fdgs_moment8_pack", "fdgs_moment8_unpack"):
+                recs = (_records.Moment8Tensor * n)(*[_records.Moment8Tensor(codes=64, exponents=64, value=64, numel=k) for k in sizes])
+                assert getattr(lib, name)(C.byref(_records.Moment8Args(n, 0, 1, 0, C.cast(recs, C.c_char_p))), None) == -4
