@@ -13,6 +13,7 @@
 // of one frequent row or the zeros of many rows that nobody asked for.  A row that is cut by a share's end leaves
 // partial sums in the workspace, which a last launch adds up in the shares' order.  No atomic touches a sum.
 #include "fdgs_common.h"
+#include <algorithm>
 #include <type_traits>
 
 // ---- element types: 16 bytes to a vector where the row is that long, else one element ----
@@ -1009,7 +1010,8 @@ static EmSortPlan em_sort_plan(long long tokens) {
 
 struct EmPlan {
     int vec, nv, tiles, lanes, groups, share;
-    long long shares, blocks;
+    int join_tiles, join_lanes;
+    long long shares, blocks, joins;                 // blocks and joins: workgroups in x
     size_t sorted, sort, info, fresh, head, tail, bytes;   // offsets into the workspace
 };
 
@@ -1032,6 +1034,11 @@ static EmPlan em_plan(long long tokens, long long rows, int dim, int type) {
     while (p.groups * p.share > EW_ITEMS) p.share >>= 1;
     p.blocks = (tokens + rows + (long long)p.groups * p.share - 1) / ((long long)p.groups * p.share);
     p.shares = p.blocks * p.groups;
+    // at most 64 lanes to a row in the join, so that there are groups to divide the partial sums of a long one
+    p.join_tiles = (p.nv + 63) / 64;
+    p.join_lanes = (p.nv + p.join_tiles - 1) / p.join_tiles;
+    const int scan = EC_SCAN(EW_THREADS / p.join_lanes);
+    p.joins = (p.shares + scan - 1) / scan;
     size_t at = 0;
     auto take = [&at](size_t n) { const size_t o = at; at += (n + 255) / 256 * 256; return o; };
     p.sorted = take(tokens * 8);
@@ -1166,14 +1173,23 @@ extern "C" int fdgs_embedding_fwd(const fdgs_embedding_fwd_args* a, void* stream
         if (a->workspace_bytes < em_sort_plan(a->num_tokens).bytes || (a->workspace_bytes > 0 && !a->workspace)) return FDGS_EWORKSPACE;
         const EmIds in = {a->ids, k.padding, (uint32_t)a->num_rows, k.tokens, k.wide};
         f.by_tiles = em_div_of((uint32_t)tiles);
-        const bool beside = groups * tiles <= 0x3fffffffLL;
+        // (in one launch of the sort there are at most 1024 workgroups of 256 threads, or as many threads, beside them)
+        const bool beside = groups * tiles <= FDGS_MAX_GROUPS(EF_THREADS) - 2048;
         EM_RUN(em_sort(in, (uint2*)a->sorted, (char*)a->workspace, beside ? &f : nullptr, groups * tiles, s));
         if (beside) return FDGS_OK;
     }
-    const dim3 grid((unsigned)groups, (unsigned)tiles);
-    if (a->type == FDGS_TYPE_F32) return em_fwd_launch<EmF32>(k, f.vec, grid, s);
-    if (a->type == FDGS_TYPE_BF16) return em_fwd_launch<EmBf16>(k, f.vec, grid, s);
-    return em_fwd_launch<EmF16>(k, f.vec, grid, s);
+    for (long long g = 0; g < groups; g += FDGS_MAX_GROUPS(EF_THREADS)) {
+        const long long now = std::min(groups - g, FDGS_MAX_GROUPS(EF_THREADS)), token = g * k.per_group;
+        EmFwd part = k;
+        part.ids = (const char*)k.ids + token * a->id_bytes;
+        part.out = (char*)k.out + token * row;
+        part.tokens = (int)std::min(k.tokens - token, now * k.per_group);
+        const dim3 grid((unsigned)now, (unsigned)tiles);
+        if (a->type == FDGS_TYPE_F32) EM_RUN(em_fwd_launch<EmF32>(part, f.vec, grid, s));
+        else if (a->type == FDGS_TYPE_BF16) EM_RUN(em_fwd_launch<EmBf16>(part, f.vec, grid, s));
+        else EM_RUN(em_fwd_launch<EmF16>(part, f.vec, grid, s));
+    }
+    return FDGS_OK;
 }
 
 template <class T>
@@ -1188,13 +1204,10 @@ static int em_bwd_launch(const EmBwd& k, const EmPlan& p, hipStream_t s) {
     if (p.vec > 1) hipLaunchKernelGGL((embedding_walk_kernel<T, T::full, false>), grid, threads, 0, s, k);
     else hipLaunchKernelGGL((embedding_walk_kernel<T, 1, false>), grid, threads, 0, s, k);
     FDGS_CHECK_LAUNCH();
-    // at most 64 lanes to a row here, so that there are groups to divide the partial sums of a long one
     EmBwd j = k;
-    const int tiles = (p.nv + 63) / 64;
-    j.lanes = (p.nv + tiles - 1) / tiles;
-    j.groups = EW_THREADS / j.lanes;
-    const int scan = EC_SCAN(j.groups);
-    const dim3 joins((unsigned)((p.shares + scan - 1) / scan), (unsigned)tiles);
+    j.lanes = p.join_lanes;
+    j.groups = EW_THREADS / p.join_lanes;
+    const dim3 joins((unsigned)p.joins, (unsigned)p.join_tiles);
     if (p.vec == 1) hipLaunchKernelGGL((embedding_join_kernel<T, 1, true>), joins, threads, 0, s, j);
     else if (p.groups > 1) hipLaunchKernelGGL((embedding_join_kernel<T, T::full, true>), joins, threads, 0, s, j);
     else hipLaunchKernelGGL((embedding_join_kernel<T, T::full, false>), joins, threads, 0, s, j);
@@ -1210,7 +1223,7 @@ extern "C" int fdgs_embedding_bwd(const fdgs_embedding_bwd_args* a, void* stream
     if (a->dim > FDGS_EMBEDDING_MAX_DIM || a->num_tokens > FDGS_EMBEDDING_MAX_TOKENS) return FDGS_ETOOLARGE;
     const EmPlan p = em_plan(a->num_tokens, a->num_rows, a->dim, a->type);
     static_assert(FDGS_EMBEDDING_MAX_DIM / EmF32::full / 64 <= 65535, "column tiles in a grid's second dimension");
-    if (p.shares > 0x7fffffffLL) return FDGS_ETOOLARGE;
+    if (p.shares > 0x7fffffffLL || p.blocks > FDGS_MAX_GROUPS(EW_THREADS) || p.joins > FDGS_MAX_GROUPS(EW_THREADS)) return FDGS_ETOOLARGE;
     if (!a->workspace || a->workspace_bytes < p.bytes) return FDGS_EWORKSPACE;
     hipStream_t s = (hipStream_t)stream;
     char* ws = (char*)a->workspace;

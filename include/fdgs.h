@@ -557,7 +557,8 @@ int fdgs_moment8_pack(const fdgs_moment8_args* a, void* stream);
  * in an order that the ids alone decide: equal inputs give equal bits.
  * A token has no row - zeros in out, nothing in the gradient - when its id is negative or padding_id; an id of num_rows
  * or more gives a row of NaN, and nothing in the gradient.                                            */
-#define FDGS_EMBEDDING_MAX_TOKENS (1 << 30)          /* of the gradient; the lookup takes 2^31 - 1 */
+#define FDGS_EMBEDDING_MAX_TOKENS (1 << 30)          /* of the gradient; the lookup takes 2^31 - 1.  (In the gradient of rows of one
+                                                        element, rows and tokens are fewer than 2^31 together) */
 #define FDGS_EMBEDDING_MAX_DIM (1 << 22)
 #define FDGS_EMBEDDING_FEW 128                       /* so few tokens need no sort of their own: `sorted` is not used */
 typedef struct {

@@ -526,3 +526,30 @@ def test_views_that_are_still_to_be_negated():
         assert torch.equal(embedding(ids, x), x[ids].resolve_neg())
         assert torch.equal(embedding_grad(x[:4], ids, 6), embedding_grad(x[:4].resolve_neg().contiguous(), ids, 6))
     assert torch.equal(embedding(torch._neg_view(-ids), z.imag), z.imag[ids])
+
+
+def test_a_lookup_of_more_workgroups_than_a_launch_has():
+    """73 tokens of 7 float16 numbers to a workgroup: 2^24 workgroups of 256 threads are one launch too many.  17 GB of output."""
+    from fdgs.embedding import embedding
+    tokens, rows = 73 * (1 << 24) + 500, 1000
+    table = torch.randn(rows, 7, device="cuda").half()
+    ids = (torch.arange(tokens, dtype=torch.int32, device="cuda") * 7 + 3) % (rows + 1) - 1
+    y = embedding(ids, table, scale=0.5)
+    half = torch.cat([table * 0.5, torch.zeros_like(table[:1])])            # -1: the last row; exact
+    part = 1 << 26
+    for at in range(0, tokens, part):
+        assert torch.equal(y[at:at + part], half[ids[at:at + part].long()]), at
+
+
+def test_a_recorded_lookup_of_more_workgroups_than_a_launch_has():
+    """One token to a workgroup: the sort runs by itself, the lookup in two launches.  69 GB of output."""
+    from fdgs.embedding import embedding
+    tokens, rows, dim = (1 << 24) + 5, 500, 2056
+    table = torch.randn(rows, dim, device="cuda").bfloat16().requires_grad_(True)
+    ids = (torch.arange(tokens, device="cuda") * 7 + 3) % (rows + 1) - 1
+    y = embedding(ids, table).detach()
+    want = torch.cat([table.detach(), torch.zeros_like(table[:1])])
+    part = 1 << 20
+    for at in range(0, tokens, part):
+        assert torch.equal(y[at:at + part], want[ids[at:at + part]]), at
+    torch.cuda.empty_cache()

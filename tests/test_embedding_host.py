@@ -122,3 +122,11 @@ def test_rows_of_views_that_are_still_to_be_negated():
     assert z.conj().imag.is_neg()
     assert rows_layout(z.imag, 1) == (True, 1, 2) and rows_layout(z.conj().imag, 1) == (False, 1, 1)
     assert rows_layout(torch._neg_view(torch.zeros(3, 4)), 1) == (False, 4, 4)
+
+
+def test_gradients_that_no_grid_holds_are_refused():
+    """A launch has fewer than 2^32 threads: rows of one element, 128 rows and tokens to a workgroup of the join."""
+    for rows, tokens in (((1 << 31) - 1, 1), ((1 << 31) - 129, 129), ((1 << 31) - 1, 1 << 30)):
+        assert _bwd(num_rows=rows, num_tokens=tokens, dim=1) == -4
+    for rows, tokens, dim in (((1 << 31) - 200000, 129, 1), ((1 << 31) - 1, 1 << 30, 2)):
+        assert _bwd(num_rows=rows, num_tokens=tokens, dim=dim) == -3                    # as far as the workspace
