@@ -302,6 +302,8 @@ class TrainStep:
             vgrad = torch.zeros(n, 3, device=dev)
             if dp.is_dist():
                 gaussian_ids = {id(t) for t in self.g.parameters()} if hasattr(self.g, "parameters") else set()
+                if self.codebook is not None:       # whether or not the model counts it among its own
+                    gaussian_ids.add(id(self.codebook.table))
                 for p in self.params:
                     if p.requires_grad and p.grad is None and ("fine" in self.stage or id(p) in gaussian_ids):
                         p.grad = torch.zeros_like(p)

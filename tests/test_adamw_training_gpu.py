@@ -269,3 +269,30 @@ def test_lookup_gradient_and_step_together(bits):
     with pytest.raises(ValueError, match="f_dc"):
         step.densify(0.0, 1.0)
     assert math.isfinite(float(step(cams, iteration=2)))
+
+
+@pytest.mark.parametrize("stage", ["coarse", "fine"])
+def test_a_rank_without_views_exchanges_the_codebooks_gradient(stage, monkeypatch):
+    """The exchange adds up the gradients that there are: the same tensors have one on a rank that has views and on one that has none,
+    the codebook's table among them also where the model's parameters() does not name it."""
+    from fdgs import dp
+    from fdgs.embedding import FeatureCodebook
+    from fdgs.train_step import TrainStep
+    have = []
+    for views in (True, False):
+        g, deforms, cams, bg = _scene()
+        gen = torch.Generator().manual_seed(7)
+        g.feature_codebook = FeatureCodebook(0.1 * torch.randn(20, 16, 3, generator=gen), torch.randint(0, 20, (g._xyz.shape[0],), generator=gen)).cuda()
+        assert all(p is not g.feature_codebook.table for p in g.parameters())
+        step = TrainStep(g, deforms, bg, stage=stage)
+        seen = {}
+        with monkeypatch.context() as m:
+            m.setattr(dp, "is_dist", lambda: True)
+            m.setattr(dp, "all_reduce_", lambda *a, **k: None)
+            if not views:
+                m.setattr(dp, "shard_views", lambda v: [])
+            step(cams, before_optimizer_step=lambda s: seen.update(grads=[p.grad is not None for p in s.params],
+                                                                   table=g.feature_codebook.table.grad is not None))
+        assert seen["table"]
+        have.append(seen["grads"])
+    assert have[0] == have[1]
