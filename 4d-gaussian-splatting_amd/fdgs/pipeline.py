@@ -17,6 +17,7 @@ import torch
 
 from . import _lib, deformation as _deformation, rasterizer as _rasterizer
 from ._lib import lib, ptr
+from .embedding import FeatureCodebook
 
 
 def arena_layout(N, deform_numel):
@@ -64,9 +65,12 @@ class ViewPipeline:
         self._aside = None                       # (stream, event before the view, event after the work)
 
     # ------------------------------------------------------------------------------------------------------
+    def _has_codebook(self):
+        return isinstance(getattr(self.g, "feature_codebook", None), FeatureCodebook)
+
     def usable(self, stage):
         g = self.g
-        return (g.scaling_activation is torch.exp and g.opacity_activation is torch.sigmoid
+        return (not self._has_codebook() and g.scaling_activation is torch.exp and g.opacity_activation is torch.sigmoid
                 and g.rotation_activation is torch.nn.functional.normalize
                 and ("coarse" in stage or (self.net is not None
                                            and self.net.deformation_net.W == _deformation.KERNEL_WIDTH)))
@@ -193,6 +197,8 @@ class ViewPipeline:
         1 the view's range is added to set 0's - the running sum of the rank's earlier views - and that is handed
         over."""
         g = self.g
+        if self._has_codebook():
+            raise ValueError("a model with a feature_codebook goes through render(): the pipeline reads _features_dc and _features_rest")
         xyz = g._xyz.detach()
         dev = xyz.device
         N = xyz.shape[0]

@@ -130,3 +130,17 @@ def test_gradients_that_no_grid_holds_are_refused():
         assert _bwd(num_rows=rows, num_tokens=tokens, dim=1) == -4
     for rows, tokens, dim in (((1 << 31) - 200000, 129, 1), ((1 << 31) - 1, 1 << 30, 2)):
         assert _bwd(num_rows=rows, num_tokens=tokens, dim=dim) == -3                    # as far as the workspace
+
+
+def test_pipeline_refuses_a_codebook():
+    """It reads _features_dc and _features_rest, which a model with a codebook may have beside it."""
+    from types import SimpleNamespace
+    from fdgs.embedding import FeatureCodebook
+    from fdgs.pipeline import ViewPipeline
+    model = SimpleNamespace(scaling_activation=torch.exp, opacity_activation=torch.sigmoid, rotation_activation=torch.nn.functional.normalize)
+    pipe = ViewPipeline(model, None, torch.zeros(3))
+    assert pipe.usable("coarse")
+    model.feature_codebook = FeatureCodebook(torch.zeros(3, 16, 3), torch.tensor([0, 2]))
+    assert not pipe.usable("coarse")
+    with pytest.raises(ValueError, match="feature_codebook"):
+        pipe.run(None, None, 1.0, "coarse")
