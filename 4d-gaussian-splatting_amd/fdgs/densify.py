@@ -14,6 +14,7 @@ from torch import nn
 
 from . import _lib
 from ._lib import lib, ptr
+from .embedding import FeatureCodebook
 
 PARAM_NAMES = ("xyz", "f_dc", "f_rest", "opacity", "scaling", "rotation")
 _ATTR = {"xyz": "_xyz", "f_dc": "_features_dc", "f_rest": "_features_rest", "opacity": "_opacity",
@@ -160,6 +161,8 @@ class GaussianSurgery:
         """Rebuilds every per-Gaussian array for the classes `cls`.  noise: [2 S, 3] unit normal samples for the
         split children (drawn here when None).  reset_stats: the statistics restart from zero at the new size
         (densification, fdgs_trainer.py:468-475); otherwise they are carried row by row (pruning, :381-386)."""
+        if isinstance(getattr(self.gaussians, "feature_codebook", None), FeatureCodebook):
+            raise ValueError("the surgery moves f_dc and f_rest, not the ids of a feature_codebook")
         groups = self._groups()
         src, rows_after, survivors, clones, splits = surgery_plan(cls)
         old = {n: groups[n]["params"][0].detach() for n in PARAM_NAMES}

@@ -144,3 +144,15 @@ def test_pipeline_refuses_a_codebook():
     assert not pipe.usable("coarse")
     with pytest.raises(ValueError, match="feature_codebook"):
         pipe.run(None, None, 1.0, "coarse")
+
+
+def test_surgery_refuses_a_codebook_beside_the_groups_that_it_moves():
+    """The ids would stay where they are while the Gaussians move."""
+    from types import SimpleNamespace
+    from fdgs.densify import PARAM_NAMES, GaussianSurgery
+    from fdgs.embedding import FeatureCodebook
+    model = SimpleNamespace(feature_codebook=FeatureCodebook(torch.zeros(3, 16, 3), torch.tensor([0, 2])))
+    groups = [{"name": k, "params": [torch.zeros(2, 3, requires_grad=True)]} for k in PARAM_NAMES]
+    surgery = GaussianSurgery(model, SimpleNamespace(param_groups=groups, state={}))
+    with pytest.raises(ValueError, match="f_dc and f_rest"):
+        surgery.apply_classes(torch.zeros(2, dtype=torch.uint8))
