@@ -710,3 +710,54 @@ def test_a_read_out_is_seen_by_saved_graphs():
         loss.backward()
     with torch.inference_mode():                             # tensors without a version
         assert (unpack8(pack8([torch.ones(8, device="cuda")], False))[0] == 1).all()
+
+
+def test_indexes_past_32_bits():
+    """A tensor of 2^32 + 1004 elements with 8-bit moments and a gradient in rows: blocks at both ends and on either side of the numbers
+    that 31 and 32 bits hold have the format's codes (whose random numbers depend on all of the index) and the formula's weights,
+    everything else stays; then the moments' conversions.  66 GB."""
+    from fdgs.adamw import Moment8, adamw_step, pack8, unpack8
+    f, b1, b2, lr, eps, t, key = np.float32, 0.9, 0.999, 1e-2, 1e-8, 3, 12345
+    rows = 1431656100
+    n = 3 * rows
+    assert n == (1 << 32) + 1004
+    windows = [(at, min(at + 512, n)) for at in (0, (1 << 31) - 256, (1 << 32) - 256, (1 << 32) + 768)]     # the last one's block is not whole
+    wide = torch.zeros(rows, 4, device="cuda")
+    rng = np.random.default_rng(0)
+    grads = []
+    for lo, hi in windows:                                   # written through their rows: column 3 lies between
+        x = rng.standard_normal(hi - lo).astype(f)
+        i = torch.arange(lo, hi, device="cuda")
+        wide.view(-1)[torch.div(i, 3, rounding_mode="floor") * 4 + i % 3] = torch.from_numpy(x).cuda()
+        grads.append(x)
+    p = torch.ones(rows, 3, device="cuda")
+    m, v = Moment8.zeros_like(p, True), Moment8.zeros_like(p, False)
+    adamw_step([p], [wide[:, :3]], [m], [v], steps=t, lr=lr, eps=eps, weight_decay=0.0, keys=[key])
+    del wide
+    count = 0
+    for (lo, hi), x in zip(windows, grads):
+        zero = np.zeros(hi - lo, f)
+        m1, v1 = ac.adamw32(x, zero, zero, b1, b2)
+        h = ac.hash32(np.arange(lo, hi), key)
+        for got, want in ((m, ac.encode(m1, h >> 16, True)), (v, ac.encode(v1, h & 0xFFFF, False))):
+            assert np.array_equal(got.codes.view(-1)[lo:hi].cpu().numpy(), want[0])
+            assert np.array_equal(got.exponents[lo // 256:-(-hi // 256)].cpu().numpy(), want[1])
+        count += int((ac.encode(v1, h & 0xFFFF, False)[0] != 0).sum())
+        denom = np.sqrt(v1) * f(1.0 / math.sqrt(1.0 - b2 ** t)) + f(eps)
+        want = np.ones_like(x) - (m1 * f(lr / (1.0 - b1 ** t))) / denom
+        assert np.array_equal(p.view(-1)[lo:hi].cpu().numpy().view(np.int32), want.view(np.int32))
+    chunks = lambda x: x.view(-1).split(1 << 28)             # noqa: E731
+    assert sum(int(c.count_nonzero()) for c in chunks(v.codes)) == count
+    assert sum(int((c != 1).sum()) for c in chunks(p)) <= count
+    del p
+    x, = unpack8([m])
+    for lo, hi in windows:
+        part = Moment8(m.codes.view(-1)[lo:hi], m.exponents[lo // 256:-(-hi // 256)], True)
+        assert torch.equal(x.view(-1)[lo:hi], unpack8([part])[0])
+    assert sum(int(c.count_nonzero()) for c in chunks(x)) == sum(int((c & 127).count_nonzero()) for c in chunks(m.codes))
+    x.mul_(1.03)                                             # off the grid: the random numbers count
+    again, = pack8([x], True, [key])
+    for lo, hi in windows:
+        codes, exps = ac.encode(x.view(-1)[lo:hi].cpu().numpy(), ac.hash32(np.arange(lo, hi), key) >> 16, True)
+        assert np.array_equal(again.codes.view(-1)[lo:hi].cpu().numpy(), codes)
+        assert np.array_equal(again.exponents[lo // 256:-(-hi // 256)].cpu().numpy(), exps)

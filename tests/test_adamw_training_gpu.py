@@ -296,3 +296,51 @@ def test_a_rank_without_views_exchanges_the_codebooks_gradient(stage, monkeypatc
         assert seen["table"]
         have.append(seen["grads"])
     assert have[0] == have[1]
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_surgery_moves_every_moment_with_its_gaussian(bits):
+    """Known classes: the moments of those that stay follow them in their old order, clones and children begin with none.  In 8 bits the
+    new blocks of 256 are the format's, to the nearest, of the old values."""
+    from fdgs import _lib
+    from fdgs.train_step import TrainStep
+    g, deforms, cams, bg = _scene(n=1501)
+    step = TrainStep(g, deforms, bg, adamw={"state_bits": bits})
+    for k in range(2):
+        step(cams, iteration=k + 1)
+    names = ("xyz", "f_dc", "f_rest", "opacity", "scaling", "rotation")
+
+    def moments():
+        params = {gr["name"]: gr["params"][0] for gr in step.optimizer.param_groups if gr["name"] in names}
+        return {k: [m.cpu().numpy() for m in step.optimizer.moments(params[k])] for k in names}
+
+    def stored(x, signed):
+        if bits == 32:
+            return x
+        flat = np.ascontiguousarray(x).reshape(-1)
+        return ac.decode(*ac.encode(flat, 0x8000, signed), signed).reshape(x.shape)
+
+    gen = torch.Generator().manual_seed(0)
+    for kind in ("densify", "prune"):
+        n = g._xyz.shape[0]
+        before, steps = moments(), step.optimizer.state[g._xyz]["step"]
+        draw = torch.rand(n, generator=gen)
+        if kind == "densify":
+            cls = torch.full((n,), _lib.CLS_KEEP, dtype=torch.uint8)
+            cls[draw < 0.3], cls[draw < 0.2], cls[draw < 0.1] = _lib.CLS_CLONE, _lib.CLS_SPLIT, _lib.CLS_DROP
+            stay = (cls == _lib.CLS_KEEP) | (cls == _lib.CLS_CLONE)
+            out = step.surgery().apply_classes(cls.cuda())
+            assert out["clones"] == int((cls == _lib.CLS_CLONE).sum()) > 0 and out["splits"] == int((cls == _lib.CLS_SPLIT).sum()) > 0
+        else:
+            stay = draw > 0.25
+            out = step.surgery().prune_points((~stay).cuda())
+        rows = g._xyz.shape[0]
+        assert out["survivors"] == int(stay.sum()) < n and out["rows"] == rows
+        after = moments()
+        for k in names:
+            for old, new, signed in zip(before[k], after[k], (True, False)):
+                assert (old != 0).any()
+                want = np.zeros((rows, *old.shape[1:]), np.float32)
+                want[:out["survivors"]] = old[stay.numpy()]
+                assert new.shape == want.shape and np.array_equal(new, stored(want, signed)), (kind, k, signed)
+        assert step.optimizer.state[g._xyz]["step"] == steps

@@ -553,3 +553,53 @@ def test_a_recorded_lookup_of_more_workgroups_than_a_launch_has():
     for at in range(0, tokens, part):
         assert torch.equal(y[at:at + part], want[ids[at:at + part]]), at
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("dim, dtype", [(1, torch.float32), (3, torch.bfloat16), (8, torch.float32), (48, torch.float32), (100, torch.float16),
+                                        (1030, torch.float32), (2048, torch.bfloat16)])
+@pytest.mark.parametrize("rows, where", [(1, "one"), (5000, "one"), (5000, "two"), (5000, "three"), (40, "even"), (5000, "half")])
+def test_sums_of_rows_with_very_many_tokens_are_exact(dim, dtype, rows, where):
+    """Gradients of whole numbers, the sums of which float32 holds whatever the order: a token that is left out, taken twice or added
+    to another row shows.  Rows that begin and end inside workgroups of the walk and hold whole ones between."""
+    from fdgs.embedding import embedding_grad
+    tokens = 2000000 // max(dim, 20)
+    gen = torch.Generator().manual_seed(dim + rows)
+    ids = torch.randint(0, rows, (tokens,), generator=gen)
+    if where == "one":
+        ids[:] = rows // 2
+    elif where == "two":
+        ids = rows // 2 + (torch.rand(tokens, generator=gen) < 0.3).long()
+    elif where == "three":
+        ids[torch.rand(tokens, generator=gen) < 0.9] = rows // 3
+        ids[torch.rand(tokens, generator=gen) < 0.5] = rows // 2
+    elif where == "half":
+        ids[torch.rand(tokens, generator=gen) < 0.5] = rows - 1
+        ids[torch.rand(tokens, generator=gen) < 0.1] = -1
+    gy = torch.randint(1, 8, (tokens, dim), generator=gen).to(dtype)         # none of them zero: every token counts
+    got = embedding_grad(gy.cuda(), ids.int().cuda(), rows, scale=0.25).cpu()
+    ok = ids >= 0
+    want = torch.zeros(rows, dim, dtype=torch.float64).index_add_(0, ids[ok], gy[ok].double())
+    assert want.max() < 2 ** 24 and torch.equal(got, (0.25 * want).float().to(dtype))
+
+
+@pytest.mark.parametrize("tokens", [2097152, 2097153, 2100000, 5000000])
+@pytest.mark.parametrize("rows, dim", [(300, 1), (511, 3), (70000, 1), (600000, 2)])
+def test_sorts_whose_workgroups_take_several_tiles(tokens, rows, dim):
+    """More than 1024 tiles of 2048 tokens: a workgroup of the sort goes on with a second and a third.  One to three digits, ids that are
+    skewed, partly absent; by itself and beside the lookup.  Whole numbers: exact in any order."""
+    from fdgs.embedding import embedding, embedding_grad
+    gen = torch.Generator(device="cuda").manual_seed(tokens + rows)
+    ids = (rows * torch.rand(tokens, generator=gen, device="cuda", dtype=torch.float64) ** 4).long()
+    ids[torch.rand(tokens, generator=gen, device="cuda") < 0.05] = -1
+    ids[torch.rand(tokens, generator=gen, device="cuda") < 0.02] = rows
+    ids[-3:] = torch.tensor([rows - 1, 0, rows - 1], device="cuda")
+    gy = torch.randint(-8, 9, (tokens, dim), generator=gen, device="cuda").float()
+    ok = (ids >= 0) & (ids < rows)
+    here = ids[ok].cpu()                                     # (the GPU's own sums wait for one another at a frequent row)
+    want = torch.stack([torch.bincount(here, x, rows) for x in gy[ok].double().cpu().t()], 1).float().cuda()
+    assert torch.equal(embedding_grad(gy, ids, rows), want)
+    table = torch.randn(rows, dim, generator=gen, device="cuda", requires_grad=True)
+    y = embedding(ids.int(), table)
+    assert torch.equal(torch.autograd.grad(y, table, gy)[0], want)
+    y = y.detach()
+    assert torch.equal(y[ok], table.detach()[ids[ok]]) and (y[ids < 0] == 0).all() and y[ids == rows].isnan().all()
