@@ -7,7 +7,8 @@
 //   first moment:  sign and code 1..127,            base = max(0, 8 (E + 1) - 127)         15.75 powers of two
 // Code 0 is zero.  Because the grid is a cut of the float32 pattern, its points do not move when a block's exponent
 // does: a value that is stored, read and stored again stays what it is.  The largest code stands for 2^(E + 1 - 127),
-// so a largest value that rounds up has a place.
+// so a largest value that rounds up has a place: up to E = 253.  With E = 254 that place is infinity's, and a value above
+// 1.875 times 2^127 may be read back as such; squares of gradients come there from 10^19 on.
 //
 // The cut is stochastic (a 16-bit random number is added just below the last kept bit).  With beta2 = 0.999 a step
 // moves v by a thousandth of g^2 - v while the grid's points are an eighth to a sixteenth of v apart: a cut to the

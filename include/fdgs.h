@@ -488,7 +488,8 @@ int fdgs_adam_step(const fdgs_adam_args* a, void* stream);
  * FDGS_MOMENT8_BLOCK consecutive elements.  With E the block's exponent byte (the biased float32 exponent of its largest
  * magnitude) a code c > 0 stands for the float32 with bit pattern (c + max(0, 8 (E+1) - 255)) << 20 in the second
  * moment, for sign (bit 7) and ((c & 127) + max(0, 8 (E+1) - 127)) << 20 in the first; c = 0 is zero, E = 255 makes the
- * whole block NaN (it was given a value that is not finite).  All zeros to begin with.  Values are rounded
+ * whole block NaN (it was given a value that is not finite).  (In a block with E = 254 the code of 2^128, which values above
+ * 1.875 times 2^127 may round up to, is an infinity.)  All zeros to begin with.  Values are rounded
  * stochastically, by 16 bits each of a hash of the element's index and `round_key`: give every tensor and step a key of
  * its own, and every replica the same one.  A second moment that is not zero is never rounded to zero.
  *

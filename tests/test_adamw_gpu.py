@@ -761,3 +761,17 @@ def test_indexes_past_32_bits():
         codes, exps = ac.encode(x.view(-1)[lo:hi].cpu().numpy(), ac.hash32(np.arange(lo, hi), key) >> 16, True)
         assert np.array_equal(again.codes.view(-1)[lo:hi].cpu().numpy(), codes)
         assert np.array_equal(again.exponents[lo // 256:-(-hi // 256)].cpu().numpy(), exps)
+
+
+@pytest.mark.parametrize("signed", [True, False])
+def test_the_largest_code_of_a_block(signed):
+    """It stands for the power of two above the block's largest value: infinity where float32 has no such power."""
+    from fdgs.adamw import pack8, unpack8
+    top = np.float32(2.0 - 2.0 ** -23)
+    for e in (-126, 0, 126, 127):
+        x = torch.full((300,), float(np.ldexp(top, e)), device="cuda")
+        got, = unpack8(pack8([x], signed))
+        assert (got == 2.0 ** (e + 1)).all() if e < 127 else got.isinf().all()
+        x[:256] = float(np.ldexp(np.float32(1.875), e))          # on the grid
+        got, = unpack8(pack8([x], signed, [7]))
+        assert torch.equal(got[:256], x[:256])

@@ -603,3 +603,38 @@ def test_sorts_whose_workgroups_take_several_tiles(tokens, rows, dim):
     assert torch.equal(torch.autograd.grad(y, table, gy)[0], want)
     y = y.detach()
     assert torch.equal(y[ok], table.detach()[ids[ok]]) and (y[ids < 0] == 0).all() and y[ids == rows].isnan().all()
+
+
+def test_as_many_tokens_as_a_gradient_takes():
+    """2^30 tokens of one and the same gradient, every row's count known beforehand: sums exact below 2^24.  30 GB."""
+    from fdgs.embedding import embedding_grad
+    tokens, rows, often = 1 << 30, 1009, 1 << 23
+    ids = torch.empty(tokens, dtype=torch.int32, device="cuda")
+    part = 1 << 27
+    for at in range(0, tokens, part):
+        ids[at:at + part] = (torch.arange(at, at + part, device="cuda") * 787 % rows).int()
+    count = torch.full((rows,), tokens // rows, dtype=torch.int64)
+    count[torch.arange(tokens % rows) * 787 % rows] += 1
+    place = torch.arange(often, device="cuda") * 127 + 5         # these change to one row
+    count -= torch.bincount(ids[place].cpu(), minlength=rows)
+    ids[place] = 500
+    count[500] += often
+    assert int(count.sum()) == tokens and int(count.max()) < 1 << 24
+    got = embedding_grad(torch.ones((), device="cuda").expand(tokens, 1), ids, rows)
+    assert torch.equal(got[:, 0].cpu(), count.float())
+
+
+def test_a_table_of_nearly_2_to_the_31_rows():
+    """Items past 2^31 in the walk, keys of 31 bits."""
+    from fdgs.embedding import embedding, embedding_grad
+    rows = (1 << 31) - 200000
+    ids = torch.tensor([rows - 1, 0, rows - 1, 1 << 30, -1, rows, rows - 2, 0, 0] * 20, device="cuda")
+    gy = torch.arange(1, 181, device="cuda").half()[:, None]
+    got = embedding_grad(gy, ids, rows)
+    where = torch.tensor([0, 1 << 30, rows - 2, rows - 1], device="cuda")
+    want = torch.stack([gy[ids == r].double().sum() for r in where]).half()
+    assert torch.equal(got[where, 0], want)
+    assert sum(int(c.count_nonzero()) for c in got.view(-1).split(1 << 28)) == 4
+    y = embedding(ids, got)
+    assert torch.equal(y[(ids >= 0) & (ids < rows)], got[ids[(ids >= 0) & (ids < rows)]]) and (y[ids < 0] == 0).all() and y[ids == rows].isnan().all()
+    torch.cuda.empty_cache()
