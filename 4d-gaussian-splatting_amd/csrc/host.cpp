@@ -408,13 +408,13 @@ int type_of(const Tensor& t, const char* what) {
 Tensor ids_of(const Tensor& ids, const at::Device& device) {
     if (ids.scalar_type() != at::kInt && ids.scalar_type() != at::kLong) value_error("ids are int32 or int64");
     if (ids.device() != device) value_error("ids and table have to be on one device");
-    return ids.resolve_neg().contiguous();
+    return (ids.is_neg() ? ids.resolve_neg() : ids).contiguous();
 }
 
 // t [lead..., row...] with rows that are contiguous runs a constant, not negative distance apart: t itself where it is
 // laid out so, else a copy.
 Tensor rows_of(const Tensor& t0, int64_t lead, int64_t& width, int64_t& stride) {
-    const Tensor t = t0.resolve_neg();
+    const Tensor t = t0.is_neg() ? t0.resolve_neg() : t0;
     width = 1;
     for (int64_t d = lead; d < t.dim(); ++d) width *= t.size(d);
     stride = width;
@@ -619,7 +619,7 @@ PyObject* embedding(PyObject* a) {
     const Tensor &ids = tensor(io, "ids"), &table = tensor(to, "the table");
     if (table.dim() < 2) value_error("the table is [rows, ...] in float32, bfloat16 or float16");
     type_of(table, "the table");
-    no_tangent(table, "the table");
+    if (!table.is_cuda()) no_tangent(table, "the table");                // (lookup() looks at the others)
     on_gpu(table);
     const int64_t padding = padding_of(po);
     Tensor out;
