@@ -16,8 +16,8 @@
 #include <type_traits>
 
 #define AW_MAX 40                                // tensors whose records fill 4 KB of kernel arguments
-// A wave has one block (with two the step over 2,000,000 Gaussians with 8-bit moments, and their read-out, takes 527 us, not 513),
-// a workgroup eight of them (97 bfloat16 tensors: 194 us, 202 with four, 193 with sixteen, with which 8-bit moments lose 3 %).
+// A wave has one block (with two the step over 2,000,000 Gaussians with 8-bit moments, and their read-out, takes 3 % longer),
+// a workgroup eight of them (97 bfloat16 tensors: 184 us, 192 with four, 185 with sixteen, with which 8-bit moments lose 4 to 10 %).
 #define AW_THREADS 512
 #define AW_PER_GROUP (AW_THREADS / 64 * M8_BLOCK)
 
@@ -51,7 +51,7 @@ __device__ __forceinline__ int aw_find(Ints start, int num, int b) {
 }
 
 // Where the records of a launch lie: in its arguments, or (more tensors than these hold) the last ones there and the others in a
-// table in device memory that small launches before it have filled from theirs, 1.5 to 2.5 us each.  60 float32 tensors of 5,000
+// table in device memory that small launches before it have filled from theirs, 1.5 us each, the first of them up to 5.  60 float32 tensors of 5,000
 // elements: 6.5 us (8.4 in two launches over arguments), 100: 9.4 (11.1 with all records in the table); 211 bfloat16 tensors
 // with 8-bit moments and their read-out 181 (250 in six launches and five).
 template <class Record, int MAX>
@@ -211,7 +211,7 @@ __device__ __forceinline__ void aw_join4(const aw_h4& h, const aw_h4& l, float* 
 __device__ __forceinline__ float aw_bf16(uint16_t h) { return __uint_as_float((uint32_t)h << 16); }
 
 // The update, every operation correctly rounded.  (With the chip's root and reciprocal, 1.6 units of 2^-24 off each, the step over
-// 2,000,000 Gaussians with 8-bit moments and their read-out takes 512 us, not 524; which form the moments have is no reason for
+// 2,000,000 Gaussians with 8-bit moments and their read-out takes 512 us, not 522; which form the moments have is no reason for
 // another rounding.)
 __device__ __forceinline__ float aw_update(float w, float m, float v, const AwStep& k, const AwTensor& t) {
 #pragma clang fp contract(off)

@@ -92,7 +92,7 @@ struct EmFwd {
 // A workgroup has whole tokens, as many as make up to 512 or 1024 vectors (or, of a longer row, so many of one token): a
 // thread has up to two or four vectors, all of whose ids and then all of whose rows are asked for before the first is used.
 // Bound by the output's lines and, where the table does not fit an XCD's 4 MB of L2, by the rows that come from behind it:
-// 300,000 x 48 floats 12.6 us (4.8 TB/s), 2,000,000 x 48 from 65,536 rows 120 us, from 8,192 rows 66 us (5.8 TB/s).
+// 300,000 x 48 floats 11.9 us (5.1 TB/s), 2,000,000 x 48 from 65,536 rows 120 us, from 8,192 rows 66 us (5.8 TB/s).
 template <class T, int VEC>
 __device__ __forceinline__ void ef_group(const EmFwd& a, int group, int tile, uint32_t thread) {
     typedef EmVec<T, VEC> Vec;
@@ -1161,7 +1161,8 @@ extern "C" int fdgs_embedding_fwd(const fdgs_embedding_fwd_args* a, void* stream
     k.nv = (k.dim + f.vec - 1) / f.vec;
     k.by_nv = em_div_of((uint32_t)k.nv);
     // Four vectors a thread where rows come from behind L2 for long (2,000,000 x 48 floats from 12.6 MB of table, with the sort:
-    // 153 us, 160 with two), else two (300,000 x 48 floats 12.5 us, 14 with four, 17 with eight; one token 2.5, 2.7, 3.2).
+    // 153 us, 160 with two), else two (the kernel for 300,000 x 48 floats, launched by itself, 12.4 us, 14 with four, 17 with eight;
+    // for one token 2.1, 2.7, 3.2).
     const long long size = a->type == FDGS_TYPE_F32 ? 4 : 2, row = (long long)k.dim * size;
     k.vectors = row * k.rows > (4 << 20) && row * k.tokens > (64 << 20) ? EF_VECTORS : EF_VECTORS / 2;
     k.per_group = k.nv < k.vectors ? k.vectors / k.nv : 1;

@@ -52,11 +52,12 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, steps, lr, betas=(0.9, 0
                residuals=None, keys=None):
     """One AdamW step over lists of tensors, in place: params, their moments (contiguous float32 tensors, or Moment8),
     and for bfloat16 params `residuals` (int16), each of its parameter's shape or flat.  grads: the parameters' type and shape;
-    contiguous, or column slices of wider row-major arrays (read in place), anything else is copied.  steps (1-based), lr and weight_decay: one value, or
-    one for each tensor.  keys: for 8-bit moments, 32-bit numbers, one for each tensor, others at every step.
-    All tensors are on one GPU, have one type, and the step runs on its current stream; no tensor that it writes overlaps another one.  Tensors
-    without elements are passed over.  The call reads steps, lr and keys on the host: a captured graph would replay
-    the ones it was captured with, so a stream that is being captured is refused."""
+    contiguous, or column slices of wider row-major arrays (read in place), anything else is copied.  steps (1-based), lr
+    and weight_decay: one value, or one for each tensor.  keys: for 8-bit moments, 32-bit numbers, one for each tensor,
+    others at every step.  All tensors are on one GPU, have one type, and the step runs on its current stream; no tensor
+    that it writes overlaps another one.  Tensors without elements are passed over.  The call reads steps, lr and keys on
+    the host: a captured graph would replay the ones it was captured with, so a stream that is being captured is
+    refused."""
     _host.adamw_step(params, grads, exp_avgs, exp_avg_sqs, residuals, steps, lr, weight_decay, keys, Moment8, *betas, eps)
     GENERATION[0] += 1
 
