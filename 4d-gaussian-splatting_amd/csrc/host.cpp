@@ -4,6 +4,7 @@
 // costs 0.1 to 0.4 us, 5 to 7 us a tensor, several times what the GPU needs for the step; here the whole list costs
 // 0.1 to 0.2 us a tensor.  Every check raises the Python exception that a caller sees.
 // The lookup of one token takes the GPU 4 us; its checks, output and call take 12 from Python, its training pass 130.
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -683,6 +684,8 @@ PyObject* guarded(PyObject*, PyObject* args) {
     } catch (const Raised&) {
     } catch (const Refused& r) {
         PyErr_SetString(r.type, r.what());
+    } catch (python_error& e) {                      // out of a hook that autograd has called: it stays what it is
+        e.restore();
     } catch (const std::bad_alloc&) {
         PyErr_NoMemory();
     } catch (const c10::Error& e) {

@@ -17,8 +17,9 @@ def embedding(ids, table, scale=1.0, padding_id=None):
     table is read in place) -> [*ids.shape, *table.shape[1:]] in the table's type, rounded once.  Negative ids and
     `padding_id` give zeros and take no part in the gradient; an id of V or more - an error that only the GPU sees -
     gives a row of NaN.  The gradient of the table is dense, with the table's shape and type, and the same bits for the
-    same inputs; it can be differentiated again (in reverse: a table with a forward-mode tangent is refused).  A call that is recorded for a gradient also sorts its tokens, which the
-    backward pass needs (8 bytes a token until then); under torch.no_grad() it does not."""
+    same inputs; it can be differentiated again, in reverse (a table with a forward-mode tangent is refused).  A call that
+    is recorded for a gradient also sorts its tokens, which the backward pass needs (8 bytes a token until then); under
+    torch.no_grad() it does not."""
     return _host.embedding(ids, table, scale, padding_id)
 
 

@@ -638,3 +638,37 @@ def test_a_table_of_nearly_2_to_the_31_rows():
     y = embedding(ids, got)
     assert torch.equal(y[(ids >= 0) & (ids < rows)], got[ids[(ids >= 0) & (ids < rows)]]) and (y[ids < 0] == 0).all() and y[ids == rows].isnan().all()
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("tokens", [20, 500, 20000])
+def test_what_is_saved_may_be_kept_elsewhere_or_made_again(tokens):
+    """Under saved-tensor hooks and activation checkpointing (whose recomputation ends by an exception out of such a hook)."""
+    from fdgs.embedding import embedding
+    from torch.utils.checkpoint import checkpoint
+    ids = torch.randint(-1, 90, (tokens,), device="cuda")
+    table = torch.randn(90, 12, device="cuda", requires_grad=True)
+    gy = torch.randn(tokens, 12, device="cuda")
+    want, = torch.autograd.grad(embedding(ids, table), table, gy)
+    for pinned in (False, True):
+        with torch.autograd.graph.save_on_cpu(pin_memory=pinned):
+            y = embedding(ids, table)
+        assert torch.equal(torch.autograd.grad(y, table, gy)[0], want)
+    for reentrant in (False, True):
+        table.grad = None
+        (0.5 * checkpoint(lambda t: 2 * embedding(ids, t), table, use_reentrant=reentrant)).backward(gy)
+        assert torch.equal(table.grad, want)
+
+
+def test_an_exception_out_of_a_hook_stays_what_it_is():
+    from fdgs.embedding import embedding
+
+    class Stop(Exception):
+        pass
+
+    def pack(x):
+        raise Stop(tuple(x.shape))
+    ids, table = torch.tensor([1, 0, 1], device="cuda"), torch.randn(2, 8, device="cuda", requires_grad=True)
+    with pytest.raises(Stop, match="(3,)"):
+        with torch.autograd.graph.saved_tensors_hooks(pack, lambda x: x):
+            embedding(ids, table)
+    assert embedding(ids, table).shape == (3, 8)
