@@ -213,9 +213,10 @@ void launch(const char* name, int (*fn)(const Args*, void*), const Args& a, cons
         if (profiled) r = PyObject_CallMethod(library.module, "call_address", "sK", name, (unsigned long long)(uintptr_t)&a);
         const bool failed = profiled && !r;
         Py_XDECREF(r);
-        if (failed) PyErr_Clear();
+        python_error raised;
+        if (failed) raised.persist();
         PyGILState_Release(gil);
-        if (failed) throw std::runtime_error(std::string(name) + " failed in its profiled call");
+        if (failed) throw std::move(raised);
         if (profiled) return;
     }
     const int rc = fn(&a, (void*)c10::hip::getCurrentHIPStream(device.index()).stream());

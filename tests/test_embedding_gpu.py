@@ -672,3 +672,19 @@ def test_an_exception_out_of_a_hook_stays_what_it_is():
         with torch.autograd.graph.saved_tensors_hooks(pack, lambda x: x):
             embedding(ids, table)
     assert embedding(ids, table).shape == (3, 8)
+
+
+def test_an_exception_in_a_profiled_call_stays_what_it_is():
+    from fdgs import _lib
+    from fdgs.embedding import embedding
+    ids, table = torch.tensor([1, 0, 1], device="cuda"), torch.randn(2, 8, device="cuda", requires_grad=True)
+    y = embedding(ids, table)
+    _lib.PROFILE = ()                                        # not a dict
+    try:
+        for call in (lambda: embedding(ids, table), lambda: y.sum().backward()):
+            with pytest.raises(AttributeError, match="setdefault"):
+                call()
+    finally:
+        _lib.PROFILE = None
+    embedding(ids, table).sum().backward()
+    assert table.grad.sum() == 24
