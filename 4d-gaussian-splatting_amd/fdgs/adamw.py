@@ -106,7 +106,7 @@ class FusedAdamW:
     state[p]["residual"] beside them.  seed: of the 8-bit moments' rounding; replicas of a model have to have the same one
     (and the same order of parameters) to stay the same.  state_dict() holds tensors only, with the keys of
     torch.optim.AdamW where moments are in 32 bits; load_state_dict() takes a state in either width and converts it, also one
-    of torch.optim.Adam or FusedAdam."""
+    of torch.optim.Adam (without weight decay, which means another thing there) or FusedAdam."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, seed=0):
         if state_bits not in (8, 32):
@@ -260,6 +260,8 @@ class FusedAdamW:
             for i, p in zip(saved["params"], g["params"]):
                 by_index[int(i)] = p
         self._check_groups(merged)
+        if any(saved.get("weight_decay") and saved.get("decoupled_weight_decay") is False for saved in groups):
+            raise ValueError("the loaded state's weight decay is part of the gradient (torch.optim.Adam's), this optimizer's is not")
         state = {by_index[int(i)]: self._loaded(by_index[int(i)], st) for i, st in sd["state"].items()}
         for g, m in zip(self.param_groups, merged):
             g.update(m)

@@ -161,3 +161,17 @@ def test_steps_and_conversions_that_no_grid_holds_are_refused():
             for name in ("fdgs_moment8_pack", "fdgs_moment8_unpack"):
                 recs = (_records.Moment8Tensor * n)(*[_records.Moment8Tensor(codes=64, exponents=64, value=64, numel=k) for k in sizes])
                 assert getattr(lib, name)(C.byref(_records.Moment8Args(n, 0, 1, 0, C.cast(recs, C.c_char_p))), None) == -4
+
+
+def test_a_weight_decay_of_another_kind_is_not_taken_over():
+    """Adam adds it to the gradient, AdamW takes it off the weight: the number means another step."""
+    from fdgs.adamw import FusedAdamW
+    p = torch.zeros(4, requires_grad=True)
+    opt = FusedAdamW([p], weight_decay=0.3)
+    with pytest.raises(ValueError, match="part of the gradient"):
+        opt.load_state_dict(torch.optim.Adam([p], weight_decay=0.1).state_dict())
+    assert opt.param_groups[0]["weight_decay"] == 0.3
+    opt.load_state_dict(torch.optim.AdamW([p], weight_decay=0.2).state_dict())
+    assert opt.param_groups[0]["weight_decay"] == 0.2
+    opt.load_state_dict(torch.optim.Adam([p]).state_dict())
+    assert opt.param_groups[0]["weight_decay"] == 0 and opt.param_groups[0]["decoupled_weight_decay"]
